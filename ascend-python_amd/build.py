@@ -3,9 +3,9 @@
 1. Every ``csrc/**/*.hip`` file outside ``csrc/calib`` is compiled for gfx950
    with hipcc and linked into ``op_plugin_amd/libqk_hip.so`` -- the C ABI of
    ``include/qk_abi.h``.
-2. ``csrc/ops/npu_quant_ops.cpp`` (torch.ops.npu.* registration) is compiled
-   with the host C++ compiler against torch's headers and linked against
-   ``libqk_hip.so`` into ``op_plugin_amd/_npu_ops.so``.
+2. ``csrc/ops/*.cpp`` (torch.ops.npu.* registration) are compiled with the host
+   C++ compiler against torch's headers and linked against ``libqk_hip.so``
+   into ``op_plugin_amd/_npu_ops.so``.
 3. ``csrc/calib/calibrate.hip`` (roofline calibration kernels for
    ``bench.py --calibrate``; not part of the op path) becomes
    ``op_plugin_amd/libqk_calib.so``.
@@ -82,12 +82,16 @@ def build_ops(verbose: bool = False) -> str:
                                                                  f"-I{sysconfig.get_paths()['include']}"]
     out = os.path.join(PKG, "_npu_ops.so")
     tmp = out + ".tmp"
-    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_npu_ops",
-           "-fvisibility=hidden", *incs, os.path.join(CSRC, "ops", "npu_quant_ops.cpp"),
-           "-o", tmp, f"-L{PKG}", "-lqk_hip", f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch",
-           "-ltorch_cpu", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
-    _run(cmd, verbose)
+    srcs = sorted(glob.glob(os.path.join(CSRC, "ops", "*.cpp")))
+    objs = [os.path.join(OBJ, "ops_" + os.path.basename(s) + ".o") for s in srcs]
+    compile_cmd = ["g++", "-std=c++17", "-O2", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+                   "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_npu_ops",
+                   "-fvisibility=hidden", *incs, "-c"]
+    with cf.ThreadPoolExecutor(max_workers=len(srcs)) as ex:
+        for f in [ex.submit(_run, [*compile_cmd, s, "-o", o], verbose) for s, o in zip(srcs, objs)]:
+            f.result()
+    _run(["g++", "-shared", *objs, "-o", tmp, f"-L{PKG}", "-lqk_hip", f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch",
+          "-ltorch_cpu", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"], verbose)
     os.replace(tmp, out)
     return out
 

@@ -226,6 +226,16 @@ int check_workspace(const char* op, size_t need, const void* workspace, size_t w
 
 }  // namespace
 
+namespace qk {
+
+void abi_begin() { g_last_error.clear(); }
+int abi_error(int code, const char* message) {
+    g_last_error = message;
+    return code;
+}
+
+}  // namespace qk
+
 extern "C" {
 
 const char* qk_last_error(void) { return g_last_error.c_str(); }

@@ -28,6 +28,18 @@ Importing this package loads ``_npu_ops.so``, which registers
 * ``torch.ops.npu.npu_quant_matmul_swiglu_quant(x1, x2, scale, *, pertoken_scale=None, output_dtype=None) -> (q,
   scale)``: the same followed by npu_dynamic_quant of h, bit for bit; the GEMM's epilogue stores each row's
   partial absmax, so the quantizer reads h once with no row reduction
+* attention over a paged key-value cache (index tensors are int32 on the device):
+  ``torch.ops.npu.npu_paged_attention(query, key_cache, value_cache, block_table, context_lens, *, key_scale=None,
+  value_scale=None, scale=None, window=0, sinks=0) -> (out, lse)`` (one new token per sequence),
+  ``torch.ops.npu.npu_prompt_attention(query, key, value, cu_seqlens_q, *, cu_seqlens_k=None, block_table=None,
+  context_lens=None, key_scale=None, value_scale=None, scale=None, window=0, sinks=0) -> (out, lse)`` (ragged prompts or
+  prompt chunks, causal, keys contiguous or paged)
+* ``torch.ops.npu.npu_mrope(positions, query, key, cos_sin_cache, *, mrope_section=None, rotary_mode="half") -> (query,
+  key)`` and ``torch.ops.npu.npu_mrope_scatter_kv(positions, query, key, value, cos_sin_cache, key_cache, value_cache,
+  slot_mapping, *, key_scale=None, value_scale=None, mrope_section=None, rotary_mode="half") -> query``: rotary
+  positions of one to four axes, alone or with the write into the cache (int8 with scales per token and head)
+* the cache's pages: ``npu_kv_extend``, ``npu_kv_fork``, ``npu_kv_free``, ``npu_kv_copy_pages``, ``npu_kv_compact``
+  (``op_plugin_amd.kv_cache.PagedKVCache`` holds their state)
 
 and exposes the same callables here, so code written as
 ``torch_npu.npu_quant_matmul(...)`` runs as ``op_plugin_amd.npu_quant_matmul(...)``
@@ -70,6 +82,15 @@ npu_rms_norm_dynamic_quant = torch.ops.npu.npu_rms_norm_dynamic_quant
 npu_swiglu_dynamic_quant = torch.ops.npu.npu_swiglu_dynamic_quant
 npu_quant_matmul_swiglu = torch.ops.npu.npu_quant_matmul_swiglu
 npu_quant_matmul_swiglu_quant = torch.ops.npu.npu_quant_matmul_swiglu_quant
+npu_paged_attention = torch.ops.npu.npu_paged_attention
+npu_prompt_attention = torch.ops.npu.npu_prompt_attention
+npu_mrope = torch.ops.npu.npu_mrope
+npu_mrope_scatter_kv = torch.ops.npu.npu_mrope_scatter_kv
+npu_kv_copy_pages = torch.ops.npu.npu_kv_copy_pages
+npu_kv_fork = torch.ops.npu.npu_kv_fork
+npu_kv_free = torch.ops.npu.npu_kv_free
+npu_kv_extend = torch.ops.npu.npu_kv_extend
+npu_kv_compact = torch.ops.npu.npu_kv_compact
 
 # qk_abi.h constants
 QK_F16, QK_BF16, QK_F32, QK_I8, QK_I32, QK_U8, QK_I4_NZ, QK_I8_NZ, QK_I8_NK = 1, 2, 3, 4, 5, 6, 16, 17, 18
@@ -83,8 +104,28 @@ ABI_SYMBOLS = (
     "qk_weight_quant_bmm", "qk_weight_quant_bmm_noalloc", "qk_int4_pack", "qk_weight_format_cast",
     "qk_quantize_per_tensor", "qk_quantize_per_channel", "qk_dequantize", "qk_rms_norm", "qk_rms_norm_quant",
     "qk_swiglu", "qk_swiglu_quant", "qk_quant_matmul_swiglu", "qk_quant_matmul_swiglu_quant_workspace_size",
-    "qk_quant_matmul_swiglu_quant",
+    "qk_quant_matmul_swiglu_quant", "qk_paged_attention_workspace_size", "qk_paged_attention",
+    "qk_prompt_attention_workspace_size", "qk_prompt_attention", "qk_mrope", "qk_kv_copy_pages",
+    "qk_kv_fork_workspace_size", "qk_kv_fork", "qk_kv_free", "qk_kv_extend_workspace_size", "qk_kv_extend",
+    "qk_kv_compact_workspace_size", "qk_kv_compact",
 )
+
+
+class KvCache(ctypes.Structure):
+    """qk_kv_cache: the keys and values of one layer, as the C ABI takes them (strides in elements)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("key", "value", "key_scale", "value_scale")] + \
+               [(n, ctypes.c_int64) for n in (
+                   "num_pages", "page_size", "kv_heads", "head_dim", "key_page_stride", "key_token_stride",
+                   "key_head_stride", "value_page_stride", "value_token_stride", "value_head_stride",
+                   "key_scale_page_stride", "key_scale_token_stride", "key_scale_head_stride",
+                   "value_scale_page_stride", "value_scale_token_stride", "value_scale_head_stride")] + \
+               [("dtype", ctypes.c_int)]
+
+
+class Pages(ctypes.Structure):
+    """qk_pages: a cache tensor as pages of page_bytes bytes, page_stride bytes apart."""
+    _fields_ = [("base", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("page_bytes", ctypes.c_int64)]
+
 
 _abi = None
 
@@ -120,6 +161,21 @@ def abi() -> ctypes.CDLL:
         L.qk_quant_matmul_swiglu.argtypes = [P, I64, P, I, I64, I64, I64, I64, P, I64, P, P, I, P]
         L.qk_quant_matmul_swiglu_quant_workspace_size.argtypes = [I64, I64, P]
         L.qk_quant_matmul_swiglu_quant.argtypes = [P, I64, P, I, I64, I64, I64, I64, P, I64, P, I, P, P, P, SZ, P]
+        C, G, Z = ctypes.POINTER(KvCache), ctypes.POINTER(Pages), ctypes.POINTER(SZ)
+        L.qk_paged_attention_workspace_size.argtypes = [I64, I64, C, I64, I64, I64, Z]
+        L.qk_paged_attention.argtypes = [P, I, I64, I64, I64, I64, C, P, I64, I64, P, F, I64, I64, P, P, P, SZ, P]
+        L.qk_prompt_attention_workspace_size.argtypes = [I64, I64, I64, C, I64, I64, I64, Z]
+        L.qk_prompt_attention.argtypes = [P, I, I64, I64, I64, I64, I64, P, C, P, P, I64, I64, P, F, I64, I64, P, P, P,
+                                          SZ, P]
+        L.qk_mrope.argtypes = [P, P, P, I] + [I64] * 10 + [P, I64, I64, P, P, I, I64, I64, I, P, P, C, P, P]
+        L.qk_kv_copy_pages.argtypes = [G, I64, I64, P, P, I64, P]
+        L.qk_kv_fork_workspace_size.argtypes = [I64, Z]
+        L.qk_kv_fork.argtypes = [G, I64, I64, I64, P, I64, I64, I64, P, P, P, P, I64, P, P, SZ, P]
+        L.qk_kv_free.argtypes = [I64, I64, P, I64, I64, I64, P, P, P, I64, P]
+        L.qk_kv_extend_workspace_size.argtypes = [I64, I64, Z]
+        L.qk_kv_extend.argtypes = [I64, I64, P, I64, I64, I64, P, P, P, P, I64, I64, P, P, P, P, SZ, P]
+        L.qk_kv_compact_workspace_size.argtypes = [I64, Z]
+        L.qk_kv_compact.argtypes = [G, I64, I64, P, I64, I64, I64, P, P, P, P, P, SZ, P]
         for name in ABI_SYMBOLS:
             getattr(L, name).restype = I if name != "qk_last_error" else ctypes.c_char_p
         _abi = L
@@ -151,5 +207,7 @@ __all__ = [
     "npu_dynamic_quant", "npu_quant_matmul", "npu_weight_quant_batchmatmul",
     "npu_convert_weight_to_int4pack", "npu_format_cast", "get_npu_format", "quantize_per_tensor",
     "quantize_per_channel", "dequantize", "npu_rms_norm", "npu_swiglu", "npu_rms_norm_dynamic_quant",
-    "npu_swiglu_dynamic_quant", "npu_quant_matmul_swiglu", "npu_quant_matmul_swiglu_quant", "abi", "last_error", "debug_set_plan", "LIB_PATH", "OPS_PATH",
+    "npu_swiglu_dynamic_quant", "npu_quant_matmul_swiglu", "npu_quant_matmul_swiglu_quant", "npu_paged_attention",
+    "npu_prompt_attention", "npu_mrope", "npu_mrope_scatter_kv", "npu_kv_copy_pages", "npu_kv_fork", "npu_kv_free",
+    "npu_kv_extend", "npu_kv_compact", "abi", "last_error", "debug_set_plan", "LIB_PATH", "OPS_PATH",
 ]

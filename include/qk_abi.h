@@ -401,6 +401,157 @@ int qk_quant_matmul_swiglu_quant(const int8_t* x1, int64_t ldx1, const int8_t* x
                                  int64_t scale_len, const float* pertoken_scale, int h_dtype, int8_t* q,
                                  float* q_scale, void* workspace, size_t workspace_bytes, qk_stream_t stream);
 
+/* ------------------------------------------------------------------ attention over a key-value cache
+ *
+ * The other half of a decoder layer in serving: rotary positions, a key-value
+ * cache in pages, attention over it.  The reference reaches fused attention
+ * through npu_prompt_flash_attention and npu_incre_flash_attention
+ * (op_plugin/ops/v2r2/opapi/FlashAttentionKernelNpuOpApi.cpp:361-408); the ops
+ * below keep its two phases (prompt, one token) and add the page table.
+ *
+ * Indexes (page tables, lengths, slots, positions, counts) are int32 on the
+ * device.  They are checked where they are used: an index outside its array is
+ * never followed, with the effect stated at each function.
+ */
+
+/* Keys and values of one layer.  key / value: [num_pages][page_size][kv_heads][head_dim] elements of `dtype`
+ * (QK_F16, QK_BF16 or QK_I8), read through strides in elements (head_dim contiguous): any order of the axes.  Rows of
+ * a head start at multiples of 16 bytes.  QK_I8 holds round(x / scale): key_scale / value_scale, fp32
+ * [num_pages][page_size][kv_heads] through strides of their own, one scale per token and head, as npu_dynamic_quant
+ * gives them.  head_dim: a multiple of 8 (QK_I8: of 16), at most 256.  Where a function takes contiguous keys
+ * [tokens][kv_heads][head_dim], they are one page: num_pages = 1, page_size = tokens. */
+typedef struct qk_kv_cache {
+    void* key;
+    void* value;
+    float* key_scale;
+    float* value_scale;
+    int64_t num_pages, page_size, kv_heads, head_dim;
+    int64_t key_page_stride, key_token_stride, key_head_stride;
+    int64_t value_page_stride, value_token_stride, value_head_stride;
+    int64_t key_scale_page_stride, key_scale_token_stride, key_scale_head_stride;
+    int64_t value_scale_page_stride, value_scale_token_stride, value_scale_head_stride;
+    int dtype;
+} qk_kv_cache;
+
+/*
+ * npu_paged_attention -- attention of one new token per sequence over its pages (the op of one token,
+ * npu_incre_flash_attention, op_plugin/ops/v2r2/opapi/FlashAttentionKernelNpuOpApi.cpp:385-408; golden
+ * test/test_custom_ops/test_incre_flash_attention.py:15-23).  query: [batch][q_heads][head_dim] of dtype (QK_F16 /
+ * QK_BF16; a 16-bit cache has the same), through strides in elements (multiples of 8).  q_heads is a multiple of
+ * cache->kv_heads: head h reads key-value head h / (q_heads / kv_heads).  Sequence b holds context_lens[b] tokens, the
+ * newest included, token j in slot j % page_size of page block_table[b * table_stride + j / page_size].  The query
+ * stands at the last of them, p, and sees the keys j <= p with p - j < window (window 0: all) or j < sinks.
+ *   s_j = scale * q . k_j,  out = sum exp(s_j - m) v_j / sum exp(s_j - m),  lse = m + ln sum exp(s_j - m)
+ * in fp32, m the largest s_j; out: [batch][q_heads][head_dim] of dtype, lse: [batch][q_heads] fp32 or NULL.  A sequence
+ * without a visible key (length 0) gives out = 0 and lse = -inf.  Lengths are cut to table_width * page_size; a token
+ * whose page id is outside [0, num_pages) is not seen.  Workspace: partial results where the keys of a sequence are
+ * split over workgroups.
+ */
+int qk_paged_attention_workspace_size(int64_t batch, int64_t q_heads, const qk_kv_cache* cache, int64_t table_width,
+                                      int64_t window, int64_t sinks, size_t* bytes);
+int qk_paged_attention(const void* query, int dtype, int64_t batch, int64_t q_heads, int64_t q_token_stride,
+                       int64_t q_head_stride, const qk_kv_cache* cache, const int32_t* block_table,
+                       int64_t table_width, int64_t table_stride, const int32_t* context_lens, float scale,
+                       int64_t window, int64_t sinks, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                       qk_stream_t stream);
+
+/*
+ * npu_prompt_attention -- causal attention of ragged prompts or prompt chunks (the op of whole prompts,
+ * npu_prompt_flash_attention, op_plugin/ops/v2r2/opapi/FlashAttentionKernelNpuOpApi.cpp:361-383; golden
+ * test/test_custom_ops/test_prompt_flash_attention.py:15-21).  query: [tokens][q_heads][head_dim]; sequence b's rows
+ * are cu_seqlens_q[b] .. cu_seqlens_q[b + 1] (batch + 1 values, the first 0, none falling).  Its keys: with
+ * block_table, kv_lens[b] tokens in pages, as above; without (NULL, cache->num_pages 1), rows cu_seqlens_k[b] ..
+ * cu_seqlens_k[b + 1] of the contiguous keys.  Query i of n, of a sequence with m keys, stands at p = m - n + i and sees
+ * the keys j <= p with p - j < window (window 0: all) or j < sinks.  Same formula, outputs and rules as
+ * qk_paged_attention; a row that sees no key, and a row past the last sequence, gives out = 0 and lse = -inf.
+ */
+int qk_prompt_attention_workspace_size(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache* cache,
+                                       int64_t table_width, int64_t window, int64_t sinks, size_t* bytes);
+int qk_prompt_attention(const void* query, int dtype, int64_t tokens, int64_t batch, int64_t q_heads,
+                        int64_t q_token_stride, int64_t q_head_stride, const int32_t* cu_seqlens_q,
+                        const qk_kv_cache* cache, const int32_t* cu_seqlens_k, const int32_t* block_table,
+                        int64_t table_width, int64_t table_stride, const int32_t* kv_lens, float scale, int64_t window,
+                        int64_t sinks, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                        qk_stream_t stream);
+
+/*
+ * npu_mrope, npu_mrope_scatter_kv -- rotary positions of one to four axes (time, height, width of an image's or a
+ * video's tokens), alone or with the write of the new keys and values into the cache.  query: [tokens][q_heads]
+ * [head_dim], key, value: [tokens][kv_heads][head_dim] of dtype (QK_F16 / QK_BF16) through strides in elements.
+ * positions: axes rows of `tokens` int32, position_stride apart.  cos_sin: [table_rows][rotary_dim] fp32 or of dtype,
+ * each row rotary_dim / 2 cosines, then as many sines; rotary_dim even, at most head_dim.  Pair i < rotary_dim / 2
+ * takes its row at positions[a][t], a being the section that i lies in (sections[axes], summing to rotary_dim / 2).
+ * interleave 0: pair (x_i, x_{i + rotary_dim/2}); 1: (x_2i, x_2i+1).
+ *   y0 = x0 * cos - x1 * sin,  y1 = x1 * cos + x0 * sin  (fp32, each product rounded; one rounding to dtype)
+ * Dimensions past rotary_dim are copied.  A position outside the table makes its pairs NaN.  out_query, out_key
+ * (contiguous, either may be NULL).  With cache: token t's rotated key and its value (NULL: not written) go to slot
+ * slots[t] = page * page_size + token; a slot outside the cache (a padding token's -1) is not written.  An int8 cache takes
+ * each 16-bit row through npu_dynamic_quant: scale = absmax / 127, the values rint(y / scale).  No workspace.
+ */
+int qk_mrope(const void* query, const void* key, const void* value, int dtype, int64_t tokens, int64_t q_heads,
+             int64_t kv_heads, int64_t head_dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+             int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const int32_t* positions,
+             int64_t axes, int64_t position_stride, const int64_t* sections, const void* cos_sin, int cos_sin_dtype,
+             int64_t table_rows, int64_t rotary_dim, int interleave, void* out_query, void* out_key,
+             const qk_kv_cache* cache, const int32_t* slots, qk_stream_t stream);
+
+/* ------------------------------------------------------------------ pages of a cache
+ *
+ * State of a pool: block_table [max_seqs][table_width] (rows table_stride apart, -1 past a sequence's pages),
+ * context_lens [max_seqs], ref_count [num_pages], the number of sequences that hold a page.  A page with count 0 is free,
+ * and a page is allocated from the lowest free one upwards: no free list is kept, and the same calls give the same
+ * pages.  A cache tensor is described by qk_pages: page p's page_bytes bytes begin at base + p * page_stride.
+ * Sequence numbers outside [0, max_seqs) are passed over.  At most QK_MAX_SEQS sequences a call.
+ */
+typedef struct qk_pages {
+    void* base;
+    int64_t page_stride; /* bytes */
+    int64_t page_bytes;
+} qk_pages;
+#define QK_MAX_SEQS 65536
+
+/* npu_kv_copy_pages: for every i < n, page src[i] to page dst[i], in each of the tensors; a pair with an id outside
+ * [0, num_pages) is passed over.  No page may be the destination of two pairs, or of one and the source of another. */
+int qk_kv_copy_pages(const qk_pages* pages, int64_t tensors, int64_t num_pages, const int32_t* src,
+                     const int32_t* dst, int64_t n, qk_stream_t stream);
+
+/* npu_kv_fork: sequence children[i] becomes a copy of parents[i].  Whole pages are shared (count + 1); a last page that
+ * is not full goes to a new page (count 1), whose bytes are copied in each of the tensors, so no writable page is
+ * shared.  A child's former pages are not released (qk_kv_free does that before); no child may be a parent or occur
+ * twice.  missing[0] = how many free pages are missing: 0, or nothing but missing[0] is written.  Workspace: n + 1 int32
+ * pairs. */
+int qk_kv_fork_workspace_size(int64_t n, size_t* bytes);
+int qk_kv_fork(const qk_pages* pages, int64_t tensors, int64_t num_pages, int64_t page_size, int32_t* block_table,
+               int64_t max_seqs, int64_t table_width, int64_t table_stride, int32_t* context_lens, int32_t* ref_count,
+               const int32_t* parents, const int32_t* children, int64_t n, int32_t* missing, void* workspace,
+               size_t workspace_bytes, qk_stream_t stream);
+
+/* npu_kv_free: the pages of sequences seqs[i] lose a count, their table rows become -1, their lengths 0.  A sequence
+ * named twice is freed once. */
+int qk_kv_free(int64_t num_pages, int64_t page_size, int32_t* block_table, int64_t max_seqs, int64_t table_width,
+               int64_t table_stride, int32_t* context_lens, int32_t* ref_count, const int32_t* seqs, int64_t n,
+               qk_stream_t stream);
+
+/* npu_kv_extend: sequence seqs[i] (none twice) grows by cu_tokens[i + 1] - cu_tokens[i] tokens.  Pages are allocated in
+ * the order of i; slots[t] and positions[t], t < total, are the cache slot and the position of each new token (-1
+ * past cu_tokens[n], and for a sequence number that is passed over).  missing[0] = how many free pages, or table columns,
+ * are missing: 0, or slots and positions are -1 and nothing else is written.  Workspace: see the query. */
+int qk_kv_extend_workspace_size(int64_t n, int64_t num_pages, size_t* bytes);
+int qk_kv_extend(int64_t num_pages, int64_t page_size, int32_t* block_table, int64_t max_seqs, int64_t table_width,
+                 int64_t table_stride, int32_t* context_lens, int32_t* ref_count, const int32_t* seqs,
+                 const int32_t* cu_tokens, int64_t n, int64_t total, int32_t* slots, int32_t* positions,
+                 int32_t* missing, void* workspace, size_t workspace_bytes, qk_stream_t stream);
+
+/* npu_kv_compact: with L pages in use (count > 0), the k-th page in use of number >= L is copied to the k-th free page of
+ * number < L, in each of the tensors.  new_table [max_seqs][table_width] (contiguous) and new_count [num_pages] are the
+ * table and the counts with the pages at their new places; the old ones, and the pages moved from, stay as they were.
+ * moved[0] = how many pages moved.  Workspace: see the query. */
+int qk_kv_compact_workspace_size(int64_t num_pages, size_t* bytes);
+int qk_kv_compact(const qk_pages* pages, int64_t tensors, int64_t num_pages, const int32_t* block_table,
+                  int64_t max_seqs, int64_t table_width, int64_t table_stride, const int32_t* ref_count,
+                  int32_t* new_table, int32_t* new_count, int32_t* moved, void* workspace, size_t workspace_bytes,
+                  qk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
