@@ -2,12 +2,12 @@
 // one at a time, each lane holding every 64th element of the head, with the running maximum and sum of a softmax.
 //   m' = max(m, s),  l = l * e^(m - m') + e^(s - m'),  acc = acc * e^(m - m') + e^(s - m') * v
 // All in fp32, one rounding of acc / l at the end.  Bound by its instructions: some 40 per key and wave.
-#include "attention.h"
+#include "attention_device.h"
 
 namespace qk {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+
 constexpr int kPer = 4;  // elements per lane: head_dim <= 256
 
 __device__ __forceinline__ float load_elem(const void* p, int64_t i, int dtype) {

@@ -181,7 +181,7 @@ int qk_paged_attention_workspace_size(int64_t batch, int64_t q_heads, const qk_k
     if (int rc = check_attention_sizes(op, batch, batch, q_heads, cache, cache && cache->dtype != QK_I8 ? cache->dtype : QK_BF16,
                                        table_width, window, sinks))
         return rc;
-    *bytes = 0;
+    *bytes = qk::attention_decode_workspace(batch, q_heads, *cache, table_width, window, sinks);
     return QK_OK;
 }
 
@@ -206,7 +206,7 @@ int qk_paged_attention(const void* query, int dtype, int64_t batch, int64_t q_he
     size_t need = 0;
     if (int rc = qk_paged_attention_workspace_size(batch, q_heads, cache, table_width, window, sinks, &need)) return rc;
     if (int rc = check_workspace(op, need, workspace, workspace_bytes)) return rc;
-    return launched(qk::launch_attention_rows(a, (hipStream_t)stream), op);
+    return launched(qk::launch_attention_decode(a, workspace, workspace_bytes, (hipStream_t)stream), op);
 }
 
 int qk_prompt_attention_workspace_size(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache* cache,
