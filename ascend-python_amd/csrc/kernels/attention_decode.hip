@@ -51,11 +51,6 @@ __device__ __forceinline__ int64_t line_begin(int64_t total, int64_t workers, in
 __device__ __forceinline__ int64_t worker_of(int64_t total, int64_t workers, int64_t u) {
     return quotient((u + 1) * workers + total - 1, total) - 1;
 }
-// A value that all lanes hold, in scalar registers.
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
-    return (int64_t)((uint64_t)hi << 32 | lo);
-}
 
 __device__ __forceinline__ int32_t length_of(const AttnArgs& a, int64_t b) {
     const int64_t most = a.kv.table_width * a.kv.c.page_size, n = a.kv.lens[b];
@@ -105,7 +100,7 @@ __global__ __launch_bounds__(kThreads, KS <= 4 ? 3 : KS <= 6 ? 2 : 1) void atten
         for (int w = 0; w < wave; ++w) in += scan[w];
         mine = in - mine;  // units before this thread's sequences
     }
-    const int64_t units = uniform(scan[0] + scan[1] + scan[2] + scan[3]);
+    const int64_t units = (int64_t)uniform64(scan[0] + scan[1] + scan[2] + scan[3]);
     Line line;
     line.total = units * head_rows;
     line.workers = (int32_t)(line.total < gridDim.x ? line.total : gridDim.x);
@@ -124,7 +119,7 @@ __global__ __launch_bounds__(kThreads, KS <= 4 ? 3 : KS <= 6 ? 2 : 1) void atten
         }
     }
     __syncthreads();
-    int64_t b = uniform(found[0]), b_start = uniform(found[1]);
+    int64_t b = (int64_t)uniform64(found[0]), b_start = (int64_t)uniform64(found[1]);
 
     char* const v_lds = lds + wave * WAVE_LDS;
     float* const s_lds = (float*)(v_lds + kTile * VROW);  // [2][16] key scales, [2][16] value scales

@@ -75,6 +75,12 @@ __device__ __forceinline__ float quad_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// A value that all lanes hold, in scalar registers.
+__device__ __forceinline__ uint64_t uniform64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+    return (uint64_t)hi << 32 | lo;
+}
+
 // The keys that a position sees, without a gap: the first `sinks` of them, then those from `low` on.
 struct Seen {
     int32_t count, sinks, gap;

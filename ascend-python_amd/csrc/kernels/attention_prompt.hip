@@ -1,0 +1,513 @@
+// Causal attention of ragged prompts: s_j = scale * q . k_j over the keys that a row sees, out = sum e^(s_j - m) v_j / sum e^(s_j - m).
+//
+// Bound by the matrix cores: 4 * head_dim operations per visible pair and query head.  A workgroup takes 128 rows of one
+// key-value head and sequence, a row being a (token, query head of the group) pair, token first: so a tile of a group of four
+// spans 32 tokens, its causal edge is short, and every key read serves the whole group.  It walks the keys that any of
+// its rows sees 64 at a time, each of the four waves with 32 rows.
+//
+// Scores: K (32 keys are the rows) times Q^T (32 rows are the columns), 32x32x16: the lane holds 16 keys of one row, so
+// maximum and sum need one exchange between lane pairs, and the weights as they lie are the right operand of V^T times P^T.
+// K and V pass through registers (int8 becomes 16-bit on the way) into two LDS buffers, rows padded by 16 bytes against
+// bank conflicts; V is read back transposed.  One barrier per 64 keys: the next rows are loaded while these are worked on.
+// Where a row of the cache lies is found two tiles ahead by one wave, a lane per row.
+//
+// A masked weight is 0, but 0 times a NaN or an infinity in V is NaN: tiles that are masked for some rows look for such
+// values while they are staged, and their rows of V are added apart, for the rows that see them.
+#include <type_traits>
+
+#include "attention_device.h"
+
+namespace qk {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRows = 128;   // query rows per workgroup
+constexpr int kKeys = 64;    // keys per tile
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int DT>
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    typedef typename Mfma<DT>::v8 v8;
+    if constexpr (DT == QK_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+
+struct PromptArgs {
+    AttnArgs a;
+    Div31 group_div;  // q_heads / kv_heads
+};
+
+// Rows of tokens and keys of sequence b (b == batch: the rows past the last sequence, which see nothing)
+struct Sequence {
+    int32_t first, tokens;
+};
+__device__ __forceinline__ Sequence sequence_of(const AttnArgs& a, int64_t b) {
+    const int32_t T = (int32_t)a.tokens;
+    int32_t first = b == 0 ? 0 : a.cu_q[b], end = b == a.batch ? T : a.cu_q[b + 1];
+    first = first < 0 ? 0 : first > T ? T : first;
+    end = end > T ? T : end;
+    return {first, end > first ? end - first : 0};
+}
+
+template <int DT>
+__device__ __forceinline__ constexpr uint32_t exponent_of() {
+    return DT == QK_BF16 ? 0x7f80u : 0x7c00u;
+}
+template <int DT>
+__device__ __forceinline__ bool not_finite(u32x4 w) {
+    constexpr uint32_t E = exponent_of<DT>(), H = E << 16;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= (w[i] & E) == E || (w[i] & H) == H;
+    return any;
+}
+// The finite values, and zero for the others.
+template <int DT>
+__device__ __forceinline__ u32x4 finite_only(u32x4 w) {
+    constexpr uint32_t E = exponent_of<DT>(), H = E << 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] &= ((w[i] & E) == E ? 0u : 0xffffu) | ((w[i] & H) == H ? 0u : 0xffff0000u);
+    return w;
+}
+
+// Largest value, and sum, over lanes l and l ^ 32.
+__device__ __forceinline__ float pair_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// DP: head_dim padded to 32s; WHOLE: head_dim == DP; Q8: int8 cache
+template <int DP, int DT, bool Q8, bool WHOLE>
+__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(PromptArgs g) {
+    constexpr int KS = DP / 16;                  // steps of the first product
+    constexpr int NB = DP / 32;                  // 32-row blocks of V^T
+    constexpr int PITCH = DP * 2 + 16;
+    constexpr int ES = Q8 ? 1 : 2;
+    constexpr int CH = DP * ES / 16;             // 16-byte pieces of a cache row
+    constexpr int PIECES = kKeys * CH / kThreads; // per thread
+    constexpr int PV = Q8 ? QK_F16 : DT;
+    static_assert(kKeys * CH % kThreads == 0, "");
+    __shared__ __attribute__((aligned(16))) char lds[2][2][kKeys * PITCH];  // [buffer][K, V]
+    __shared__ int64_t info[2][kKeys][2];        // byte offsets of a key's and a value's row; -1: none
+    __shared__ uint64_t info_ok[2];              // which keys of the tile exist
+    __shared__ uint64_t bad[3];                  // which rows of V hold a NaN or an infinity
+    __shared__ float scales[2][2][kKeys];
+    __shared__ int64_t found[3];
+
+    const AttnArgs& a = g.a;
+    const qk_kv_cache& c = a.kv.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int col = lane & 31, kg = lane >> 5;
+    const int D = (int)c.head_dim, G = (int)(a.q_heads / c.kv_heads);
+    const int kvh = (int)(blockIdx.x % (uint32_t)c.kv_heads);
+
+    // ---- which tile: those of all sequences in a line, the last first (the longest of a prompt come first)
+    {
+        const int64_t per = (a.batch + 1 + kThreads - 1) / kThreads;
+        const int64_t b0 = tid * per, b1 = b0 + per < a.batch + 1 ? b0 + per : a.batch + 1;
+        int64_t mine = 0;
+        for (int64_t b = b0; b < b1; ++b) mine += ((int64_t)sequence_of(a, b).tokens * G + kRows - 1) / kRows;
+        int64_t* const sums = &info[0][0][0];
+        int64_t in = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t o = __shfl_up(in, d);
+            if (lane >= d) in += o;
+        }
+        if (lane == 63) sums[wave] = in;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) in += sums[w];
+        const int64_t total = sums[0] + sums[1] + sums[2] + sums[3];
+        const int64_t rank = total - 1 - blockIdx.x / (uint32_t)c.kv_heads;
+        if (rank < 0) return;
+        int64_t at = in - mine;
+        for (int64_t b = b0; b < b1; ++b) {
+            const int64_t n = ((int64_t)sequence_of(a, b).tokens * G + kRows - 1) / kRows;
+            if (at <= rank && rank < at + n) {
+                found[0] = b;
+                found[1] = rank - at;
+            }
+            at += n;
+        }
+        if (tid < 3) bad[tid] = 0;
+        __syncthreads();
+    }
+    const int32_t b = __builtin_amdgcn_readfirstlane((int32_t)found[0]);
+    const int32_t row0 = __builtin_amdgcn_readfirstlane((int32_t)found[1]) * kRows;
+    const Sequence seq = sequence_of(a, b);
+    const int32_t rows = (int32_t)((int64_t)seq.tokens * G - row0 < kRows ? (int64_t)seq.tokens * G - row0 : kRows);
+
+    // keys of the sequence, and the row of the first where they are contiguous
+    int32_t keys = 0, key0 = 0;
+    if (b < a.batch) {
+        if (a.kv.table) {
+            const int64_t most = a.kv.table_width * c.page_size;
+            keys = a.kv.lens[b];
+            keys = keys < 0 ? 0 : keys > most ? (int32_t)most : keys;
+        } else {
+            const int32_t all = c.num_pages ? (int32_t)c.page_size : 0;
+            key0 = b == 0 ? 0 : a.kv.cu_k[b];
+            key0 = key0 < 0 ? 0 : key0;
+            const int32_t end = a.kv.cu_k[b + 1] < all ? a.kv.cu_k[b + 1] : all;
+            keys = end > key0 ? end - key0 : 0;
+        }
+    }
+    const int32_t past = keys - seq.tokens;  // position of the first token (negative: it stands before the first key)
+    const int32_t p_first = past + div31(row0, g.group_div), p_last = past + div31(row0 + rows - 1, g.group_div);
+
+    // this lane's row (past the last: as the last) and its wave's span
+    const int32_t mine = row0 + (wave * 32 + col < rows ? wave * 32 + col : rows - 1);
+    const int32_t token = div31(mine, g.group_div);
+    const int64_t t = seq.first + token;
+    const int h = kvh * G + (mine - token * G);
+    const int32_t p = past + token;
+    const int32_t w_first = __builtin_amdgcn_readfirstlane(p), w_last = __builtin_amdgcn_readlane(p, 31);
+
+    // the keys that any row sees, without a gap: key j is place j or, past the sinks, j - gap
+    int32_t low = 0, sinks = 0;
+    if (a.window && p_first - a.window + 1 > 0) {
+        low = p_first - a.window + 1;
+        sinks = a.sinks < low ? a.sinks : low;
+    }
+    const int32_t gap = low - sinks;
+    const int32_t places = p_last < 0 ? 0 : p_last + 1 - gap;
+    const int tiles = (places + kKeys - 1) / kKeys;
+
+    // the largest score is found before the scale is applied: a negative scale's sign goes to the query
+    const uint32_t turned = a.scale < 0.0f ? 0x80008000u : 0u;
+    u32x4 q[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        const int d = 16 * s + 8 * kg;
+        q[s] = (u32x4){0, 0, 0, 0};
+        if (WHOLE || d < D) q[s] = *(const u32x4*)((const uint16_t*)a.q + t * a.q_token_stride + h * a.q_head_stride + d);
+        q[s] ^= turned;
+    }
+    f32x16 acc[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
+    float m = kLowest, l = 0.0f, v_top = 0x1p-100f, v_inv = 0x1p100f;
+    bool any = false;
+    const float factor = fabsf(a.scale) * kLog2e;
+
+    const int32_t* const table = a.kv.table ? a.kv.table + b * a.kv.table_stride : nullptr;
+    const Global zeros = global_address(kZeroRow);
+    const Global k_base = global_address(c.key) + kvh * c.key_head_stride * ES;
+    const Global v_base = global_address(c.value) + kvh * c.value_head_stride * ES;
+
+    // wave 0, a lane per row: the page of a tile's row, then its place in memory and its scales
+    auto place = [&](int tile) {
+        const int32_t v = tile * kKeys + lane;
+        return v < places ? (v < sinks ? v : v + gap) : -1;
+    };
+    auto page_of = [&](int tile) {
+        const int32_t j = place(tile);
+        return table && j >= 0 ? table[div31(j, a.kv.page_div)] : -1;
+    };
+    float ks_next = 0.0f, vs_next = 0.0f;
+    auto put_info = [&](int tile, int32_t page) {
+        const int32_t j = place(tile);
+        int32_t slot = key0 + j;
+        bool valid = j >= 0;
+        if (table) {
+            slot = j - div31(j, a.kv.page_div) * (int32_t)c.page_size;
+            valid = valid && page >= 0 && page < c.num_pages;
+        } else {
+            page = 0;
+        }
+        info[tile & 1][lane][0] = valid ? (page * c.key_page_stride + slot * c.key_token_stride) * ES : -1;
+        info[tile & 1][lane][1] = valid ? (page * c.value_page_stride + slot * c.value_token_stride) * ES : -1;
+        const uint64_t ok = __builtin_amdgcn_ballot_w64(valid);
+        if (lane == 0) info_ok[tile & 1] = ok;
+        if constexpr (Q8) {
+            Global kz = zeros, vz = zeros;
+            if (valid) {
+                kz = global_address(c.key_scale + page * c.key_scale_page_stride + slot * c.key_scale_token_stride +
+                                    kvh * c.key_scale_head_stride);
+                vz = global_address(c.value_scale + page * c.value_scale_page_stride + slot * c.value_scale_token_stride +
+                                    kvh * c.value_scale_head_stride);
+            }
+            ks_next = load_global<float>(kz);
+            vs_next = load_global<float>(vz);
+        }
+    };
+    auto put_scales = [&](int tile) {
+        if constexpr (Q8) {
+            scales[tile & 1][0][lane] = ks_next;
+            scales[tile & 1][1][lane] = vs_next;
+        }
+    };
+
+    u32x4 kr[PIECES], vr[PIECES];
+    uint64_t ok_next = 0;
+    auto load_tile = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int at = tid + i * kThreads, r = at / CH, ch = at % CH;
+            const int64_t ko = info[tile & 1][r][0], vo = info[tile & 1][r][1];
+            Global kp = zeros, vp = zeros;
+            if (ko >= 0 && (WHOLE || ch * 16 < D * ES)) {
+                kp = k_base + ko + ch * 16;
+                vp = v_base + vo + ch * 16;
+            }
+            kr[i] = load_global<u32x4>(kp);
+            vr[i] = load_global<u32x4>(vp);
+        }
+        ok_next = info_ok[tile & 1];
+    };
+
+    if (tiles > 0) {
+        int32_t page = -1;
+        if (wave == 0) {
+            put_info(0, page_of(0));
+            put_scales(0);
+            put_info(1, page_of(1));
+            page = page_of(2);
+        }
+        __syncthreads();
+        load_tile(0);
+        for (int it = 0; it < tiles; ++it) {
+            char* const kb = lds[it & 1][0];
+            char* const vb = lds[it & 1][1];
+            const uint64_t ok = uniform64(ok_next);
+            // masked for some row of the workgroup?
+            const int32_t j0 = it * kKeys + (it * kKeys < sinks ? 0 : gap), last = it * kKeys + kKeys - 1;
+            const int32_t j1 = last + (last < sinks ? 0 : gap);
+            auto all_see = [&](int32_t first_p, int32_t last_p) {
+                return ~ok == 0 && j1 <= first_p && (!a.window || j1 < a.sinks || last_p - j0 < a.window);
+            };
+            const bool edge = !all_see(p_first, p_last);
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int at = tid + i * kThreads, r = at / CH, ch = at % CH;
+                if constexpr (Q8) {
+                    *(u32x4*)(kb + r * PITCH + ch * 32) = i8_to_half<DT>(kr[i][0], kr[i][1]);
+                    *(u32x4*)(kb + r * PITCH + ch * 32 + 16) = i8_to_half<DT>(kr[i][2], kr[i][3]);
+                    *(u32x4*)(vb + r * PITCH + ch * 32) = i8_to_f16(vr[i][0], vr[i][1]);
+                    *(u32x4*)(vb + r * PITCH + ch * 32 + 16) = i8_to_f16(vr[i][2], vr[i][3]);
+                } else {
+                    *(u32x4*)(kb + r * PITCH + ch * 16) = kr[i];
+                    *(u32x4*)(vb + r * PITCH + ch * 16) = vr[i];
+                    if (edge && not_finite<DT>(vr[i])) atomicOr((unsigned long long*)&bad[it % 3], 1ull << r);
+                }
+            }
+            __syncthreads();
+            if (it + 1 < tiles) load_tile(it + 1);
+            if (wave == 0) {
+                put_scales(it + 1);
+                put_info(it + 2, page);
+                page = page_of(it + 3);
+                if (lane == 0) bad[(it + 2) % 3] = 0;
+            }
+            // no row of this wave sees the tile
+            if (j0 > w_last || (a.window && w_first - j1 >= a.window && j0 >= a.sinks)) continue;
+
+            // scores: lane (row, kg) holds keys 32 n + 8 (e / 4) + 4 kg + e % 4
+            f32x16 x[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[n][e] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+                    x[n] = mma32<DT>(*(const u32x4*)(kb + (32 * n + col) * PITCH + (2 * s + kg) * 16), q[s], x[n]);
+            }
+            if constexpr (Q8) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 k4 = *(const f32x4*)&scales[it & 1][0][32 * n + 8 * i + 4 * kg];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[n][4 * i + r] *= k4[r];
+                    }
+            }
+            uint32_t hidden = 0;  // bit 16 n + e
+            const bool masked = !all_see(w_first, w_last);
+            if (masked) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = 32 * n + 8 * (e >> 2) + 4 * kg + (e & 3);
+                        const int32_t v = it * kKeys + key, j = v < sinks ? v : v + gap;
+                        const bool sees = (ok >> key & 1) && j <= p && (!a.window || p - j < a.window || j < a.sinks);
+                        hidden |= (uint32_t)!sees << (16 * n + e);
+                        if (!sees) x[n][e] = -__builtin_inff();
+                    }
+            }
+            any |= hidden != ~0u;
+            float top = x[0][0];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[n][e]);
+            top *= factor;
+            if (__builtin_amdgcn_ballot_w64(top > m + kSlack)) {
+                const float m2 = fmaxf(m, pair_max(top));
+                const float keep = __builtin_amdgcn_exp2f(m - m2);
+                m = m2;
+                l *= keep;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) acc[i] *= keep;
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e], factor, -m));
+            if (masked) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[n][e] = hidden >> (16 * n + e) & 1 ? 0.0f : x[n][e];
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) l += x[n][e];
+            if constexpr (Q8) {
+                auto scale_of = [&](int n, int e, float v) { return masked && (hidden >> (16 * n + e) & 1) ? 0.0f : v; };
+                float most = 0.0f;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 v4 = *(const f32x4*)&scales[it & 1][1][32 * n + 8 * i + 4 * kg];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float v = scale_of(n, 4 * i + r, v4[r]);
+                            most = fmaxf(most, fabsf(v));
+                            x[n][4 * i + r] *= v;
+                        }
+                    }
+                if (__builtin_amdgcn_ballot_w64(most > v_top)) {
+                    most = fmaxf(v_top, pair_max(most));
+                    const float inv = 1.0f / most, keep = v_top * inv;
+                    v_top = most;
+                    v_inv = inv;
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) acc[i] *= keep;
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[n][e] *= v_inv;
+            }
+            // acc += V^T P^T; CLEAN: without the values of V that are not finite
+            auto second = [&](auto clean) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int n = s >> 1, e0 = 8 * (s & 1);
+                    u32x4 pw;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) pw[i] = pack2<PV>(x[n][e0 + 2 * i], x[n][e0 + 2 * i + 1]);
+                    const char* const from = vb + (16 * s + 4 * kg + (lane >> 2 & 3)) * PITCH + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) {
+                        const u32x2 lo = lds_tr16(from + 64 * i), hi = lds_tr16(from + 8 * PITCH + 64 * i);
+                        u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+                        if constexpr (decltype(clean)::value) v = finite_only<DT>(v);
+                        acc[i] = mma32<PV>(v, pw, acc[i]);
+                    }
+                }
+            };
+            if constexpr (Q8) {
+                second(std::false_type());
+            } else {
+                uint64_t left = masked ? uniform64(bad[it % 3]) : 0;
+                if (!left) {
+                    second(std::false_type());
+                } else {
+                    second(std::true_type());
+                    for (; left; left &= left - 1) {
+                        const int key = __builtin_ctzll(left);
+                        // this row's weight of the key, from whichever of the two lanes holds it, and whether it is seen
+                        float w = 0.0f;
+                        bool sees = false;
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (key == 32 * n + 8 * (e >> 2) + 4 * kg + (e & 3)) {
+                                    w = x[n][e];
+                                    sees = !(hidden >> (16 * n + e) & 1);
+                                }
+                        w = pair_sum(w);
+                        sees = pair_max(sees ? 1.0f : 0.0f) != 0.0f;
+#pragma unroll
+                        for (int i = 0; i < NB; ++i)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const uint32_t bits = *(const uint16_t*)(vb + key * PITCH + (32 * i + 8 * (e >> 2) + 4 * kg + (e & 3)) * 2);
+                                if (sees && (bits & exponent_of<DT>()) == exponent_of<DT>()) acc[i][e] += w * load_half_bits(bits, DT);
+                            }
+                    }
+                }
+            }
+        }
+    }
+
+    l = pair_sum(l);
+    any = pair_max(any ? 1.0f : 0.0f) != 0.0f;
+    if (wave * 32 + col >= rows) return;
+    const float inv = (Q8 ? v_top : 1.0f) / l;
+    const int64_t o = t * a.q_heads + h;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = 32 * i + 2 * e + 4 * kg;
+            if (!WHOLE && d >= D) continue;
+            f32x4 r;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r[k] = any ? acc[i][e + k] * inv : 0.0f;
+            *(u32x2*)((uint16_t*)a.out + o * D + d) = (u32x2){pack2<DT>(r[0], r[1]), pack2<DT>(r[2], r[3])};
+        }
+    if (kg == 0 && a.lse) a.lse[o] = any ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -__builtin_inff();
+}
+
+template <int DP, int DT, bool Q8>
+void launch_width(const PromptArgs& g, int64_t grid, hipStream_t stream) {
+    if (g.a.kv.c.head_dim == DP) attention_prompt<DP, DT, Q8, true><<<dim3((unsigned)grid), kThreads, 0, stream>>>(g);
+    else attention_prompt<DP, DT, Q8, false><<<dim3((unsigned)grid), kThreads, 0, stream>>>(g);
+}
+template <int DT, bool Q8>
+void launch_type(const PromptArgs& g, int64_t grid, hipStream_t stream) {
+    const int64_t D = g.a.kv.c.head_dim;
+    if (D <= 64) launch_width<64, DT, Q8>(g, grid, stream);
+    else if (D <= 96 && !Q8) launch_width<96, DT, false>(g, grid, stream);
+    else if (D <= 128) launch_width<128, DT, Q8>(g, grid, stream);
+    else if (D <= 192) launch_width<192, DT, Q8>(g, grid, stream);
+    else launch_width<256, DT, Q8>(g, grid, stream);
+}
+
+}  // namespace
+
+hipError_t launch_attention_prompt(const AttnArgs& a, hipStream_t stream) {
+    PromptArgs g = {};
+    g.a = a;
+    const int64_t group = a.q_heads / a.kv.c.kv_heads;
+    g.group_div = div31((uint32_t)group);
+    // at most: whole tiles, and a last one for every sequence and for the rows past them
+    const int64_t some = a.batch < a.tokens ? a.batch : a.tokens;
+    const int64_t grid = (a.tokens * group / kRows + some + 1) * a.kv.c.kv_heads;
+    const bool q8 = a.kv.c.dtype == QK_I8;
+    if (a.dtype == QK_BF16) {
+        if (q8) launch_type<QK_BF16, true>(g, grid, stream);
+        else launch_type<QK_BF16, false>(g, grid, stream);
+    } else {
+        if (q8) launch_type<QK_F16, true>(g, grid, stream);
+        else launch_type<QK_F16, false>(g, grid, stream);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace qk

@@ -254,7 +254,7 @@ int qk_prompt_attention(const void* query, int dtype, int64_t tokens, int64_t ba
     size_t need = 0;
     if (int rc = qk_prompt_attention_workspace_size(tokens, batch, q_heads, cache, table_width, window, sinks, &need)) return rc;
     if (int rc = check_workspace(op, need, workspace, workspace_bytes)) return rc;
-    return launched(qk::launch_attention_rows(a, (hipStream_t)stream), op);
+    return launched(qk::launch_attention_prompt(a, (hipStream_t)stream), op);
 }
 
 int qk_mrope(const void* query, const void* key, const void* value, int dtype, int64_t tokens, int64_t q_heads,
