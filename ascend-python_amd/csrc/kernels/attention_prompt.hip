@@ -7,14 +7,16 @@
 //
 // Scores: K (32 keys are the rows) times Q^T (32 rows are the columns), 32x32x16: the lane holds 16 keys of one row, so
 // maximum and sum need one exchange between lane pairs, and the weights as they lie are the right operand of V^T times P^T.
-// K and V pass through registers (int8 becomes 16-bit on the way) into two LDS buffers, rows padded by 16 bytes against
-// bank conflicts; V is read back transposed.  One barrier per 64 keys: the next rows are loaded while these are worked on.
-// Where a row of the cache lies is found two tiles ahead by one wave, a lane per row.
+// K and V go straight from memory into two LDS buffers (an int8 cache through registers, where it becomes 16-bit), the 16-byte
+// pieces of a row exchanged so that neither the reads of K nor the transposing reads of V meet in a bank.  One barrier per
+// 64 keys: the next rows are on their way while these are worked on.  Where a row of the cache lies is found two tiles
+// ahead, a lane per row, by the waves in turn.
+//
+// The running maximum is not looked for in every tile: the weights are taken against the one there is, and only where their sum
+// shows that a score lies far above it are the scores made again and the maximum moved.
 //
 // A masked weight is 0, but 0 times a NaN or an infinity in V is NaN: tiles that are masked for some rows look for such
-// values while they are staged, and their rows of V are added apart, for the rows that see them.
-#include <type_traits>
-
+// values once they are staged, and the values are added apart, for the rows that see them.
 #include "attention_device.h"
 
 namespace qk {
@@ -23,6 +25,11 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRows = 128;   // query rows per workgroup
 constexpr int kKeys = 64;    // keys per tile
+// A lane's 32 weights of a tile may sum to this before the maximum is looked for again: far inside the range of either
+// 16-bit type and of the fp32 sums.
+constexpr float kMostSum = 4096.0f;
+
+constexpr int kMfma = 0x8, kDsRead = 0x100;  // instruction groups of the scheduler
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -33,6 +40,17 @@ __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+
+// v, as a value that is made here: what follows from it is not computed ahead of the loop, where it would hold registers.
+__device__ __forceinline__ int here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// 16 bytes per lane from memory into LDS bytes [lds + 16 * lane, +16); the kernel waits on vmcnt itself (as dma16).
+__device__ __forceinline__ void global_to_lds(Global from, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(lds));
 }
 
 struct PromptArgs {
@@ -88,18 +106,21 @@ template <int DP, int DT, bool Q8, bool WHOLE>
 __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(PromptArgs g) {
     constexpr int KS = DP / 16;                  // steps of the first product
     constexpr int NB = DP / 32;                  // 32-row blocks of V^T
-    constexpr int PITCH = DP * 2 + 16;
+    constexpr int LS = DP <= 64 ? 128 : DP <= 128 ? 256 : 512;  // bytes of a row in LDS
+    constexpr int CHL = LS / 16;                 // 16-byte pieces of it
     constexpr int ES = Q8 ? 1 : 2;
     constexpr int CH = DP * ES / 16;             // 16-byte pieces of a cache row
-    constexpr int PIECES = kKeys * CH / kThreads; // per thread
+    constexpr int PIECES = Q8 ? kKeys * CH / kThreads : 1;  // int8: per thread
+    constexpr int DMAS = CHL / 4;                // 16-bit: 1 KB loads per wave for K, and for V
     constexpr int PV = Q8 ? QK_F16 : DT;
-    static_assert(kKeys * CH % kThreads == 0, "");
-    __shared__ __attribute__((aligned(16))) char lds[2][2][kKeys * PITCH];  // [buffer][K, V]
-    __shared__ int64_t info[2][kKeys][2];        // byte offsets of a key's and a value's row; -1: none
+    static_assert(!Q8 || kKeys * CH % kThreads == 0, "");
+    constexpr int TILE = kKeys * LS;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];  // buffer 0: K, V; buffer 1: K, V
+    __shared__ __attribute__((aligned(16))) uint64_t info[3][kKeys][2];  // addresses of a key's and a value's row (none: of zeros)
     __shared__ uint64_t info_ok[2];              // which keys of the tile exist
     __shared__ uint64_t bad[3];                  // which rows of V hold a NaN or an infinity
     __shared__ float scales[2][2][kKeys];
-    __shared__ int64_t found[3];
+    __shared__ int64_t found[2];
 
     const AttnArgs& a = g.a;
     const qk_kv_cache& c = a.kv.c;
@@ -114,7 +135,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         const int64_t b0 = tid * per, b1 = b0 + per < a.batch + 1 ? b0 + per : a.batch + 1;
         int64_t mine = 0;
         for (int64_t b = b0; b < b1; ++b) mine += ((int64_t)sequence_of(a, b).tokens * G + kRows - 1) / kRows;
-        int64_t* const sums = &info[0][0][0];
+        int64_t* const sums = (int64_t*)&info[0][0][0];
         int64_t in = mine;
         for (int d = 1; d < 64; d <<= 1) {
             const int64_t o = __shfl_up(in, d);
@@ -203,7 +224,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     const Global k_base = global_address(c.key) + kvh * c.key_head_stride * ES;
     const Global v_base = global_address(c.value) + kvh * c.value_head_stride * ES;
 
-    // wave 0, a lane per row: the page of a tile's row, then its place in memory and its scales
+    // a lane per row of a tile: its page, then its place in memory and its scales
     auto place = [&](int tile) {
         const int32_t v = tile * kKeys + lane;
         return v < places ? (v < sinks ? v : v + gap) : -1;
@@ -223,8 +244,13 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         } else {
             page = 0;
         }
-        info[tile & 1][lane][0] = valid ? (page * c.key_page_stride + slot * c.key_token_stride) * ES : -1;
-        info[tile & 1][lane][1] = valid ? (page * c.value_page_stride + slot * c.value_token_stride) * ES : -1;
+        Global kp = zeros, vp = zeros;
+        if (valid) {
+            kp = k_base + (page * c.key_page_stride + slot * c.key_token_stride) * ES;
+            vp = v_base + (page * c.value_page_stride + slot * c.value_token_stride) * ES;
+        }
+        info[tile % 3][lane][0] = (uint64_t)(uintptr_t)kp;
+        info[tile % 3][lane][1] = (uint64_t)(uintptr_t)vp;
         const uint64_t ok = __builtin_amdgcn_ballot_w64(valid);
         if (lane == 0) info_ok[tile & 1] = ok;
         if constexpr (Q8) {
@@ -246,37 +272,56 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         }
     };
 
+    // the place of piece ch of row r in LDS
+    auto k_turn = [](int r) { return CHL == 8 ? r >> 1 & 7 : r & 15; };
+    auto v_turn = [](int r) { return CHL == 8 ? (r >> 1 & 3) << 1 : (r & 7) << 1; };
     u32x4 kr[PIECES], vr[PIECES];
     uint64_t ok_next = 0;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     auto load_tile = [&](int tile) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int at = tid + i * kThreads, r = at / CH, ch = at % CH;
-            const int64_t ko = info[tile & 1][r][0], vo = info[tile & 1][r][1];
-            Global kp = zeros, vp = zeros;
-            if (ko >= 0 && (WHOLE || ch * 16 < D * ES)) {
-                kp = k_base + ko + ch * 16;
-                vp = v_base + vo + ch * 16;
-            }
-            kr[i] = load_global<u32x4>(kp);
-            vr[i] = load_global<u32x4>(vp);
-        }
         ok_next = info_ok[tile & 1];
+        if constexpr (Q8) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int at = tid + i * kThreads, r = at / CH, ch = at % CH;
+                Global kp = (Global)(uintptr_t)info[tile % 3][r][0] + ch * 16, vp = (Global)(uintptr_t)info[tile % 3][r][1] + ch * 16;
+                if (!WHOLE && ch * 16 >= D) kp = vp = zeros;
+                kr[i] = load_global<u32x4>(kp);
+                vr[i] = load_global<u32x4>(vp);
+            }
+        } else {
+            const uint32_t buffer = lds0 + (tile & 1) * 2 * TILE;
+#pragma unroll
+            for (int i = 0; i < DMAS; ++i) {
+                const int block = wave * DMAS + i, slot = block * 64 + lane, r = slot / CHL;
+                const int kc = slot % CHL ^ k_turn(r), vc = slot % CHL ^ v_turn(r);
+                Global kp = (Global)(uintptr_t)info[tile % 3][r][0] + kc * 16, vp = (Global)(uintptr_t)info[tile % 3][r][1] + vc * 16;
+                if (!WHOLE || DP * 2 < LS) {
+                    if (kc * 8 >= D) kp = zeros;
+                    if (vc * 8 >= D) vp = zeros;
+                }
+                global_to_lds(kp, buffer + block * 1024);
+                global_to_lds(vp, buffer + TILE + block * 1024);
+            }
+        }
     };
 
     if (tiles > 0) {
-        int32_t page = -1;
-        if (wave == 0) {
-            put_info(0, page_of(0));
-            put_scales(0);
-            put_info(1, page_of(1));
-            page = page_of(2);
+        int32_t page = page_of(wave);
+        if (wave < 2) {
+            put_info(wave, page);
+            page = page_of(wave + 4);
         }
+        if (wave == 0) put_scales(0);
         __syncthreads();
         load_tile(0);
+        const int k_at = col * LS + ((kg ^ k_turn(col)) << 4);
+        const int v_row = 4 * kg + (lane >> 2 & 3);
+        const int v_at = v_row * LS + (((lane >> 4 & 1) << 1 | (lane >> 1 & 1)) ^ v_turn(v_row)) * 16 + 8 * (lane & 1);
+        bool fresh = true;  // the maximum has to be looked for
         for (int it = 0; it < tiles; ++it) {
-            char* const kb = lds[it & 1][0];
-            char* const vb = lds[it & 1][1];
+            char* const kb = lds + (it & 1) * 2 * TILE;
+            char* const vb = kb + TILE;
             const uint64_t ok = uniform64(ok_next);
             // masked for some row of the workgroup?
             const int32_t j0 = it * kKeys + (it * kKeys < sinks ? 0 : gap), last = it * kKeys + kKeys - 1;
@@ -285,96 +330,124 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 return ~ok == 0 && j1 <= first_p && (!a.window || j1 < a.sinks || last_p - j0 < a.window);
             };
             const bool edge = !all_see(p_first, p_last);
+            if constexpr (Q8) {
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i) {
-                const int at = tid + i * kThreads, r = at / CH, ch = at % CH;
-                if constexpr (Q8) {
-                    *(u32x4*)(kb + r * PITCH + ch * 32) = i8_to_half<DT>(kr[i][0], kr[i][1]);
-                    *(u32x4*)(kb + r * PITCH + ch * 32 + 16) = i8_to_half<DT>(kr[i][2], kr[i][3]);
-                    *(u32x4*)(vb + r * PITCH + ch * 32) = i8_to_f16(vr[i][0], vr[i][1]);
-                    *(u32x4*)(vb + r * PITCH + ch * 32 + 16) = i8_to_f16(vr[i][2], vr[i][3]);
-                } else {
-                    *(u32x4*)(kb + r * PITCH + ch * 16) = kr[i];
-                    *(u32x4*)(vb + r * PITCH + ch * 16) = vr[i];
-                    if (edge && not_finite<DT>(vr[i])) atomicOr((unsigned long long*)&bad[it % 3], 1ull << r);
+                for (int i = 0; i < PIECES; ++i) {
+                    const int at = tid + i * kThreads, r = at / CH, ch = 2 * (at % CH);
+                    char* const kt = kb + r * LS;
+                    char* const vt = vb + r * LS;
+                    *(u32x4*)(kt + ((ch ^ k_turn(r)) << 4)) = i8_to_half<DT>(kr[i][0], kr[i][1]);
+                    *(u32x4*)(kt + ((ch + 1 ^ k_turn(r)) << 4)) = i8_to_half<DT>(kr[i][2], kr[i][3]);
+                    *(u32x4*)(vt + ((ch ^ v_turn(r)) << 4)) = i8_to_f16(vr[i][0], vr[i][1]);
+                    *(u32x4*)(vt + ((ch + 1 ^ v_turn(r)) << 4)) = i8_to_f16(vr[i][2], vr[i][3]);
+                }
+            } else {
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // this wave's part of the tile is in LDS
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < DMAS; ++i) {
+                        const int slot = (wave * DMAS + i) * 64 + lane, r = slot / CHL;
+                        const u32x4 v = *(const u32x4*)(vb + slot * 16);
+                        if (not_finite<DT>(v)) {
+                            *(u32x4*)(vb + slot * 16) = finite_only<DT>(v);
+                            atomicOr((unsigned long long*)&bad[it % 3], 1ull << r);
+                        }
+                    }
                 }
             }
             __syncthreads();
-            if (it + 1 < tiles) load_tile(it + 1);
-            if (wave == 0) {
-                put_scales(it + 1);
+            if (wave == ((it + 2) & 3)) {
                 put_info(it + 2, page);
-                page = page_of(it + 3);
+                page = page_of(it + 6);
                 if (lane == 0) bad[(it + 2) % 3] = 0;
             }
+            if (Q8 && wave == ((it + 1) & 3)) put_scales(it + 1);
+            if (it + 1 < tiles) load_tile(it + 1);
             // no row of this wave sees the tile
             if (j0 > w_last || (a.window && w_first - j1 >= a.window && j0 >= a.sinks)) continue;
 
-            // scores: lane (row, kg) holds keys 32 n + 8 (e / 4) + 4 kg + e % 4
-            f32x16 x[2];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[n][e] = 0.0f;
-#pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    x[n] = mma32<DT>(*(const u32x4*)(kb + (32 * n + col) * PITCH + (2 * s + kg) * 16), q[s], x[n]);
-            }
-            if constexpr (Q8) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 k4 = *(const f32x4*)&scales[it & 1][0][32 * n + 8 * i + 4 * kg];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) x[n][4 * i + r] *= k4[r];
-                    }
-            }
-            uint32_t hidden = 0;  // bit 16 n + e
             const bool masked = !all_see(w_first, w_last);
+            uint32_t hidden = 0;  // bit 16 n + e
             if (masked) {
+                const int kg4 = here(4 * kg);
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const int key = 32 * n + 8 * (e >> 2) + 4 * kg + (e & 3);
+                        const int key = 32 * n + 8 * (e >> 2) + kg4 + (e & 3);
                         const int32_t v = it * kKeys + key, j = v < sinks ? v : v + gap;
                         const bool sees = (ok >> key & 1) && j <= p && (!a.window || p - j < a.window || j < a.sinks);
                         hidden |= (uint32_t)!sees << (16 * n + e);
-                        if (!sees) x[n][e] = -__builtin_inff();
                     }
             }
             any |= hidden != ~0u;
-            float top = x[0][0];
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[n][e]);
-            top *= factor;
-            if (__builtin_amdgcn_ballot_w64(top > m + kSlack)) {
-                const float m2 = fmaxf(m, pair_max(top));
-                const float keep = __builtin_amdgcn_exp2f(m - m2);
-                m = m2;
-                l *= keep;
-#pragma unroll
-                for (int i = 0; i < NB; ++i) acc[i] *= keep;
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e], factor, -m));
-            if (masked) {
+            f32x16 x[2];
+            float sum;
+            for (;;) {
+                // scores: lane (row, kg) holds keys 32 n + 8 (e / 4) + 4 kg + e % 4
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[n][e] = hidden >> (16 * n + e) & 1 ? 0.0f : x[n][e];
+                    for (int e = 0; e < 16; ++e) x[n][e] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) x[n] = mma32<DT>(*(const u32x4*)(kb + (k_at ^ s << 5) + 32 * n * LS), q[s], x[n]);
+                // six reads ahead of the products, then one with each
+                __builtin_amdgcn_sched_group_barrier(kDsRead, 6, 0);
+#pragma unroll
+                for (int s = 0; s < 2 * KS - 6; ++s) {
+                    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(kMfma, 6, 0);
+                if constexpr (Q8) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const f32x4 k4 = *(const f32x4*)&scales[it & 1][0][32 * n + 8 * i + 4 * kg];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) x[n][4 * i + r] *= k4[r];
+                        }
+                }
+                if (fresh) {
+                    const uint32_t shut = here(hidden);
+                    float top = -__builtin_inff();
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) top = fmaxf(top, shut >> (16 * n + e) & 1 ? -__builtin_inff() : x[n][e]);
+                    const float m2 = fmaxf(m, pair_max(top) * factor);
+                    const float keep = __builtin_amdgcn_exp2f(m - m2);
+                    m = m2;
+                    l *= keep;
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) acc[i] *= keep;
+                }
+                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e], factor, -m));
+                if (masked) {
+                    const uint32_t shut = here(hidden);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[n][e] = shut >> (16 * n + e) & 1 ? 0.0f : x[n][e];
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) part[e & 3] += x[n][e];
+                sum = (part[0] + part[1]) + (part[2] + part[3]);
+                if (fresh || !__builtin_amdgcn_ballot_w64(!(sum <= kMostSum))) break;
+                fresh = true;
             }
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) l += x[n][e];
+            fresh = false;
+            l += sum;
             if constexpr (Q8) {
-                auto scale_of = [&](int n, int e, float v) { return masked && (hidden >> (16 * n + e) & 1) ? 0.0f : v; };
                 float most = 0.0f;
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
@@ -383,7 +456,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                         const f32x4 v4 = *(const f32x4*)&scales[it & 1][1][32 * n + 8 * i + 4 * kg];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const float v = scale_of(n, 4 * i + r, v4[r]);
+                            const float v = hidden >> (16 * n + 4 * i + r) & 1 ? 0.0f : v4[r];
                             most = fmaxf(most, fabsf(v));
                             x[n][4 * i + r] *= v;
                         }
@@ -401,57 +474,54 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[n][e] *= v_inv;
             }
-            // acc += V^T P^T; CLEAN: without the values of V that are not finite
-            auto second = [&](auto clean) {
+            if constexpr (!Q8) {
+                for (uint64_t left = edge ? uniform64(bad[it % 3]) : 0; left; left &= left - 1) {
+                    const int key = __builtin_ctzll(left), kg4 = here(4 * kg);
+                    // this row's weight of the key, from whichever of the two lanes holds it, and whether it is seen
+                    float w = 0.0f;
+                    bool sees = false;
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const int n = s >> 1, e0 = 8 * (s & 1);
-                    u32x4 pw;
+                    for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) pw[i] = pack2<PV>(x[n][e0 + 2 * i], x[n][e0 + 2 * i + 1]);
-                    const char* const from = vb + (16 * s + 4 * kg + (lane >> 2 & 3)) * PITCH + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) {
-                        const u32x2 lo = lds_tr16(from + 64 * i), hi = lds_tr16(from + 8 * PITCH + 64 * i);
-                        u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
-                        if constexpr (decltype(clean)::value) v = finite_only<DT>(v);
-                        acc[i] = mma32<PV>(v, pw, acc[i]);
-                    }
-                }
-            };
-            if constexpr (Q8) {
-                second(std::false_type());
-            } else {
-                uint64_t left = masked ? uniform64(bad[it % 3]) : 0;
-                if (!left) {
-                    second(std::false_type());
-                } else {
-                    second(std::true_type());
-                    for (; left; left &= left - 1) {
-                        const int key = __builtin_ctzll(left);
-                        // this row's weight of the key, from whichever of the two lanes holds it, and whether it is seen
-                        float w = 0.0f;
-                        bool sees = false;
-#pragma unroll
-                        for (int n = 0; n < 2; ++n)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (key == 32 * n + 8 * (e >> 2) + 4 * kg + (e & 3)) {
-                                    w = x[n][e];
-                                    sees = !(hidden >> (16 * n + e) & 1);
-                                }
-                        w = pair_sum(w);
-                        sees = pair_max(sees ? 1.0f : 0.0f) != 0.0f;
-#pragma unroll
-                        for (int i = 0; i < NB; ++i)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const uint32_t bits = *(const uint16_t*)(vb + key * PITCH + (32 * i + 8 * (e >> 2) + 4 * kg + (e & 3)) * 2);
-                                if (sees && (bits & exponent_of<DT>()) == exponent_of<DT>()) acc[i][e] += w * load_half_bits(bits, DT);
+                        for (int e = 0; e < 16; ++e)
+                            if (key == 32 * n + 8 * (e >> 2) + kg4 + (e & 3)) {
+                                w = x[n][e];
+                                sees = !(hidden >> (16 * n + e) & 1);
                             }
-                    }
+                    w = pair_sum(w);
+                    sees = pair_max(sees ? 1.0f : 0.0f) != 0.0f;
+                    const Global row = (Global)(uintptr_t)info[it % 3][key][1];
+#pragma unroll
+                    for (int i = 0; i < NB; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int d = 32 * i + 8 * (e >> 2) + kg4 + (e & 3);
+                            const uint32_t bits = WHOLE || d < D ? load_global<uint16_t>(row + d * 2) : 0;
+                            if (sees && (bits & exponent_of<DT>()) == exponent_of<DT>()) acc[i][e] += w * load_half_bits(bits, DT);
+                        }
                 }
             }
+            // acc += V^T P^T
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int n = s >> 1, e0 = 8 * (s & 1);
+                u32x4 pw;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pw[i] = pack2<PV>(x[n][e0 + 2 * i], x[n][e0 + 2 * i + 1]);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    const char* const from = vb + (v_at ^ i << 6) + 16 * s * LS;
+                    const u32x2 lo = lds_tr16(from), hi = lds_tr16(from + 8 * LS);
+                    acc[i] = mma32<PV>((u32x4){lo[0], lo[1], hi[0], hi[1]}, pw, acc[i]);
+                }
+            }
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 1);
+#pragma unroll
+            for (int s = 0; s < 4 * NB - 4; ++s) {
+                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
+                __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
+            }
+            __builtin_amdgcn_sched_group_barrier(kMfma, 4, 1);
         }
     }
 
