@@ -51,10 +51,12 @@ struct AttnArgs {
 // One token per sequence (cu_q == nullptr), keys in pages.
 size_t attention_decode_workspace(int64_t batch, int64_t q_heads, const qk_kv_cache& c, int64_t table_width, int64_t window,
                                   int64_t sinks);
-hipError_t launch_attention_decode(const AttnArgs& a, void* workspace, size_t workspace_bytes, hipStream_t stream);
+hipError_t launch_attention_decode(const AttnArgs& a, void* workspace, hipStream_t stream);
 
 // Ragged prompts (cu_q != nullptr).
-hipError_t launch_attention_prompt(const AttnArgs& a, hipStream_t stream);
+size_t attention_prompt_workspace(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache& c, int64_t table_width,
+                                  int64_t window, int64_t sinks);
+hipError_t launch_attention_prompt(const AttnArgs& a, void* workspace, hipStream_t stream);
 
 struct MropeArgs {
     const void *q, *k, *v;

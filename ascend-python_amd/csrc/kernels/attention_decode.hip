@@ -485,7 +485,7 @@ size_t attention_decode_workspace(int64_t batch, int64_t q_heads, const qk_kv_ca
     return (size_t)(p.arrivals_bytes + p.part_bytes);
 }
 
-hipError_t launch_attention_decode(const AttnArgs& a, void* workspace, size_t, hipStream_t stream) {
+hipError_t launch_attention_decode(const AttnArgs& a, void* workspace, hipStream_t stream) {
     const Plan p = plan(a.batch, a.q_heads, a.kv.c, a.kv.table_width, a.window, a.sinks);
     DecodeArgs g = {};
     g.a = a;

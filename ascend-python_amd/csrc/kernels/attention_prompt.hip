@@ -25,6 +25,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRows = 128;   // query rows per workgroup
 constexpr int kKeys = 64;    // keys per tile
+// A tile's keys are cut, where there are few tiles, into parts of at least so many steps: a part costs its write and its
+// share of the join.
+constexpr int kSplitTiles = 8;
+constexpr int64_t kResident = 512;  // workgroups that the card holds, two per CU
 // A lane's 32 weights of a tile may sum to this before the maximum is looked for again: far inside the range of either
 // 16-bit type and of the fp32 sums.
 constexpr float kMostSum = 4096.0f;
@@ -56,6 +60,11 @@ __device__ __forceinline__ void global_to_lds(Global from, uint32_t lds) {
 struct PromptArgs {
     AttnArgs a;
     Div31 group_div;  // q_heads / kv_heads
+    int splits;       // at most: parts that a tile's keys are cut into
+    uint64_t tag;
+    uint64_t* arrivals;   // a counter for every tile and key-value head
+    float* parts;         // [tile and head][splits][kRows * (DP + 2)], in the order of the registers
+    int64_t part_bytes;   // of one of them
 };
 
 // Rows of tokens and keys of sequence b (b == batch: the rows past the last sequence, which see nothing)
@@ -145,7 +154,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         __syncthreads();
         for (int w = 0; w < wave; ++w) in += sums[w];
         const int64_t total = sums[0] + sums[1] + sums[2] + sums[3];
-        const int64_t rank = total - 1 - blockIdx.x / (uint32_t)c.kv_heads;
+        const int64_t rank = total - 1 - blockIdx.x / (uint32_t)(c.kv_heads * g.splits);
         if (rank < 0) return;
         int64_t at = in - mine;
         for (int64_t b = b0; b < b1; ++b) {
@@ -198,7 +207,13 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     }
     const int32_t gap = low - sinks;
     const int32_t places = p_last < 0 ? 0 : p_last + 1 - gap;
-    const int tiles = (places + kKeys - 1) / kKeys;
+    const int all_tiles = (places + kKeys - 1) / kKeys;
+    // this workgroup's part of them
+    const int split = (int)(blockIdx.x / (uint32_t)c.kv_heads % (uint32_t)g.splits);
+    int splits = (all_tiles + kSplitTiles - 1) / kSplitTiles;
+    splits = splits < 1 ? 1 : splits < g.splits ? splits : g.splits;
+    if (split >= splits) return;
+    const int tile0 = (int)((int64_t)all_tiles * split / splits), tiles = (int)((int64_t)all_tiles * (split + 1) / splits);
 
     // the largest score is found before the scale is applied: a negative scale's sign goes to the query
     const uint32_t turned = a.scale < 0.0f ? 0x80008000u : 0u;
@@ -306,20 +321,22 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         }
     };
 
-    if (tiles > 0) {
-        int32_t page = page_of(wave);
-        if (wave < 2) {
-            put_info(wave, page);
-            page = page_of(wave + 4);
+    const bool no_rows = wave * 32 >= rows;  // for this wave
+    if (tile0 < tiles) {
+        const int turn = wave - tile0 & 3;  // tiles tile0 + turn, + 4, ... are this wave's to find
+        int32_t page = page_of(tile0 + turn);
+        if (turn < 2) {
+            put_info(tile0 + turn, page);
+            page = page_of(tile0 + turn + 4);
         }
-        if (wave == 0) put_scales(0);
+        if (turn == 0) put_scales(tile0);
         __syncthreads();
-        load_tile(0);
+        load_tile(tile0);
         const int k_at = col * LS + ((kg ^ k_turn(col)) << 4);
         const int v_row = 4 * kg + (lane >> 2 & 3);
         const int v_at = v_row * LS + (((lane >> 4 & 1) << 1 | (lane >> 1 & 1)) ^ v_turn(v_row)) * 16 + 8 * (lane & 1);
         bool fresh = true;  // the maximum has to be looked for
-        for (int it = 0; it < tiles; ++it) {
+        for (int it = tile0; it < tiles; ++it) {
             char* const kb = lds + (it & 1) * 2 * TILE;
             char* const vb = kb + TILE;
             const uint64_t ok = uniform64(ok_next);
@@ -364,7 +381,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             if (Q8 && wave == ((it + 1) & 3)) put_scales(it + 1);
             if (it + 1 < tiles) load_tile(it + 1);
             // no row of this wave sees the tile
-            if (j0 > w_last || (a.window && w_first - j1 >= a.window && j0 >= a.sinks)) continue;
+            if (no_rows || j0 > w_last || (a.window && w_first - j1 >= a.window && j0 >= a.sinks)) continue;
 
             const bool masked = !all_see(w_first, w_last);
             uint32_t hidden = 0;  // bit 16 n + e
@@ -527,8 +544,60 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
 
     l = pair_sum(l);
     any = pair_max(any ? 1.0f : 0.0f) != 0.0f;
+    if (Q8) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) acc[i] *= v_top;
+    }
+    if (splits > 1) {
+        const int64_t place = (blockIdx.x / (uint32_t)(c.kv_heads * g.splits)) * c.kv_heads + kvh;
+        // in the order of the registers: whole lines, and the joining lane finds its own rows
+        constexpr uint32_t SUMS = 4 * NB * 4 * 1024;
+        auto part = [&](int s) { return make_rsrc((const char*)g.parts + (place * g.splits + s) * g.part_bytes, (uint32_t)g.part_bytes); };
+        const __amdgpu_buffer_rsrc_t own = part(split);
+        if (!no_rows) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    __builtin_amdgcn_raw_buffer_store_b128(
+                        __builtin_bit_cast(u32x4, (f32x4){acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]}), own,
+                        lane * 16, ((wave * NB + i) * 4 + e) * 1024, kCoherent);
+            if (kg == 0)
+                __builtin_amdgcn_raw_buffer_store_b64((u32x2){__float_as_uint(any ? m : -__builtin_inff()), __float_as_uint(l)}, own,
+                                                      SUMS + (wave * 32 + col) * 8, 0, kCoherent);
+        }
+        if (!splitk_last(g.arrivals + place, (uint32_t)splits, g.tag)) return;
+        m = -__builtin_inff();
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
+        if (!no_rows) {
+            for (int s = 0; s < splits; ++s) {
+                const __amdgpu_buffer_rsrc_t rs = part(s);
+                f32x4 v[NB][4];
+                const u32x2 ml = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, SUMS + (wave * 32 + col) * 8, 0, kCoherent));
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        v[i][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, lane * 16, ((wave * NB + i) * 4 + e) * 1024, kCoherent));
+                const float pm = __uint_as_float(ml[0]), m2 = fmaxf(m, pm);
+                const bool none = pm == -__builtin_inff();
+                const float keep = none ? 1.0f : __builtin_amdgcn_exp2f(m - m2), f = none ? 0.0f : __builtin_amdgcn_exp2f(pm - m2);
+                m = m2;
+                l = l * keep + (none ? 0.0f : __uint_as_float(ml[1]) * f);
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[i][e] = none ? acc[i][e] : acc[i][e] * keep + v[i][e >> 2][e & 3] * f;
+            }
+        }
+        any = m != -__builtin_inff();
+    }
     if (wave * 32 + col >= rows) return;
-    const float inv = (Q8 ? v_top : 1.0f) / l;
+    const float inv = 1.0f / l;
     const int64_t o = t * a.q_heads + h;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
@@ -559,23 +628,60 @@ void launch_type(const PromptArgs& g, int64_t grid, hipStream_t stream) {
     else launch_width<256, DT, Q8>(g, grid, stream);
 }
 
+struct Plan {
+    int64_t grid, arrivals_bytes, part_bytes;
+    int splits;
+};
+
+Plan plan(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache& c, int64_t table_width, int64_t window, int64_t sinks) {
+    Plan p = {};
+    const int64_t group = q_heads / c.kv_heads;
+    // at most: whole tiles, and a last one for every sequence and for the rows past them
+    const int64_t some = batch < tokens ? batch : tokens;
+    const int64_t tiles = (tokens * group / kRows + some + 1) * c.kv_heads;
+    int64_t most = (table_width ? table_width : 1) * c.page_size;
+    if (window && most > window && most - window > sinks + kRows) most = window + sinks + kRows;
+    const int64_t steps = (most + kKeys - 1) / kKeys;
+    int64_t splits = kResident / tiles;
+    if (splits > steps / kSplitTiles) splits = steps / kSplitTiles;
+    p.splits = splits < 1 ? 1 : (int)splits;
+    p.grid = tiles * p.splits;
+    if (p.splits > 1) {
+        const int64_t D = c.head_dim, width = D <= 64 ? 64 : D <= 96 && c.dtype != QK_I8 ? 96 : D <= 128 ? 128 : D <= 192 ? 192 : 256;
+        p.arrivals_bytes = (tiles * 8 + 255) / 256 * 256;
+        p.part_bytes = kRows * (width + 2) * 4;
+    }
+    return p;
+}
+
 }  // namespace
 
-hipError_t launch_attention_prompt(const AttnArgs& a, hipStream_t stream) {
+size_t attention_prompt_workspace(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache& c, int64_t table_width,
+                                  int64_t window, int64_t sinks) {
+    if (tokens == 0) return 0;
+    const Plan p = plan(tokens, batch, q_heads, c, table_width, window, sinks);
+    return (size_t)(p.arrivals_bytes + p.grid * p.part_bytes);
+}
+
+hipError_t launch_attention_prompt(const AttnArgs& a, void* workspace, hipStream_t stream) {
+    const Plan p = plan(a.tokens, a.batch, a.q_heads, a.kv.c, a.kv.table_width, a.window, a.sinks);
     PromptArgs g = {};
     g.a = a;
-    const int64_t group = a.q_heads / a.kv.c.kv_heads;
-    g.group_div = div31((uint32_t)group);
-    // at most: whole tiles, and a last one for every sequence and for the rows past them
-    const int64_t some = a.batch < a.tokens ? a.batch : a.tokens;
-    const int64_t grid = (a.tokens * group / kRows + some + 1) * a.kv.c.kv_heads;
+    g.group_div = div31((uint32_t)(a.q_heads / a.kv.c.kv_heads));
+    g.splits = p.splits;
+    if (p.splits > 1) {
+        g.tag = next_split_tag();
+        g.arrivals = (uint64_t*)workspace;
+        g.parts = (float*)((char*)workspace + p.arrivals_bytes);
+        g.part_bytes = p.part_bytes;
+    }
     const bool q8 = a.kv.c.dtype == QK_I8;
     if (a.dtype == QK_BF16) {
-        if (q8) launch_type<QK_BF16, true>(g, grid, stream);
-        else launch_type<QK_BF16, false>(g, grid, stream);
+        if (q8) launch_type<QK_BF16, true>(g, p.grid, stream);
+        else launch_type<QK_BF16, false>(g, p.grid, stream);
     } else {
-        if (q8) launch_type<QK_F16, true>(g, grid, stream);
-        else launch_type<QK_F16, false>(g, grid, stream);
+        if (q8) launch_type<QK_F16, true>(g, p.grid, stream);
+        else launch_type<QK_F16, false>(g, p.grid, stream);
     }
     return hipGetLastError();
 }

@@ -206,7 +206,7 @@ int qk_paged_attention(const void* query, int dtype, int64_t batch, int64_t q_he
     size_t need = 0;
     if (int rc = qk_paged_attention_workspace_size(batch, q_heads, cache, table_width, window, sinks, &need)) return rc;
     if (int rc = check_workspace(op, need, workspace, workspace_bytes)) return rc;
-    return launched(qk::launch_attention_decode(a, workspace, workspace_bytes, (hipStream_t)stream), op);
+    return launched(qk::launch_attention_decode(a, workspace, (hipStream_t)stream), op);
 }
 
 int qk_prompt_attention_workspace_size(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache* cache,
@@ -217,7 +217,7 @@ int qk_prompt_attention_workspace_size(int64_t tokens, int64_t batch, int64_t q_
     if (int rc = check_attention_sizes(op, tokens, batch, q_heads, cache, cache && cache->dtype != QK_I8 ? cache->dtype : QK_BF16,
                                        table_width, window, sinks))
         return rc;
-    *bytes = 0;
+    *bytes = qk::attention_prompt_workspace(tokens, batch, q_heads, *cache, table_width, window, sinks);
     return QK_OK;
 }
 
@@ -254,7 +254,7 @@ int qk_prompt_attention(const void* query, int dtype, int64_t tokens, int64_t ba
     size_t need = 0;
     if (int rc = qk_prompt_attention_workspace_size(tokens, batch, q_heads, cache, table_width, window, sinks, &need)) return rc;
     if (int rc = check_workspace(op, need, workspace, workspace_bytes)) return rc;
-    return launched(qk::launch_attention_prompt(a, (hipStream_t)stream), op);
+    return launched(qk::launch_attention_prompt(a, workspace, (hipStream_t)stream), op);
 }
 
 int qk_mrope(const void* query, const void* key, const void* value, int dtype, int64_t tokens, int64_t q_heads,
