@@ -9,11 +9,11 @@
 // maximum and sum need one exchange between lane pairs, and the weights as they lie are the right operand of V^T times P^T.
 // K and V go straight from memory into two LDS buffers (an int8 cache through registers, where it becomes 16-bit), the 16-byte
 // pieces of a row exchanged so that neither the reads of K nor the transposing reads of V meet in a bank.  One barrier per
-// 64 keys: the next rows are on their way while these are worked on.  Where a row of the cache lies is found two tiles
+// 64 keys: the next rows are on their way while these are worked on.  Where a row of the cache lies is found three tiles
 // ahead, a lane per row, by the waves in turn.
 //
-// The running maximum is not looked for in every tile: the weights are taken against the one there is, and only where their sum
-// shows that a score lies far above it are the scores made again and the maximum moved.
+// The next tile's scores are made between the exponentials of this one, so that a wave keeps both pipes busy.  The running
+// maximum moves only where a score lies far above it: most tiles rescale nothing and need no exchange between lanes.
 //
 // A masked weight is 0, but 0 times a NaN or an infinity in V is NaN: tiles that are masked for some rows look for such
 // values once they are staged, and the values are added apart, for the rows that see them.
@@ -29,12 +29,6 @@ constexpr int kKeys = 64;    // keys per tile
 // share of the join.
 constexpr int kSplitTiles = 8;
 constexpr int64_t kResident = 512;  // workgroups that the card holds, two per CU
-// A lane's 32 weights of a tile may sum to this before the maximum is looked for again: far inside the range of either
-// 16-bit type and of the fp32 sums.
-constexpr float kMostSum = 4096.0f;
-
-constexpr int kMfma = 0x8, kDsRead = 0x100;  // instruction groups of the scheduler
-
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <int DT>
@@ -44,6 +38,15 @@ __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+
+// 16 bytes from LDS address `at` + offset; and 8 of them as lds_tr16
+__device__ __forceinline__ u32x4 lds_load(uint32_t at, int offset) {
+    return *(const __attribute__((address_space(3))) u32x4*)((const __attribute__((address_space(3))) char*)(uintptr_t)at + offset);
+}
+__device__ __forceinline__ u32x2 lds_tr16(uint32_t at, int offset) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) i16x4*)((__attribute__((address_space(3))) char*)(uintptr_t)at + offset)));
 }
 
 // v, as a value that is made here: what follows from it is not computed ahead of the loop, where it would hold registers.
@@ -125,15 +128,15 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     static_assert(!Q8 || kKeys * CH % kThreads == 0, "");
     constexpr int TILE = kKeys * LS;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];  // buffer 0: K, V; buffer 1: K, V
-    __shared__ __attribute__((aligned(16))) uint64_t info[3][kKeys][2];  // addresses of a key's and a value's row (none: of zeros)
-    __shared__ uint64_t info_ok[2];              // which keys of the tile exist
+    __shared__ __attribute__((aligned(16))) uint64_t info[4][kKeys][2];  // addresses of a key's and a value's row (none: of zeros)
+    __shared__ uint64_t info_ok[4];              // which keys of the tile exist
     __shared__ uint64_t bad[3];                  // which rows of V hold a NaN or an infinity
-    __shared__ float scales[2][2][kKeys];
+    __shared__ float scales[4][2][kKeys];
     __shared__ int64_t found[2];
 
     const AttnArgs& a = g.a;
     const qk_kv_cache& c = a.kv.c;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, kg = lane >> 5;
     const int D = (int)c.head_dim, G = (int)(a.q_heads / c.kv_heads);
     const int kvh = (int)(blockIdx.x % (uint32_t)c.kv_heads);
@@ -232,13 +235,19 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
     float m = kLowest, l = 0.0f, v_top = 0x1p-100f, v_inv = 0x1p100f;
     bool any = false;
-    const float factor = fabsf(a.scale) * kLog2e;
+    // (a scale of 0 becomes one that leaves every product 0: -inf, a masked score, must stay what it is)
+    const float factor = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(fabsf(a.scale) * kLog2e, 0x1p-120f))));
 
-    const int32_t* const table = a.kv.table ? a.kv.table + b * a.kv.table_stride : nullptr;
+    const bool paged = a.kv.table != nullptr;
     const Global zeros = global_address(kZeroRow);
-    const Global k_base = global_address(c.key) + kvh * c.key_head_stride * ES;
-    const Global v_base = global_address(c.value) + kvh * c.value_head_stride * ES;
-
+    // What finds the rows' places reads its arguments from memory again each time: they would hold scalar registers that the
+    // loop has better use for.
+    auto args = []() {
+        const __attribute__((address_space(4))) PromptArgs* from =
+            (const __attribute__((address_space(4))) PromptArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(from));
+        return from;
+    };
     // a lane per row of a tile: its page, then its place in memory and its scales
     auto place = [&](int tile) {
         const int32_t v = tile * kKeys + lane;
@@ -246,28 +255,33 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     };
     auto page_of = [&](int tile) {
         const int32_t j = place(tile);
-        return table && j >= 0 ? table[div31(j, a.kv.page_div)] : -1;
+        if (!paged || j < 0) return (int32_t)-1;
+        const auto* g = args();
+        const Global table = global_address(g->a.kv.table + b * g->a.kv.table_stride);
+        return load_global<int32_t>(table + (int64_t)div31(j, (Div31){g->a.kv.page_div.m, g->a.kv.page_div.s}) * 4);
     };
     float ks_next = 0.0f, vs_next = 0.0f;
     auto put_info = [&](int tile, int32_t page) {
+        const auto* g = args();
+        const auto& c = g->a.kv.c;
         const int32_t j = place(tile);
         int32_t slot = key0 + j;
         bool valid = j >= 0;
-        if (table) {
-            slot = j - div31(j, a.kv.page_div) * (int32_t)c.page_size;
+        if (paged) {
+            slot = j - div31(j, (Div31){g->a.kv.page_div.m, g->a.kv.page_div.s}) * (int32_t)c.page_size;
             valid = valid && page >= 0 && page < c.num_pages;
         } else {
             page = 0;
         }
         Global kp = zeros, vp = zeros;
         if (valid) {
-            kp = k_base + (page * c.key_page_stride + slot * c.key_token_stride) * ES;
-            vp = v_base + (page * c.value_page_stride + slot * c.value_token_stride) * ES;
+            kp = global_address(c.key) + (page * c.key_page_stride + slot * c.key_token_stride + kvh * c.key_head_stride) * ES;
+            vp = global_address(c.value) + (page * c.value_page_stride + slot * c.value_token_stride + kvh * c.value_head_stride) * ES;
         }
-        info[tile % 3][lane][0] = (uint64_t)(uintptr_t)kp;
-        info[tile % 3][lane][1] = (uint64_t)(uintptr_t)vp;
+        info[tile & 3][lane][0] = (uint64_t)(uintptr_t)kp;
+        info[tile & 3][lane][1] = (uint64_t)(uintptr_t)vp;
         const uint64_t ok = __builtin_amdgcn_ballot_w64(valid);
-        if (lane == 0) info_ok[tile & 1] = ok;
+        if (lane == 0) info_ok[tile & 3] = ok;
         if constexpr (Q8) {
             Global kz = zeros, vz = zeros;
             if (valid) {
@@ -282,8 +296,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     };
     auto put_scales = [&](int tile) {
         if constexpr (Q8) {
-            scales[tile & 1][0][lane] = ks_next;
-            scales[tile & 1][1][lane] = vs_next;
+            scales[tile & 3][0][lane] = ks_next;
+            scales[tile & 3][1][lane] = vs_next;
         }
     };
 
@@ -291,32 +305,48 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     auto k_turn = [](int r) { return CHL == 8 ? r >> 1 & 7 : r & 15; };
     auto v_turn = [](int r) { return CHL == 8 ? (r >> 1 & 3) << 1 : (r & 7) << 1; };
     u32x4 kr[PIECES], vr[PIECES];
-    uint64_t ok_next = 0;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-    auto load_tile = [&](int tile) {
-        ok_next = info_ok[tile & 1];
+    const int k_piece = (lane % CHL ^ k_turn(lane / CHL)) << 4, v_piece = (lane % CHL ^ v_turn(lane / CHL)) << 4;
+    const int lane_rows = (wave * 16 + lane / CHL) * 2;
+    // Addresses of this lane's pieces of K (which 0) or V (1) of a tile, and piece i on its way to LDS buffer tile & 1.
+    // Load i of the wave fills rows i * R + lane / CHL of its 16; the turn of a sum of rows is the turns' exclusive or.
+    constexpr int R = 64 / CHL;
+    auto address = [&](int tile, int which, int i) {
+        const int ch = (which ? v_piece : k_piece) ^ (which ? v_turn(i * R) : k_turn(i * R)) << 4;
+        Global from = (Global)(uintptr_t)(&info[tile & 3][0][which] + lane_rows)[i * R * 2] + ch;
+        if (!WHOLE || DP * 2 < LS) {
+            if (ch >= D * 2) from = zeros;
+        }
+        return from;
+    };
+    auto send = [&](int tile, int which, int i, Global from) {
+        global_to_lds(from, lds0 + (2 * (tile & 1) + which) * TILE + (wave * DMAS + i) * 1024);
+    };
+    // the whole of it; int8: into registers
+    auto load_tile = [&](int tile, int which) {
         if constexpr (Q8) {
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
                 const int at = tid + i * kThreads, r = at / CH, ch = at % CH;
-                Global kp = (Global)(uintptr_t)info[tile % 3][r][0] + ch * 16, vp = (Global)(uintptr_t)info[tile % 3][r][1] + ch * 16;
-                if (!WHOLE && ch * 16 >= D) kp = vp = zeros;
-                kr[i] = load_global<u32x4>(kp);
-                vr[i] = load_global<u32x4>(vp);
+                Global from = (Global)(uintptr_t)info[tile & 3][r][which] + ch * 16;
+                if (!WHOLE && ch * 16 >= D) from = zeros;
+                (which ? vr : kr)[i] = load_global<u32x4>(from);
             }
         } else {
-            const uint32_t buffer = lds0 + (tile & 1) * 2 * TILE;
 #pragma unroll
-            for (int i = 0; i < DMAS; ++i) {
-                const int block = wave * DMAS + i, slot = block * 64 + lane, r = slot / CHL;
-                const int kc = slot % CHL ^ k_turn(r), vc = slot % CHL ^ v_turn(r);
-                Global kp = (Global)(uintptr_t)info[tile % 3][r][0] + kc * 16, vp = (Global)(uintptr_t)info[tile % 3][r][1] + vc * 16;
-                if (!WHOLE || DP * 2 < LS) {
-                    if (kc * 8 >= D) kp = zeros;
-                    if (vc * 8 >= D) vp = zeros;
-                }
-                global_to_lds(kp, buffer + block * 1024);
-                global_to_lds(vp, buffer + TILE + block * 1024);
+            for (int i = 0; i < DMAS; ++i) send(tile, which, i, address(tile, which, i));
+        }
+    };
+    // int8: K or V of a tile from the registers, as 16-bit values
+    auto store_tile = [&](int tile, int which) {
+        if constexpr (Q8) {
+            char* const buffer = lds + (2 * (tile & 1) + which) * TILE;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int at = tid + i * kThreads, r = at / CH, ch = 2 * (at % CH), turn = which ? v_turn(r) : k_turn(r);
+                const u32x4 w = (which ? vr : kr)[i];
+                *(u32x4*)(buffer + r * LS + ((ch ^ turn) << 4)) = which ? i8_to_f16(w[0], w[1]) : i8_to_half<DT>(w[0], w[1]);
+                *(u32x4*)(buffer + r * LS + ((ch + 1 ^ turn) << 4)) = which ? i8_to_f16(w[2], w[3]) : i8_to_half<DT>(w[2], w[3]);
             }
         }
     };
@@ -325,21 +355,45 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     if (tile0 < tiles) {
         const int turn = wave - tile0 & 3;  // tiles tile0 + turn, + 4, ... are this wave's to find
         int32_t page = page_of(tile0 + turn);
-        if (turn < 2) {
+        if (turn < 3) {
             put_info(tile0 + turn, page);
             page = page_of(tile0 + turn + 4);
+            if (turn < 2) put_scales(tile0 + turn);
         }
-        if (turn == 0) put_scales(tile0);
         __syncthreads();
-        load_tile(tile0);
+        load_tile(tile0, 0);
+        if constexpr (Q8) {
+            store_tile(tile0, 0);
+            load_tile(tile0 + 1, 0);
+            load_tile(tile0, 1);
+        } else {
+            if (tile0 + 1 < tiles) load_tile(tile0 + 1, 0);
+            load_tile(tile0, 1);
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        }
+        __syncthreads();
+
         const int k_at = col * LS + ((kg ^ k_turn(col)) << 4);
         const int v_row = 4 * kg + (lane >> 2 & 3);
         const int v_at = v_row * LS + (((lane >> 4 & 1) << 1 | (lane >> 1 & 1)) ^ v_turn(v_row)) * 16 + 8 * (lane & 1);
-        bool fresh = true;  // the maximum has to be looked for
-        for (int it = tile0; it < tiles; ++it) {
-            char* const kb = lds + (it & 1) * 2 * TILE;
-            char* const vb = kb + TILE;
-            const uint64_t ok = uniform64(ok_next);
+        // scores of a tile: lane (row, kg) holds keys 32 n + 8 (e / 4) + 4 kg + e % 4
+        auto scores = [&](int tile, f32x16 (&x)[2]) {
+            const char* const kb = lds + 2 * (tile & 1) * TILE;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[n][e] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) x[n] = mma32<DT>(*(const u32x4*)(kb + (k_at ^ s << 5) + 32 * n * LS), q[s], x[n]);
+        };
+
+        // One step: the tile's weights from its scores x, while the next tile's scores are made (into y), then its values.
+        // K of the next tile and V of this one are in LDS at its barrier.
+        auto step = [&](int it, f32x16 (&x)[2], f32x16 (&y)[2]) {
+            char* const vb = lds + (2 * (it & 1) + 1) * TILE;
+            const uint64_t ok = uniform64(info_ok[it & 3]);
             // masked for some row of the workgroup?
             const int32_t j0 = it * kKeys + (it * kKeys < sinks ? 0 : gap), last = it * kKeys + kKeys - 1;
             const int32_t j1 = last + (last < sinks ? 0 : gap);
@@ -348,18 +402,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             };
             const bool edge = !all_see(p_first, p_last);
             if constexpr (Q8) {
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i) {
-                    const int at = tid + i * kThreads, r = at / CH, ch = 2 * (at % CH);
-                    char* const kt = kb + r * LS;
-                    char* const vt = vb + r * LS;
-                    *(u32x4*)(kt + ((ch ^ k_turn(r)) << 4)) = i8_to_half<DT>(kr[i][0], kr[i][1]);
-                    *(u32x4*)(kt + ((ch + 1 ^ k_turn(r)) << 4)) = i8_to_half<DT>(kr[i][2], kr[i][3]);
-                    *(u32x4*)(vt + ((ch ^ v_turn(r)) << 4)) = i8_to_f16(vr[i][0], vr[i][1]);
-                    *(u32x4*)(vt + ((ch + 1 ^ v_turn(r)) << 4)) = i8_to_f16(vr[i][2], vr[i][3]);
-                }
+                store_tile(it + 1, 0);
+                store_tile(it, 1);
             } else {
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // this wave's part of the tile is in LDS
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // this wave's part is in LDS
                 if (edge) {
 #pragma unroll
                     for (int i = 0; i < DMAS; ++i) {
@@ -373,19 +419,43 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 }
             }
             __syncthreads();
-            if (wave == ((it + 2) & 3)) {
-                put_info(it + 2, page);
-                page = page_of(it + 6);
+            if (Q8 && wave == (it + 2 & 3)) put_scales(it + 2);
+            if (wave == (it + 3 & 3)) {
+                put_info(it + 3, page);
+                page = page_of(it + 7);
                 if (lane == 0) bad[(it + 2) % 3] = 0;
             }
-            if (Q8 && wave == ((it + 1) & 3)) put_scales(it + 1);
-            if (it + 1 < tiles) load_tile(it + 1);
-            // no row of this wave sees the tile
-            if (no_rows || j0 > w_last || (a.window && w_first - j1 >= a.window && j0 >= a.sinks)) continue;
+            // What is sent for: K two tiles on, V one (past the last: a row of zeros, or one that is not used).  The 16-bit loads go out
+            // between the products, their addresses being read here.
+            constexpr int SENDS = Q8 ? 1 : 2 * DMAS;
+            Global from[SENDS];
+            if (Q8 || no_rows) {
+                load_tile(it + 2, 0);
+                load_tile(it + 1, 1);
+                if (no_rows) return;
+            } else {
+#pragma unroll
+                for (int i = 0; i < SENDS; ++i) from[i] = address(i < DMAS ? it + 2 : it + 1, i / DMAS, i % DMAS);
+            }
+            constexpr int AHEAD1 = 6;
+            const uint32_t k_from = lds0 + 2 * (it + 1 & 1) * TILE + here(k_at);
+            auto k_operand = [&](int i) { return lds_load(k_from ^ (i >> 1) << 5, 32 * (i & 1) * LS); };
+            u32x4 k_ring[AHEAD1];
+#pragma unroll
+            for (int i = 0; i < AHEAD1; ++i) k_ring[i] = k_operand(i);
 
-            const bool masked = !all_see(w_first, w_last);
+            if constexpr (Q8) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 k4 = *(const f32x4*)&scales[it & 3][0][32 * n + 8 * i + 4 * kg];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[n][4 * i + r] *= k4[r];
+                    }
+            }
             uint32_t hidden = 0;  // bit 16 n + e
-            if (masked) {
+            if (!all_see(w_first, w_last)) {
                 const int kg4 = here(4 * kg);
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
@@ -395,89 +465,66 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                         const int32_t v = it * kKeys + key, j = v < sinks ? v : v + gap;
                         const bool sees = (ok >> key & 1) && j <= p && (!a.window || p - j < a.window || j < a.sinks);
                         hidden |= (uint32_t)!sees << (16 * n + e);
+                        x[n][e] = sees ? x[n][e] : -__builtin_inff();
                     }
             }
             any |= hidden != ~0u;
-            f32x16 x[2];
-            float sum;
-            for (;;) {
-                // scores: lane (row, kg) holds keys 32 n + 8 (e / 4) + 4 kg + e % 4
+            // does a score lie far above the maximum that the weights are taken against? (a NaN does not matter)
+            float top = x[0][0];
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+            for (int e = 1; e < 16; ++e) top = __builtin_elementwise_maximum(top, x[0][e]);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[n][e] = 0.0f;
+            for (int e = 0; e < 16; ++e) top = __builtin_elementwise_maximum(top, x[1][e]);
+            if (__builtin_amdgcn_ballot_w64(top * factor > m + kSlack)) {
+                const float m2 = fmaxf(m, pair_max(top * factor));
+                const float keep = __builtin_amdgcn_exp2f(m - m2);
+                m = m2;
+                l *= keep;
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) x[n] = mma32<DT>(*(const u32x4*)(kb + (k_at ^ s << 5) + 32 * n * LS), q[s], x[n]);
-                // six reads ahead of the products, then one with each
-                __builtin_amdgcn_sched_group_barrier(kDsRead, 6, 0);
-#pragma unroll
-                for (int s = 0; s < 2 * KS - 6; ++s) {
-                    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
-                }
-                __builtin_amdgcn_sched_group_barrier(kMfma, 6, 0);
-                if constexpr (Q8) {
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const f32x4 k4 = *(const f32x4*)&scales[it & 1][0][32 * n + 8 * i + 4 * kg];
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) x[n][4 * i + r] *= k4[r];
-                        }
-                }
-                if (fresh) {
-                    const uint32_t shut = here(hidden);
-                    float top = -__builtin_inff();
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) top = fmaxf(top, shut >> (16 * n + e) & 1 ? -__builtin_inff() : x[n][e]);
-                    const float m2 = fmaxf(m, pair_max(top) * factor);
-                    const float keep = __builtin_amdgcn_exp2f(m - m2);
-                    m = m2;
-                    l *= keep;
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) acc[i] *= keep;
-                }
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][e], factor, -m));
-                if (masked) {
-                    const uint32_t shut = here(hidden);
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) x[n][e] = shut >> (16 * n + e) & 1 ? 0.0f : x[n][e];
-                }
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) part[e & 3] += x[n][e];
-                sum = (part[0] + part[1]) + (part[2] + part[3]);
-                if (fresh || !__builtin_amdgcn_ballot_w64(!(sum <= kMostSum))) break;
-                fresh = true;
+                for (int i = 0; i < NB; ++i) acc[i] *= keep;
             }
-            fresh = false;
-            l += sum;
+            // the next tile's scores, with this one's weights between the products
+            {
+                constexpr int N = 2 * KS;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) y[n][e] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    y[i & 1] = mma32<DT>(k_ring[i % AHEAD1], q[i >> 1], y[i & 1]);
+                    if (i + AHEAD1 < N) k_ring[i % AHEAD1] = k_operand(i + AHEAD1);
+                    if constexpr (!Q8) {
+#pragma unroll
+                        for (int k = i * SENDS / N; k < (i + 1) * SENDS / N; ++k)
+                            send(k < DMAS ? it + 2 : it + 1, k / DMAS, k % DMAS, from[k]);
+                    }
+#pragma unroll
+                    for (int k = i * 32 / N; k < (i + 1) * 32 / N; ++k) {
+                        float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 4][k & 15], factor, -m));
+                        asm volatile("" : "+v"(w));  // made here, not where it is used
+                        x[k >> 4][k & 15] = w;
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if constexpr (Q8) {
-                float most = 0.0f;
+                float part = 0.0f, most = 0.0f;
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const f32x4 v4 = *(const f32x4*)&scales[it & 1][1][32 * n + 8 * i + 4 * kg];
+                        const f32x4 v4 = *(const f32x4*)&scales[it & 3][1][32 * n + 8 * i + 4 * kg];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const float v = hidden >> (16 * n + 4 * i + r) & 1 ? 0.0f : v4[r];
                             most = fmaxf(most, fabsf(v));
+                            part += x[n][4 * i + r];
                             x[n][4 * i + r] *= v;
                         }
                     }
+                l += part;
                 if (__builtin_amdgcn_ballot_w64(most > v_top)) {
                     most = fmaxf(v_top, pair_max(most));
                     const float inv = 1.0f / most, keep = v_top * inv;
@@ -490,8 +537,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[n][e] *= v_inv;
-            }
-            if constexpr (!Q8) {
+            } else {
                 for (uint64_t left = edge ? uniform64(bad[it % 3]) : 0; left; left &= left - 1) {
                     const int key = __builtin_ctzll(left), kg4 = here(4 * kg);
                     // this row's weight of the key, from whichever of the two lanes holds it, and whether it is seen
@@ -507,7 +553,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                             }
                     w = pair_sum(w);
                     sees = pair_max(sees ? 1.0f : 0.0f) != 0.0f;
-                    const Global row = (Global)(uintptr_t)info[it % 3][key][1];
+                    const Global row = (Global)(uintptr_t)info[it & 3][key][1];
 #pragma unroll
                     for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -518,27 +564,48 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                         }
                 }
             }
-            // acc += V^T P^T
+            // acc += V^T P^T, with the weights' sum and their rounding to 16 bits between the products
+            {
+                constexpr int N = 4 * NB, AHEAD = 4;
+                const uint32_t at = lds0 + (2 * (it & 1) + 1) * TILE + here(v_at);
+                auto operand = [&](int i) {
+                    const uint32_t from = at ^ (i % NB) << 6;
+                    const u32x2 lo = lds_tr16(from, 16 * (i / NB) * LS), hi = lds_tr16(from, (16 * (i / NB) + 8) * LS);
+                    return (u32x4){lo[0], lo[1], hi[0], hi[1]};
+                };
+                auto weights = [&](int s, int i) {
+                    return pack2<PV>(x[s >> 1][8 * (s & 1) + 2 * i], x[s >> 1][8 * (s & 1) + 2 * i + 1]);
+                };
+                u32x4 ring[AHEAD], pw[2];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int n = s >> 1, e0 = 8 * (s & 1);
-                u32x4 pw;
+                for (int i = 0; i < AHEAD; ++i) ring[i] = operand(i);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) pw[i] = pack2<PV>(x[n][e0 + 2 * i], x[n][e0 + 2 * i + 1]);
+                for (int i = 0; i < 4; ++i) pw[0][i] = weights(0, i);
+                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    const char* const from = vb + (v_at ^ i << 6) + 16 * s * LS;
-                    const u32x2 lo = lds_tr16(from), hi = lds_tr16(from + 8 * LS);
-                    acc[i] = mma32<PV>((u32x4){lo[0], lo[1], hi[0], hi[1]}, pw, acc[i]);
+                for (int i = 0; i < N; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int s = i / NB;
+                    acc[i % NB] = mma32<PV>(ring[i % AHEAD], pw[s & 1], acc[i % NB]);
+                    if (i + AHEAD < N) ring[i % AHEAD] = operand(i + AHEAD);
+                    if (s < 3) {
+#pragma unroll
+                        for (int k = i % NB * 4 / NB; k < (i % NB + 1) * 4 / NB; ++k) pw[s + 1 & 1][k] = weights(s + 1, k);
+                    }
+                    if constexpr (!Q8) {
+#pragma unroll
+                        for (int k = i * 32 / N; k < (i + 1) * 32 / N; ++k) part[k & 3] += x[k >> 4][k & 15];
+                    }
                 }
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (!Q8) l += (part[0] + part[1]) + (part[2] + part[3]);
             }
-            __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 1);
-#pragma unroll
-            for (int s = 0; s < 4 * NB - 4; ++s) {
-                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
-                __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
-            }
-            __builtin_amdgcn_sched_group_barrier(kMfma, 4, 1);
+        };
+        f32x16 xa[2], xb[2];
+        if (!no_rows) scores(tile0, xa);
+        for (int it = tile0; it < tiles; it += 2) {
+            step(it, xa, xb);
+            if (it + 1 < tiles) step(it + 1, xb, xa);
         }
     }
 
