@@ -9,8 +9,8 @@
 // maximum and sum need one exchange between lane pairs, and the weights as they lie are the right operand of V^T times P^T.
 // K and V go straight from memory into two LDS buffers (an int8 cache through registers, where it becomes 16-bit), the 16-byte
 // pieces of a row exchanged so that neither the reads of K nor the transposing reads of V meet in a bank.  One barrier per
-// 64 keys: the next rows are on their way while these are worked on.  Where a row of the cache lies is found three tiles
-// ahead, a lane per row, by the waves in turn.
+// 64 keys: the next rows are on their way while these are worked on.  Where the rows of the cache lie is found for four
+// tiles at a time, ahead of them.
 //
 // The next tile's scores are made between the exponentials of this one, so that a wave keeps both pipes busy.  The running
 // maximum moves only where a score lies far above it: most tiles rescale nothing and need no exchange between lanes.
@@ -21,6 +21,9 @@
 
 namespace qk {
 namespace {
+
+// The parts of the kernel are lambdas, some of them used in several places: none may become a function.
+#define INLINE __attribute__((always_inline))
 
 constexpr int kThreads = 256;
 constexpr int kRows = 128;   // query rows per workgroup
@@ -113,6 +116,15 @@ __device__ __forceinline__ float pair_sum(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+__device__ __forceinline__ float largest(const f32x16 (&x)[2]) {
+    float top = x[0][0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = __builtin_elementwise_maximum(top, x[0][e]);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = __builtin_elementwise_maximum(top, x[1][e]);
+    return top;
+}
+
 // DP: head_dim padded to 32s; WHOLE: head_dim == DP; Q8: int8 cache
 template <int DP, int DT, bool Q8, bool WHOLE>
 __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(PromptArgs g) {
@@ -128,10 +140,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     static_assert(!Q8 || kKeys * CH % kThreads == 0, "");
     constexpr int TILE = kKeys * LS;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];  // buffer 0: K, V; buffer 1: K, V
-    __shared__ __attribute__((aligned(16))) uint64_t info[4][kKeys][2];  // addresses of a key's and a value's row (none: of zeros)
-    __shared__ uint64_t info_ok[4];              // which keys of the tile exist
+    __shared__ __attribute__((aligned(16))) uint64_t info[8][kKeys][2];  // addresses of a key's and a value's row (none: of zeros)
+    __shared__ uint64_t info_ok[8];              // which keys of the tile exist
     __shared__ uint64_t bad[3];                  // which rows of V hold a NaN or an infinity
-    __shared__ float scales[4][2][kKeys];
+    __shared__ float scales[8][2][kKeys];
     __shared__ int64_t found[2];
 
     const AttnArgs& a = g.a;
@@ -194,14 +206,13 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     const int32_t past = keys - seq.tokens;  // position of the first token (negative: it stands before the first key)
     const int32_t p_first = past + div31(row0, g.group_div), p_last = past + div31(row0 + rows - 1, g.group_div);
 
-    // this lane's row (past the last: as the last) and its wave's span
+    // this lane's row (past the last: as the last)
     const int32_t mine = row0 + (wave * 32 + col < rows ? wave * 32 + col : rows - 1);
     const int32_t token = div31(mine, g.group_div);
     const int64_t t = seq.first + token;
     const int h = kvh * G + (mine - token * G);
     const int32_t p = past + token;
-    const int32_t w_first = __builtin_amdgcn_readfirstlane(p), w_last = __builtin_amdgcn_readlane(p, 31);
-
+    
     // the keys that any row sees, without a gap: key j is place j or, past the sinks, j - gap
     int32_t low = 0, sinks = 0;
     if (a.window && p_first - a.window + 1 > 0) {
@@ -242,18 +253,18 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     const Global zeros = global_address(kZeroRow);
     // What finds the rows' places reads its arguments from memory again each time: they would hold scalar registers that the
     // loop has better use for.
-    auto args = []() {
+    auto args = []() INLINE {
         const __attribute__((address_space(4))) PromptArgs* from =
             (const __attribute__((address_space(4))) PromptArgs*)__builtin_amdgcn_kernarg_segment_ptr();
         asm volatile("" : "+s"(from));
         return from;
     };
-    // a lane per row of a tile: its page, then its place in memory and its scales
-    auto place = [&](int tile) {
-        const int32_t v = tile * kKeys + lane;
+    // Each wave finds its 16 rows of four tiles at a time, a lane per row: the page, then the place in memory and the scales.
+    auto place = [&](int tile) INLINE {
+        const int32_t v = (tile + kg * 2 + (col >> 4)) * kKeys + wave * 16 + (lane & 15);
         return v < places ? (v < sinks ? v : v + gap) : -1;
     };
-    auto page_of = [&](int tile) {
+    auto page_of = [&](int tile) INLINE {
         const int32_t j = place(tile);
         if (!paged || j < 0) return (int32_t)-1;
         const auto* g = args();
@@ -261,7 +272,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         return load_global<int32_t>(table + (int64_t)div31(j, (Div31){g->a.kv.page_div.m, g->a.kv.page_div.s}) * 4);
     };
     float ks_next = 0.0f, vs_next = 0.0f;
-    auto put_info = [&](int tile, int32_t page) {
+    auto put_info = [&](int tile, int32_t page) INLINE {
         const auto* g = args();
         const auto& c = g->a.kv.c;
         const int32_t j = place(tile);
@@ -278,10 +289,11 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             kp = global_address(c.key) + (page * c.key_page_stride + slot * c.key_token_stride + kvh * c.key_head_stride) * ES;
             vp = global_address(c.value) + (page * c.value_page_stride + slot * c.value_token_stride + kvh * c.value_head_stride) * ES;
         }
-        info[tile & 3][lane][0] = (uint64_t)(uintptr_t)kp;
-        info[tile & 3][lane][1] = (uint64_t)(uintptr_t)vp;
+        uint64_t* const to = info[tile + (lane >> 4) & 7][wave * 16 + (lane & 15)];
+        to[0] = (uint64_t)(uintptr_t)kp;
+        to[1] = (uint64_t)(uintptr_t)vp;
         const uint64_t ok = __builtin_amdgcn_ballot_w64(valid);
-        if (lane == 0) info_ok[tile & 3] = ok;
+        if ((lane & 15) == 0) ((uint16_t*)info_ok)[(tile + (lane >> 4) & 7) * 4 + wave] = (uint16_t)(ok >> lane);
         if constexpr (Q8) {
             Global kz = zeros, vz = zeros;
             if (valid) {
@@ -294,16 +306,16 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             vs_next = load_global<float>(vz);
         }
     };
-    auto put_scales = [&](int tile) {
+    auto put_scales = [&](int tile) INLINE {
         if constexpr (Q8) {
-            scales[tile & 3][0][lane] = ks_next;
-            scales[tile & 3][1][lane] = vs_next;
+            scales[tile + (lane >> 4) & 7][0][wave * 16 + (lane & 15)] = ks_next;
+            scales[tile + (lane >> 4) & 7][1][wave * 16 + (lane & 15)] = vs_next;
         }
     };
 
     // the place of piece ch of row r in LDS
-    auto k_turn = [](int r) { return CHL == 8 ? r >> 1 & 7 : r & 15; };
-    auto v_turn = [](int r) { return CHL == 8 ? (r >> 1 & 3) << 1 : (r & 7) << 1; };
+    auto k_turn = [](int r) INLINE { return CHL == 8 ? r >> 1 & 7 : r & 15; };
+    auto v_turn = [](int r) INLINE { return CHL == 8 ? (r >> 1 & 3) << 1 : (r & 7) << 1; };
     u32x4 kr[PIECES], vr[PIECES];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     const int k_piece = (lane % CHL ^ k_turn(lane / CHL)) << 4, v_piece = (lane % CHL ^ v_turn(lane / CHL)) << 4;
@@ -311,24 +323,24 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     // Addresses of this lane's pieces of K (which 0) or V (1) of a tile, and piece i on its way to LDS buffer tile & 1.
     // Load i of the wave fills rows i * R + lane / CHL of its 16; the turn of a sum of rows is the turns' exclusive or.
     constexpr int R = 64 / CHL;
-    auto address = [&](int tile, int which, int i) {
+    auto address = [&](int tile, int which, int i) INLINE {
         const int ch = (which ? v_piece : k_piece) ^ (which ? v_turn(i * R) : k_turn(i * R)) << 4;
-        Global from = (Global)(uintptr_t)(&info[tile & 3][0][which] + lane_rows)[i * R * 2] + ch;
+        Global from = (Global)(uintptr_t)(&info[tile & 7][0][which] + lane_rows)[i * R * 2] + ch;
         if (!WHOLE || DP * 2 < LS) {
             if (ch >= D * 2) from = zeros;
         }
         return from;
     };
-    auto send = [&](int tile, int which, int i, Global from) {
+    auto send = [&](int tile, int which, int i, Global from) INLINE {
         global_to_lds(from, lds0 + (2 * (tile & 1) + which) * TILE + (wave * DMAS + i) * 1024);
     };
     // the whole of it; int8: into registers
-    auto load_tile = [&](int tile, int which) {
+    auto load_tile = [&](int tile, int which) INLINE {
         if constexpr (Q8) {
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
                 const int at = tid + i * kThreads, r = at / CH, ch = at % CH;
-                Global from = (Global)(uintptr_t)info[tile & 3][r][which] + ch * 16;
+                Global from = (Global)(uintptr_t)info[tile & 7][r][which] + ch * 16;
                 if (!WHOLE && ch * 16 >= D) from = zeros;
                 (which ? vr : kr)[i] = load_global<u32x4>(from);
             }
@@ -338,7 +350,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         }
     };
     // int8: K or V of a tile from the registers, as 16-bit values
-    auto store_tile = [&](int tile, int which) {
+    auto store_tile = [&](int tile, int which) INLINE {
         if constexpr (Q8) {
             char* const buffer = lds + (2 * (tile & 1) + which) * TILE;
 #pragma unroll
@@ -353,13 +365,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
 
     const bool no_rows = wave * 32 >= rows;  // for this wave
     if (tile0 < tiles) {
-        const int turn = wave - tile0 & 3;  // tiles tile0 + turn, + 4, ... are this wave's to find
-        int32_t page = page_of(tile0 + turn);
-        if (turn < 3) {
-            put_info(tile0 + turn, page);
-            page = page_of(tile0 + turn + 4);
-            if (turn < 2) put_scales(tile0 + turn);
-        }
+        int32_t page = page_of(tile0);
+        put_info(tile0, page);
+        page = page_of(tile0 + 4);
+        put_scales(tile0);
         __syncthreads();
         load_tile(tile0, 0);
         if constexpr (Q8) {
@@ -367,7 +376,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             load_tile(tile0 + 1, 0);
             load_tile(tile0, 1);
         } else {
-            if (tile0 + 1 < tiles) load_tile(tile0 + 1, 0);
+            load_tile(tile0 + 1, 0);
             load_tile(tile0, 1);
             __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         }
@@ -377,7 +386,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         const int v_row = 4 * kg + (lane >> 2 & 3);
         const int v_at = v_row * LS + (((lane >> 4 & 1) << 1 | (lane >> 1 & 1)) ^ v_turn(v_row)) * 16 + 8 * (lane & 1);
         // scores of a tile: lane (row, kg) holds keys 32 n + 8 (e / 4) + 4 kg + e % 4
-        auto scores = [&](int tile, f32x16 (&x)[2]) {
+        auto scores = [&](int tile, f32x16 (&x)[2]) INLINE {
             const char* const kb = lds + 2 * (tile & 1) * TILE;
 #pragma unroll
             for (int n = 0; n < 2; ++n)
@@ -389,93 +398,18 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 for (int n = 0; n < 2; ++n) x[n] = mma32<DT>(*(const u32x4*)(kb + (k_at ^ s << 5) + 32 * n * LS), q[s], x[n]);
         };
 
-        // One step: the tile's weights from its scores x, while the next tile's scores are made (into y), then its values.
-        // K of the next tile and V of this one are in LDS at its barrier.
-        auto step = [&](int it, f32x16 (&x)[2], f32x16 (&y)[2]) {
-            char* const vb = lds + (2 * (it & 1) + 1) * TILE;
-            const uint64_t ok = uniform64(info_ok[it & 3]);
-            // masked for some row of the workgroup?
-            const int32_t j0 = it * kKeys + (it * kKeys < sinks ? 0 : gap), last = it * kKeys + kKeys - 1;
-            const int32_t j1 = last + (last < sinks ? 0 : gap);
-            auto all_see = [&](int32_t first_p, int32_t last_p) {
-                return ~ok == 0 && j1 <= first_p && (!a.window || j1 < a.sinks || last_p - j0 < a.window);
-            };
-            const bool edge = !all_see(p_first, p_last);
-            if constexpr (Q8) {
-                store_tile(it + 1, 0);
-                store_tile(it, 1);
-            } else {
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // this wave's part is in LDS
-                if (edge) {
-#pragma unroll
-                    for (int i = 0; i < DMAS; ++i) {
-                        const int slot = (wave * DMAS + i) * 64 + lane, r = slot / CHL;
-                        const u32x4 v = *(const u32x4*)(vb + slot * 16);
-                        if (not_finite<DT>(v)) {
-                            *(u32x4*)(vb + slot * 16) = finite_only<DT>(v);
-                            atomicOr((unsigned long long*)&bad[it % 3], 1ull << r);
-                        }
-                    }
-                }
-            }
-            __syncthreads();
-            if (Q8 && wave == (it + 2 & 3)) put_scales(it + 2);
-            if (wave == (it + 3 & 3)) {
-                put_info(it + 3, page);
-                page = page_of(it + 7);
-                if (lane == 0) bad[(it + 2) % 3] = 0;
-            }
-            // What is sent for: K two tiles on, V one (past the last: a row of zeros, or one that is not used).  The 16-bit loads go out
-            // between the products, their addresses being read here.
-            constexpr int SENDS = Q8 ? 1 : 2 * DMAS;
-            Global from[SENDS];
-            if (Q8 || no_rows) {
-                load_tile(it + 2, 0);
-                load_tile(it + 1, 1);
-                if (no_rows) return;
-            } else {
-#pragma unroll
-                for (int i = 0; i < SENDS; ++i) from[i] = address(i < DMAS ? it + 2 : it + 1, i / DMAS, i % DMAS);
-            }
-            constexpr int AHEAD1 = 6;
-            const uint32_t k_from = lds0 + 2 * (it + 1 & 1) * TILE + here(k_at);
-            auto k_operand = [&](int i) { return lds_load(k_from ^ (i >> 1) << 5, 32 * (i & 1) * LS); };
-            u32x4 k_ring[AHEAD1];
-#pragma unroll
-            for (int i = 0; i < AHEAD1; ++i) k_ring[i] = k_operand(i);
-
-            if constexpr (Q8) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 k4 = *(const f32x4*)&scales[it & 3][0][32 * n + 8 * i + 4 * kg];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) x[n][4 * i + r] *= k4[r];
-                    }
-            }
-            uint32_t hidden = 0;  // bit 16 n + e
-            if (!all_see(w_first, w_last)) {
-                const int kg4 = here(4 * kg);
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int key = 32 * n + 8 * (e >> 2) + kg4 + (e & 3);
-                        const int32_t v = it * kKeys + key, j = v < sinks ? v : v + gap;
-                        const bool sees = (ok >> key & 1) && j <= p && (!a.window || p - j < a.window || j < a.sinks);
-                        hidden |= (uint32_t)!sees << (16 * n + e);
-                        x[n][e] = sees ? x[n][e] : -__builtin_inff();
-                    }
-            }
-            any |= hidden != ~0u;
-            // does a score lie far above the maximum that the weights are taken against? (a NaN does not matter)
-            float top = x[0][0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) top = __builtin_elementwise_maximum(top, x[0][e]);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = __builtin_elementwise_maximum(top, x[1][e]);
-            if (__builtin_amdgcn_ballot_w64(top * factor > m + kSlack)) {
+        bool edge = false;  // some row of the workgroup does not see some key of the tile at hand
+        int32_t j0 = 0;     // the tile's first key
+        uint64_t ok = 0;    // which of its keys exist
+        auto look = [&](int tile) INLINE {
+            ok = uniform64(info_ok[tile & 7]);
+            const int32_t last = tile * kKeys + kKeys - 1, j1 = last + (last < sinks ? 0 : gap);
+            j0 = tile * kKeys + (tile * kKeys < sinks ? 0 : gap);
+            edge = ~ok != 0 || j1 > p_first || (a.window && j1 >= a.sinks && p_last - j0 >= a.window);
+        };
+        // Moves the maximum where a score lies far above it; `top` is a lane's largest score (a NaN does not matter).
+        auto raise = [&](float top) INLINE {
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(top * factor > m + kSlack) != 0, 0)) {
                 const float m2 = fmaxf(m, pair_max(top * factor));
                 const float keep = __builtin_amdgcn_exp2f(m - m2);
                 m = m2;
@@ -483,13 +417,159 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
 #pragma unroll
                 for (int i = 0; i < NB; ++i) acc[i] *= keep;
             }
+        };
+        auto apply_key_scales = [&](int tile, f32x16 (&x)[2]) INLINE {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 k4 = *(const f32x4*)&scales[tile & 7][0][32 * n + 8 * i + 4 * kg];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[n][4 * i + r] *= k4[r];
+                }
+        };
+        // The weights take the values' scales; `seen` has a bit for each key, from this lane's first on.
+        auto apply_value_scales = [&](int tile, f32x16 (&x)[2], uint64_t seen) INLINE {
+            float part = 0.0f, most = 0.0f;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 v4 = *(const f32x4*)&scales[tile & 7][1][32 * n + 8 * i + 4 * kg];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float v = seen >> (32 * n + 8 * i + r) & 1 ? v4[r] : 0.0f;
+                        most = fmaxf(most, fabsf(v));
+                        part += x[n][4 * i + r];
+                        x[n][4 * i + r] *= v;
+                    }
+                }
+            l += part;
+            if (__builtin_amdgcn_ballot_w64(most > v_top)) {
+                most = fmaxf(v_top, pair_max(most));
+                const float inv = 1.0f / most, keep = v_top * inv;
+                v_top = most;
+                v_inv = inv;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) acc[i] *= keep;
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[n][e] *= v_inv;
+        };
+        // What every step begins with: K of the next tile and V of this one are in LDS behind its barrier.
+        auto begin = [&](int it) INLINE {
+            if constexpr (Q8) {
+                store_tile(it + 1, 0);
+                store_tile(it, 1);
+            } else {
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // this wave's part is in LDS
+            }
+        };
+        auto behind_barrier = [&](int it) INLINE {
+            if (Q8 && (it - tile0 & 3) == 2) put_scales(it + 2);
+            if ((it - tile0 & 3) == 0) {
+                put_info(it + 4, page);
+                page = page_of(it + 8);
+            }
+        };
+
+        uint64_t mine = ~0ull;  // the tile's keys that this lane's row sees, from the lane's first on: bit 32 n + 8 (e / 4) + e % 4
+        // Looks at the tile whose scores x are there, `top` a lane's largest: hides what is not seen, moves the maximum.
+        auto prepare = [&](int tile, f32x16 (&x)[2], float top) INLINE {
+            look(tile);
+            if (no_rows) return;
+            if constexpr (Q8) {
+                apply_key_scales(tile, x);
+                top = largest(x);
+            }
+            mine = ~0ull;
+            if (__builtin_expect(edge, 0)) {
+                // the tile's places that this row sees: up to its own, but for those between the sinks and its window
+                auto below = [](int32_t n) INLINE { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
+                auto place_of = [&](int32_t j) INLINE { return (j < sinks ? j : j < sinks + gap ? sinks : j - gap) - tile * kKeys; };
+                uint64_t seen = ok & below(place_of(p + 1));
+                if (a.window && p >= a.window) seen &= ~below(place_of(p - a.window + 1)) | below(place_of(a.sinks));
+                any |= seen != 0;
+                mine = seen >> here(4 * kg);
+                const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[n][e] = (n ? hi : lo) & 1u << (8 * (e >> 2) + (e & 3)) ? x[n][e] : -__builtin_inff();
+                top = largest(x);
+            } else {
+                any = true;
+            }
+            raise(top);
+        };
+
+        // One step: the tile's weights from its scores x, while the next tile's scores are made (into y), then its values.
+        auto step = [&](int it, f32x16 (&x)[2], f32x16 (&y)[2]) INLINE {
+            begin(it);
+            if (!Q8 && __builtin_expect(edge, 0)) {
+                char* const vb = lds + (2 * (it & 1) + 1) * TILE;
+#pragma nounroll
+                for (int i = 0; i < DMAS; ++i) {
+                    const int slot = (wave * DMAS + i) * 64 + lane, r = slot / CHL;
+                    const u32x4 v = *(const u32x4*)(vb + slot * 16);
+                    if (not_finite<DT>(v)) {
+                        *(u32x4*)(vb + slot * 16) = finite_only<DT>(v);
+                        atomicOr((unsigned long long*)&bad[it % 3], 1ull << r);
+                    }
+                }
+            }
+            __syncthreads();
+            if (!Q8 && tid == 0) bad[(it + 2) % 3] = 0;
+            if (__builtin_expect(no_rows, 0)) {
+                behind_barrier(it);
+                load_tile(it + 2, 0);
+                load_tile(it + 1, 1);
+                look(it + 1);
+                return;
+            }
+            const uint32_t k_from = lds0 + 2 * (it + 1 & 1) * TILE + here(k_at);
+            auto k_operand = [&](int i) INLINE { return lds_load(k_from ^ (i >> 1) << 5, 32 * (i & 1) * LS); };
+            constexpr int AHEAD1 = 6;
+            u32x4 k_ring[AHEAD1];
+#pragma unroll
+            for (int i = 0; i < AHEAD1; ++i) k_ring[i] = k_operand(i);
+            behind_barrier(it);
+            // What is sent for: K two tiles on, V one (past the last: rows of zeros, or ones that are not used).  The 16-bit
+            // loads go out between the products, their addresses being read here.
+            constexpr int SENDS = Q8 ? 1 : 2 * DMAS;
+            Global from[SENDS];
+            if constexpr (Q8) {
+                load_tile(it + 2, 0);
+                load_tile(it + 1, 1);
+            } else {
+#pragma unroll
+                for (int i = 0; i < SENDS; ++i) from[i] = address(i < DMAS ? it + 2 : it + 1, i / DMAS, i % DMAS);
+            }
+            const uint32_t v_from = lds0 + (2 * (it & 1) + 1) * TILE + here(v_at);
+            auto v_operand = [&](int i) INLINE {
+                const uint32_t from = v_from ^ (i % NB) << 6;
+                const u32x2 lo = lds_tr16(from, 16 * (i / NB) * LS), hi = lds_tr16(from, (16 * (i / NB) + 8) * LS);
+                return (u32x4){lo[0], lo[1], hi[0], hi[1]};
+            };
+            constexpr int AHEAD2 = 4;
+            u32x4 v_ring[AHEAD2];
             // the next tile's scores, with this one's weights between the products
             {
-                constexpr int N = 2 * KS;
+                constexpr int N = 2 * KS, FIRST = 6;
+                auto weight = [&](int k) INLINE {
+                    float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 4][k & 15], factor, -m));
+                    asm volatile("" : "+v"(w));  // made here, not where it is used
+                    x[k >> 4][k & 15] = w;
+                };
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) y[n][e] = 0.0f;
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < FIRST; ++k) weight(k);  // while the first operands come
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     __builtin_amdgcn_sched_barrier(0);
@@ -500,85 +580,49 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                         for (int k = i * SENDS / N; k < (i + 1) * SENDS / N; ++k)
                             send(k < DMAS ? it + 2 : it + 1, k / DMAS, k % DMAS, from[k]);
                     }
+                    if (i >= N - AHEAD2) v_ring[i - N + AHEAD2] = v_operand(i - N + AHEAD2);
 #pragma unroll
-                    for (int k = i * 32 / N; k < (i + 1) * 32 / N; ++k) {
-                        float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 4][k & 15], factor, -m));
-                        asm volatile("" : "+v"(w));  // made here, not where it is used
-                        x[k >> 4][k & 15] = w;
-                    }
+                    for (int k = FIRST + i * (32 - FIRST) / N; k < FIRST + (i + 1) * (32 - FIRST) / N; ++k) weight(k);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (Q8) {
-                float part = 0.0f, most = 0.0f;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 v4 = *(const f32x4*)&scales[it & 3][1][32 * n + 8 * i + 4 * kg];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float v = hidden >> (16 * n + 4 * i + r) & 1 ? 0.0f : v4[r];
-                            most = fmaxf(most, fabsf(v));
-                            part += x[n][4 * i + r];
-                            x[n][4 * i + r] *= v;
-                        }
-                    }
-                l += part;
-                if (__builtin_amdgcn_ballot_w64(most > v_top)) {
-                    most = fmaxf(v_top, pair_max(most));
-                    const float inv = 1.0f / most, keep = v_top * inv;
-                    v_top = most;
-                    v_inv = inv;
-#pragma unroll
-                    for (int i = 0; i < NB; ++i) acc[i] *= keep;
-                }
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[n][e] *= v_inv;
-            } else {
-                for (uint64_t left = edge ? uniform64(bad[it % 3]) : 0; left; left &= left - 1) {
-                    const int key = __builtin_ctzll(left), kg4 = here(4 * kg);
+                apply_value_scales(it, x, mine);
+            } else if (__builtin_expect(edge, 0)) {
+#pragma nounroll
+                for (uint64_t left = uniform64(bad[it % 3]); left; left &= left - 1) {
+                    const int key = __builtin_ctzll(left), own = key - here(4 * kg);
                     // this row's weight of the key, from whichever of the two lanes holds it, and whether it is seen
                     float w = 0.0f;
-                    bool sees = false;
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if (key == 32 * n + 8 * (e >> 2) + kg4 + (e & 3)) {
-                                w = x[n][e];
-                                sees = !(hidden >> (16 * n + e) & 1);
-                            }
+                        for (int e = 0; e < 16; ++e) w = own == 32 * n + 8 * (e >> 2) + (e & 3) ? x[n][e] : w;
                     w = pair_sum(w);
-                    sees = pair_max(sees ? 1.0f : 0.0f) != 0.0f;
-                    const Global row = (Global)(uintptr_t)info[it & 3][key][1];
+                    const bool sees = pair_max(own >= 0 && !(own & 4) && (mine >> (own & 63) & 1) ? 1.0f : 0.0f) != 0.0f;
+                    const Global row = (Global)(uintptr_t)info[it & 7][key][1];
 #pragma unroll
                     for (int i = 0; i < NB; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int d = 32 * i + 8 * (e >> 2) + kg4 + (e & 3);
-                            const uint32_t bits = WHOLE || d < D ? load_global<uint16_t>(row + d * 2) : 0;
-                            if (sees && (bits & exponent_of<DT>()) == exponent_of<DT>()) acc[i][e] += w * load_half_bits(bits, DT);
+                        for (int e = 0; e < 16; e += 4) {
+                            const int d = 32 * i + 2 * e + 4 * kg;
+                            const u32x2 bits = WHOLE || d < D ? load_global<u32x2>(row + d * 2) : (u32x2){0, 0};
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const uint32_t h = bits[r >> 1] >> (16 * (r & 1)) & 0xffffu;
+                                if (sees && (h & exponent_of<DT>()) == exponent_of<DT>()) acc[i][e + r] += w * load_half_bits(h, DT);
+                            }
                         }
                 }
             }
-            // acc += V^T P^T, with the weights' sum and their rounding to 16 bits between the products
+            // acc += V^T P^T; between the products the weights' sum, their rounding to 16 bits, and the largest of the next scores
+            float top = y[0][0];
             {
-                constexpr int N = 4 * NB, AHEAD = 4;
-                const uint32_t at = lds0 + (2 * (it & 1) + 1) * TILE + here(v_at);
-                auto operand = [&](int i) {
-                    const uint32_t from = at ^ (i % NB) << 6;
-                    const u32x2 lo = lds_tr16(from, 16 * (i / NB) * LS), hi = lds_tr16(from, (16 * (i / NB) + 8) * LS);
-                    return (u32x4){lo[0], lo[1], hi[0], hi[1]};
-                };
-                auto weights = [&](int s, int i) {
+                constexpr int N = 4 * NB;
+                auto weights = [&](int s, int i) INLINE {
                     return pack2<PV>(x[s >> 1][8 * (s & 1) + 2 * i], x[s >> 1][8 * (s & 1) + 2 * i + 1]);
                 };
-                u32x4 ring[AHEAD], pw[2];
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) ring[i] = operand(i);
+                u32x4 pw[2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) pw[0][i] = weights(0, i);
                 float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -586,23 +630,30 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 for (int i = 0; i < N; ++i) {
                     __builtin_amdgcn_sched_barrier(0);
                     const int s = i / NB;
-                    acc[i % NB] = mma32<PV>(ring[i % AHEAD], pw[s & 1], acc[i % NB]);
-                    if (i + AHEAD < N) ring[i % AHEAD] = operand(i + AHEAD);
+                    acc[i % NB] = mma32<PV>(v_ring[i % AHEAD2], pw[s & 1], acc[i % NB]);
+                    if (i + AHEAD2 < N) v_ring[i % AHEAD2] = v_operand(i + AHEAD2);
                     if (s < 3) {
 #pragma unroll
                         for (int k = i % NB * 4 / NB; k < (i % NB + 1) * 4 / NB; ++k) pw[s + 1 & 1][k] = weights(s + 1, k);
                     }
                     if constexpr (!Q8) {
 #pragma unroll
-                        for (int k = i * 32 / N; k < (i + 1) * 32 / N; ++k) part[k & 3] += x[k >> 4][k & 15];
+                        for (int k = i * 32 / N; k < (i + 1) * 32 / N; ++k) {
+                            part[k & 3] += x[k >> 4][k & 15];
+                            top = __builtin_elementwise_maximum(top, y[k >> 4][k & 15]);
+                        }
+                        asm volatile("" : "+v"(top), "+v"(part[0]), "+v"(part[1]), "+v"(part[2]), "+v"(part[3]));
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (!Q8) l += (part[0] + part[1]) + (part[2] + part[3]);
             }
+            prepare(it + 1, y, top);
         };
+
         f32x16 xa[2], xb[2];
         if (!no_rows) scores(tile0, xa);
+        prepare(tile0, xa, largest(xa));
         for (int it = tile0; it < tiles; it += 2) {
             step(it, xa, xb);
             if (it + 1 < tiles) step(it + 1, xb, xa);
@@ -610,7 +661,6 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     }
 
     l = pair_sum(l);
-    any = pair_max(any ? 1.0f : 0.0f) != 0.0f;
     if (Q8) {
 #pragma unroll
         for (int i = 0; i < NB; ++i) acc[i] *= v_top;
@@ -619,7 +669,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         const int64_t place = (blockIdx.x / (uint32_t)(c.kv_heads * g.splits)) * c.kv_heads + kvh;
         // in the order of the registers: whole lines, and the joining lane finds its own rows
         constexpr uint32_t SUMS = 4 * NB * 4 * 1024;
-        auto part = [&](int s) { return make_rsrc((const char*)g.parts + (place * g.splits + s) * g.part_bytes, (uint32_t)g.part_bytes); };
+        auto part = [&](int s) INLINE { return make_rsrc((const char*)g.parts + (place * g.splits + s) * g.part_bytes, (uint32_t)g.part_bytes); };
         const __amdgpu_buffer_rsrc_t own = part(split);
         if (!no_rows) {
 #pragma unroll
