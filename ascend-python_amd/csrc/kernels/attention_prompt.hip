@@ -17,6 +17,8 @@
 //
 // A masked weight is 0, but 0 times a NaN or an infinity in V is NaN: tiles that are masked for some rows look for such
 // values once they are staged, and the values are added apart, for the rows that see them.
+#include <type_traits>
+
 #include "attention_device.h"
 
 namespace qk {
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     __shared__ __attribute__((aligned(16))) uint64_t info[8][kKeys][2];  // addresses of a key's and a value's row (none: of zeros)
     __shared__ uint64_t info_ok[8];              // which keys of the tile exist
     __shared__ uint64_t bad[3];                  // which rows of V hold a NaN or an infinity
-    __shared__ float scales[8][2][kKeys];
+    __shared__ float scales[8][3][kKeys];         // int8: of the scores (with log2 e), of the values, and the latter's log2
     __shared__ int64_t found[2];
 
     const AttnArgs& a = g.a;
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     const int tile0 = (int)((int64_t)all_tiles * split / splits), tiles = (int)((int64_t)all_tiles * (split + 1) / splits);
 
     // the largest score is found before the scale is applied: a negative scale's sign goes to the query
-    const uint32_t turned = a.scale < 0.0f ? 0x80008000u : 0u;
+    const uint32_t turned = !Q8 && a.scale < 0.0f ? 0x80008000u : 0u;
     u32x4 q[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -244,10 +246,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
-    float m = kLowest, l = 0.0f, v_top = 0x1p-100f, v_inv = 0x1p100f;
+    float m = kLowest, l = 0.0f;
     bool any = false;
     // (a scale of 0 becomes one that leaves every product 0: -inf, a masked score, must stay what it is)
-    const float factor = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(fabsf(a.scale) * kLog2e, 0x1p-120f))));
+    const float factor = Q8 ? 1.0f : __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(fabsf(a.scale) * kLog2e, 0x1p-120f))));
 
     const bool paged = a.kv.table != nullptr;
     const Global zeros = global_address(kZeroRow);
@@ -308,8 +310,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     };
     auto put_scales = [&](int tile) INLINE {
         if constexpr (Q8) {
-            scales[tile + (lane >> 4) & 7][0][wave * 16 + (lane & 15)] = ks_next;
-            scales[tile + (lane >> 4) & 7][1][wave * 16 + (lane & 15)] = vs_next;
+            float* const to = &scales[tile + (lane >> 4) & 7][0][wave * 16 + (lane & 15)];
+            to[0] = ks_next * (a.scale * kLog2e);
+            to[kKeys] = vs_next;
+            to[2 * kKeys] = __builtin_amdgcn_logf(fmaxf(fabsf(vs_next), 0x1p-60f));
         }
     };
 
@@ -398,6 +402,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 for (int n = 0; n < 2; ++n) x[n] = mma32<DT>(*(const u32x4*)(kb + (k_at ^ s << 5) + 32 * n * LS), q[s], x[n]);
         };
 
+        uint64_t mine = ~0ull;  // the tile's keys that this lane's row sees, from the lane's first on: bit 32 n + 8 (e / 4) + e % 4
         bool edge = false;  // some row of the workgroup does not see some key of the tile at hand
         int32_t j0 = 0;     // the tile's first key
         uint64_t ok = 0;    // which of its keys exist
@@ -418,45 +423,50 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 for (int i = 0; i < NB; ++i) acc[i] *= keep;
             }
         };
-        auto apply_key_scales = [&](int tile, f32x16 (&x)[2]) INLINE {
+        // int8: scores times the keys' scales, in units of log2; the largest of them, each with its value's scale: what the weight that
+        // goes into the product is held against.  Keys that are hidden are not looked at.
+        auto scale_scores = [&](int tile, f32x16 (&x)[2], auto hide) INLINE {
+            float top = -__builtin_inff();
+            const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);  // few of them in registers at a time
                     const f32x4 k4 = *(const f32x4*)&scales[tile & 7][0][32 * n + 8 * i + 4 * kg];
+                    const f32x4 l4 = *(const f32x4*)&scales[tile & 7][2][32 * n + 8 * i + 4 * kg];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x[n][4 * i + r] *= k4[r];
+                    for (int r = 0; r < 4; ++r) {
+                        float v = x[n][4 * i + r] * k4[r];
+                        if constexpr (decltype(hide)::value) {
+                            const bool sees = (n ? hi : lo) & 1u << (8 * i + r);
+                            v = sees ? v : -__builtin_inff();
+                            top = fmaxf(top, sees ? v + l4[r] : -__builtin_inff());
+                        } else {
+                            top = __builtin_elementwise_maximum(top, v + l4[r]);
+                        }
+                        x[n][4 * i + r] = v;
+                    }
                 }
+            return top;
         };
-        // The weights take the values' scales; `seen` has a bit for each key, from this lane's first on.
-        auto apply_value_scales = [&](int tile, f32x16 (&x)[2], uint64_t seen) INLINE {
-            float part = 0.0f, most = 0.0f;
+        // int8: the weights' sum, and the weights with the values' scales (0 for what is hidden, whatever its scale)
+        auto scale_weights = [&](int tile, f32x16 (&x)[2], auto hide) INLINE {
+            const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
+            float part[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
                     const f32x4 v4 = *(const f32x4*)&scales[tile & 7][1][32 * n + 8 * i + 4 * kg];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float v = seen >> (32 * n + 8 * i + r) & 1 ? v4[r] : 0.0f;
-                        most = fmaxf(most, fabsf(v));
-                        part += x[n][4 * i + r];
-                        x[n][4 * i + r] *= v;
+                        part[r & 1] += x[n][4 * i + r];
+                        x[n][4 * i + r] *= !decltype(hide)::value || (n ? hi : lo) & 1u << (8 * i + r) ? v4[r] : 0.0f;
                     }
                 }
-            l += part;
-            if (__builtin_amdgcn_ballot_w64(most > v_top)) {
-                most = fmaxf(v_top, pair_max(most));
-                const float inv = 1.0f / most, keep = v_top * inv;
-                v_top = most;
-                v_inv = inv;
-#pragma unroll
-                for (int i = 0; i < NB; ++i) acc[i] *= keep;
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[n][e] *= v_inv;
+            l += part[0] + part[1];
         };
         // What every step begins with: K of the next tile and V of this one are in LDS behind its barrier.
         auto begin = [&](int it) INLINE {
@@ -475,15 +485,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             }
         };
 
-        uint64_t mine = ~0ull;  // the tile's keys that this lane's row sees, from the lane's first on: bit 32 n + 8 (e / 4) + e % 4
         // Looks at the tile whose scores x are there, `top` a lane's largest: hides what is not seen, moves the maximum.
         auto prepare = [&](int tile, f32x16 (&x)[2], float top) INLINE {
             look(tile);
             if (no_rows) return;
-            if constexpr (Q8) {
-                apply_key_scales(tile, x);
-                top = largest(x);
-            }
             mine = ~0ull;
             if (__builtin_expect(edge, 0)) {
                 // the tile's places that this row sees: up to its own, but for those between the sinks and its window
@@ -493,14 +498,19 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 if (a.window && p >= a.window) seen &= ~below(place_of(p - a.window + 1)) | below(place_of(a.sinks));
                 any |= seen != 0;
                 mine = seen >> here(4 * kg);
-                const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
+                if constexpr (Q8) {
+                    top = scale_scores(tile, x, std::true_type());
+                } else {
+                    const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[n][e] = (n ? hi : lo) & 1u << (8 * (e >> 2) + (e & 3)) ? x[n][e] : -__builtin_inff();
-                top = largest(x);
+                        for (int e = 0; e < 16; ++e) x[n][e] = (n ? hi : lo) & 1u << (8 * (e >> 2) + (e & 3)) ? x[n][e] : -__builtin_inff();
+                    top = largest(x);
+                }
             } else {
                 any = true;
+                if constexpr (Q8) top = scale_scores(tile, x, std::false_type());
             }
             raise(top);
         };
@@ -531,7 +541,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             }
             const uint32_t k_from = lds0 + 2 * (it + 1 & 1) * TILE + here(k_at);
             auto k_operand = [&](int i) INLINE { return lds_load(k_from ^ (i >> 1) << 5, 32 * (i & 1) * LS); };
-            constexpr int AHEAD1 = 6;
+            constexpr int AHEAD1 = Q8 ? 4 : 6;
             u32x4 k_ring[AHEAD1];
 #pragma unroll
             for (int i = 0; i < AHEAD1; ++i) k_ring[i] = k_operand(i);
@@ -553,7 +563,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 const u32x2 lo = lds_tr16(from, 16 * (i / NB) * LS), hi = lds_tr16(from, (16 * (i / NB) + 8) * LS);
                 return (u32x4){lo[0], lo[1], hi[0], hi[1]};
             };
-            constexpr int AHEAD2 = 4;
+            constexpr int AHEAD2 = Q8 ? 2 : 4;
             u32x4 v_ring[AHEAD2];
             // the next tile's scores, with this one's weights between the products
             {
@@ -587,7 +597,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (Q8) {
-                apply_value_scales(it, x, mine);
+                if (__builtin_expect(edge, 0)) scale_weights(it, x, std::true_type());
+                else scale_weights(it, x, std::false_type());
             } else if (__builtin_expect(edge, 0)) {
 #pragma nounroll
                 for (uint64_t left = uniform64(bad[it % 3]); left; left &= left - 1) {
@@ -661,10 +672,6 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     }
 
     l = pair_sum(l);
-    if (Q8) {
-#pragma unroll
-        for (int i = 0; i < NB; ++i) acc[i] *= v_top;
-    }
     if (splits > 1) {
         const int64_t place = (blockIdx.x / (uint32_t)(c.kv_heads * g.splits)) * c.kv_heads + kvh;
         // in the order of the registers: whole lines, and the joining lane finds its own rows
