@@ -698,24 +698,45 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
         if (!no_rows) {
-            for (int s = 0; s < splits; ++s) {
-                const __amdgpu_buffer_rsrc_t rs = part(s);
-                f32x4 v[NB][4];
-                const u32x2 ml = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, SUMS + (wave * 32 + col) * 8, 0, kCoherent));
+            auto max_and_sum = [&](int s) INLINE {
+                return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(part(s), SUMS + (wave * 32 + col) * 8, 0, kCoherent));
+            };
+            for (int s = 0; s < splits; s += 8) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) m = fmaxf(m, __uint_as_float(max_and_sum(s + k < splits ? s + k : s)[0]));
+            }
+            // two parts in registers: one on its way while the other is added
+            f32x4 v[2][NB][4];
+            u32x2 ml[2];
+            auto read = [&](int s, f32x4 (&to)[NB][4], u32x2& to_ml) INLINE {
+                const __amdgpu_buffer_rsrc_t rs = part(s < splits ? s : splits - 1);
+                to_ml = max_and_sum(s < splits ? s : splits - 1);
 #pragma unroll
                 for (int i = 0; i < NB; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        v[i][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, lane * 16, ((wave * NB + i) * 4 + e) * 1024, kCoherent));
-                const float pm = __uint_as_float(ml[0]), m2 = fmaxf(m, pm);
+                        to[i][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, lane * 16, ((wave * NB + i) * 4 + e) * 1024, kCoherent));
+            };
+            auto add = [&](f32x4 (&from)[NB][4], u32x2 from_ml) INLINE {
+                const float pm = __uint_as_float(from_ml[0]);
                 const bool none = pm == -__builtin_inff();
-                const float keep = none ? 1.0f : __builtin_amdgcn_exp2f(m - m2), f = none ? 0.0f : __builtin_amdgcn_exp2f(pm - m2);
-                m = m2;
-                l = l * keep + (none ? 0.0f : __uint_as_float(ml[1]) * f);
+                const float f = none ? 0.0f : __builtin_amdgcn_exp2f(pm - m);
+                l += none ? 0.0f : __uint_as_float(from_ml[1]) * f;
 #pragma unroll
                 for (int i = 0; i < NB; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[i][e] = none ? acc[i][e] : acc[i][e] * keep + v[i][e >> 2][e & 3] * f;
+                    for (int e = 0; e < 16; ++e) acc[i][e] += none ? 0.0f : from[i][e >> 2][e & 3] * f;
+            };
+            read(0, v[0], ml[0]);
+            for (int s = 0; s < splits; s += 2) {
+                read(s + 1, v[1], ml[1]);
+                __builtin_amdgcn_sched_barrier(0);
+                add(v[0], ml[0]);
+                __builtin_amdgcn_sched_barrier(0);
+                read(s + 2, v[0], ml[0]);
+                __builtin_amdgcn_sched_barrier(0);
+                if (s + 1 < splits) add(v[1], ml[1]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         any = m != -__builtin_inff();
