@@ -34,6 +34,36 @@ __device__ __forceinline__ void turn_of(const MropeArgs& a, int64_t t, int i, fl
     }
 }
 
+// cos and sin of N pairs from `first` on (N a multiple of 4 that divides it): two runs of the table's row where they lie in one
+// section, as they all but always do.  `whole`: the table is fp32, its rows whole 16-byte pieces.
+template <int N>
+__device__ __forceinline__ void turns_of(const MropeArgs& a, int64_t t, int first, bool whole, float (&c)[N], float (&s)[N]) {
+    int ax = 0, last = 0;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        ax += k + 1 < a.axes && first >= a.section_end[k];
+        last += k + 1 < a.axes && first + N - 1 >= a.section_end[k];
+    }
+    if (whole && ax == last) {
+        const int32_t p = a.positions[ax * a.position_stride + t];
+        if (p >= 0 && p < a.table_rows) {
+            const float* const row = (const float*)a.cos_sin + p * a.rotary_dim + first;
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                const f32x4 vc = *(const f32x4*)(row + i), vs = *(const f32x4*)(row + a.rotary_dim / 2 + i);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    c[i + k] = vc[k];
+                    s[i + k] = vs[k];
+                }
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) turn_of(a, t, first + i, c[i], s[i]);
+}
+
 __device__ __forceinline__ uint32_t to_bits(float v, int dtype) {
     return dtype == QK_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
 }
@@ -55,27 +85,29 @@ __device__ __forceinline__ Place place_of(const MropeArgs& a, int64_t t) {
     return p;
 }
 
+// Where head h is read: the query's heads, then the keys', then the values'.
+__device__ __forceinline__ const uint16_t* source_of(const MropeArgs& a, int64_t t, int h) {
+    const int Hq = (int)a.q_heads, Hkv = (int)a.kv_heads;
+    if (h < Hq) return (const uint16_t*)a.q + t * a.q_token_stride + h * a.q_head_stride;
+    if (h < Hq + Hkv) return (const uint16_t*)a.k + t * a.k_token_stride + (h - Hq) * a.k_head_stride;
+    return (const uint16_t*)a.v + t * a.v_token_stride + (h - Hq - Hkv) * a.v_head_stride;
+}
+// ... and where it goes
 struct Head {
-    const uint16_t* from;
     uint16_t* out;       // 16-bit result, or null
     uint16_t* out2;      // a second one (the key's own tensor beside a 16-bit cache), or null
     int8_t* quant;       // int8 cache row, or null
     float* quant_scale;
-    bool rotate;
 };
 __device__ __forceinline__ Head head_of(const MropeArgs& a, int64_t t, int h, const Place& p) {
     const int Hq = (int)a.q_heads, Hkv = (int)a.kv_heads;
     Head r = {};
-    r.rotate = h < Hq + Hkv;
     if (h < Hq) {
-        r.from = (const uint16_t*)a.q + t * a.q_token_stride + h * a.q_head_stride;
         r.out = a.out_q ? (uint16_t*)a.out_q + (t * Hq + h) * a.head_dim : nullptr;
         return r;
     }
     const bool key = h < Hq + Hkv;
     const int g = h - Hq - (key ? 0 : Hkv);
-    r.from = key ? (const uint16_t*)a.k + t * a.k_token_stride + g * a.k_head_stride
-                 : (const uint16_t*)a.v + t * a.v_token_stride + g * a.v_head_stride;
     if (key && a.out_k) r.out = (uint16_t*)a.out_k + (t * Hkv + g) * a.head_dim;
     if (p.cached) {
         const qk_kv_cache& c = a.c;
@@ -110,80 +142,96 @@ __device__ __forceinline__ u32x4 pack8(const float (&v)[8], int dtype) {
 }
 
 // Pieces of 16 bytes: a unit is two pieces of the first rotary_dim elements (interleaved: one), then one piece of the
-// rest.  `lanes` (a power of two, at most 32) lanes hold a head.
-__global__ __launch_bounds__(kThreads) void mrope_vec(MropeArgs a, int lanes, int units, int heads, int passes) {
+// rest.  `lanes` (a power of two, at most 32) lanes hold a head.  The rows of kAhead passes are asked for before the
+// factors, whose addresses wait for the positions.
+constexpr int kAhead = 4;
+template <bool INTER>
+__global__ __launch_bounds__(kThreads) void mrope_vec(MropeArgs a, int lanes, int units, int heads, int passes, bool whole) {
+    constexpr int N = INTER ? 4 : 8;  // pairs of a lane
     const int64_t t = blockIdx.x;
     const int u = threadIdx.x & (lanes - 1), per = kThreads / lanes;
     const int half = (int)a.rotary_dim / 2;
-    const int turning = a.interleave ? (int)a.rotary_dim / 8 : half / 8;
-    const bool two = !a.interleave && u < turning;
+    const int turning = half / N;
+    const bool two = !INTER && u < turning;
     const int first = u < turning ? 8 * u : (int)a.rotary_dim + 8 * (u - turning);
     const int second = first + half;  // read only where `two`
-    const Place place = place_of(a, t);
+    const int per_pass = per * gridDim.y, h0 = blockIdx.y * per + threadIdx.x / lanes;
 
-    float c[8], s[8];
-    if (u < turning) {
-        const int n = a.interleave ? 4 : 8;
+    u32x4 in0[kAhead], in1[kAhead];
+    auto ask = [&](int pass) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            c[i] = s[i] = 0.0f;
-            if (i < n) turn_of(a, t, n * u + i, c[i], s[i]);
+        for (int k = 0; k < kAhead; ++k) {
+            const int h = h0 + (pass + k) * per_pass;
+            in0[k] = in1[k] = (u32x4){0, 0, 0, 0};
+            if (pass + k < passes && h < heads && u < units) {
+                const uint16_t* const from = source_of(a, t, h);
+                in0[k] = *(const u32x4*)(from + first);
+                if (two) in1[k] = *(const u32x4*)(from + second);
+            }
         }
-    }
-    const int per_pass = per * gridDim.y;
-    for (int pass = 0, h = blockIdx.y * per + threadIdx.x / lanes; pass < passes; ++pass, h += per_pass) {
-        const bool on = h < heads && u < units;
-        Head hd = {};
-        float x[8] = {}, y[8] = {};
-        u32x4 w0 = {}, w1 = {};
-        if (on) {
-            hd = head_of(a, t, h, place);
-            w0 = *(const u32x4*)(hd.from + first);
-            if (two) w1 = *(const u32x4*)(hd.from + second);
-            if (hd.rotate && u < turning) {
-                unpack8(w0, a.dtype, x);
-                if (two) {
+    };
+    ask(0);
+    const Place place = place_of(a, t);
+    float c[N], s[N];
+    if (u < turning) turns_of<N>(a, t, N * u, whole, c, s);
+
+    for (int pass = 0; pass < passes; pass += kAhead) {
+        if (pass) ask(pass);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int h = h0 + (pass + k) * per_pass;
+            if (pass + k >= passes) break;
+            const bool on = h < heads && u < units;
+            Head hd = {};
+            float x[8] = {}, y[8] = {};
+            u32x4 w0 = in0[k], w1 = in1[k];
+            if (on) {
+                hd = head_of(a, t, h, place);
+                if (h < a.q_heads + a.kv_heads && u < turning) {
+                    unpack8(w0, a.dtype, x);
+                    if constexpr (!INTER) {
+                        unpack8(w1, a.dtype, y);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float x0 = x[i], x1 = y[i];
+                            x[i] = x0 * c[i] - x1 * s[i];
+                            y[i] = x1 * c[i] + x0 * s[i];
+                        }
+                        w1 = pack8(y, a.dtype);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x0 = x[2 * i], x1 = x[2 * i + 1];
+                            x[2 * i] = x0 * c[i] - x1 * s[i];
+                            x[2 * i + 1] = x1 * c[i] + x0 * s[i];
+                        }
+                    }
+                    w0 = pack8(x, a.dtype);
+                }
+                if (hd.out) {
+                    *(u32x4*)(hd.out + first) = w0;
+                    if (two) *(u32x4*)(hd.out + second) = w1;
+                }
+                if (hd.out2) {
+                    *(u32x4*)(hd.out2 + first) = w0;
+                    if (two) *(u32x4*)(hd.out2 + second) = w1;
+                }
+            }
+            if (a.cached && a.c.dtype == QK_I8) {
+                float amax = 0.0f;
+                if (hd.quant) {
+                    unpack8(w0, a.dtype, x);
                     unpack8(w1, a.dtype, y);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float x0 = x[i], x1 = y[i];
-                        x[i] = x0 * c[i] - x1 * s[i];
-                        y[i] = x1 * c[i] + x0 * s[i];
-                    }
-                    w1 = pack8(y, a.dtype);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x0 = x[2 * i], x1 = x[2 * i + 1];
-                        x[2 * i] = x0 * c[i] - x1 * s[i];
-                        x[2 * i + 1] = x1 * c[i] + x0 * s[i];
-                    }
+                    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(fabsf(x[i]), two ? fabsf(y[i]) : 0.0f));
                 }
-                w0 = pack8(x, a.dtype);
-            }
-            if (hd.out) {
-                *(u32x4*)(hd.out + first) = w0;
-                if (two) *(u32x4*)(hd.out + second) = w1;
-            }
-            if (hd.out2) {
-                *(u32x4*)(hd.out2 + first) = w0;
-                if (two) *(u32x4*)(hd.out2 + second) = w1;
-            }
-        }
-        if (a.cached && a.c.dtype == QK_I8) {
-            float amax = 0.0f;
-            if (hd.quant) {
-                unpack8(w0, a.dtype, x);
-                unpack8(w1, a.dtype, y);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(fabsf(x[i]), two ? fabsf(y[i]) : 0.0f));
-            }
-            for (int d = 1; d < lanes; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
-            if (hd.quant) {
-                const RowQuant rq = row_quant(amax / 127.0f);
-                *(u32x2*)(hd.quant + first) = quant8(x, rq);
-                if (two) *(u32x2*)(hd.quant + second) = quant8(y, rq);
-                if (u == 0) *hd.quant_scale = rq.s;
+                for (int d = 1; d < lanes; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
+                if (hd.quant) {
+                    const RowQuant rq = row_quant(amax / 127.0f);
+                    *(u32x2*)(hd.quant + first) = quant8(x, rq);
+                    if (two) *(u32x2*)(hd.quant + second) = quant8(y, rq);
+                    if (u == 0) *hd.quant_scale = rq.s;
+                }
             }
         }
     }
@@ -196,6 +244,8 @@ __global__ __launch_bounds__(kThreads) void mrope_any(MropeArgs a, int heads) {
     const int h = blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6);
     if (h >= heads) return;
     const Head hd = head_of(a, t, h, place_of(a, t));
+    const uint16_t* const from = source_of(a, t, h);
+    const bool rotate = h < a.q_heads + a.kv_heads;
     const int D = (int)a.head_dim, R = (int)a.rotary_dim, half = R / 2;
     const int units = half + D - R;
     uint32_t b0[4], b1[4];
@@ -207,9 +257,9 @@ __global__ __launch_bounds__(kThreads) void mrope_any(MropeArgs a, int heads) {
         if (u >= units) continue;
         const bool pair = u < half;
         const int e0 = !pair ? R + u - half : a.interleave ? 2 * u : u, e1 = a.interleave ? e0 + 1 : e0 + half;
-        b0[i] = hd.from[e0];
-        if (pair) b1[i] = hd.from[e1];
-        if (pair && hd.rotate) {
+        b0[i] = from[e0];
+        if (pair) b1[i] = from[e1];
+        if (pair && rotate) {
             float c, s;
             turn_of(a, t, u, c, s);
             const float x0 = load_half_bits(b0[i], a.dtype), x1 = load_half_bits(b1[i], a.dtype);
@@ -269,7 +319,10 @@ hipError_t launch_mrope(const MropeArgs& a, hipStream_t stream) {
         ++spread;
         passes = (heads + per * spread - 1) / (per * spread);
     }
-    mrope_vec<<<dim3((unsigned)a.tokens, (unsigned)spread), kThreads, 0, stream>>>(a, lanes, units, heads, passes);
+    const bool whole = a.cos_sin_dtype == QK_F32 && (uintptr_t)a.cos_sin % 16 == 0;
+    const dim3 grid((unsigned)a.tokens, (unsigned)spread);
+    if (a.interleave) mrope_vec<true><<<grid, kThreads, 0, stream>>>(a, lanes, units, heads, passes, whole);
+    else mrope_vec<false><<<grid, kThreads, 0, stream>>>(a, lanes, units, heads, passes, whole);
     return hipGetLastError();
 }
 
