@@ -289,7 +289,8 @@ __global__ __launch_bounds__(kPlan) void extend_plan(PoolArgs p, const int32_t* 
         if (i < n && seqs[i] >= 0 && seqs[i] < p.max_seqs) {
             const int64_t old = length_of(p, seqs[i]), len = old + grown_by(cu, i);
             const int64_t now = (len + p.page_size - 1) / p.page_size;
-            if (now > p.table_width) excess = (int32_t)(now - p.table_width);
+            // (no sum of the excesses passes 31 bits, whatever cu holds)
+            if (now > p.table_width) excess = (int32_t)(now - p.table_width < 32767 ? now - p.table_width : 32767);
             else pages = (int32_t)(now - (old + p.page_size - 1) / p.page_size);
         }
         int32_t all;

@@ -23,6 +23,8 @@ int launched(hipError_t e, const char* op) {
 
 constexpr int64_t kInt31 = ((int64_t)1 << 31) - 1;
 constexpr int64_t kMaxHeads = 65535;
+// Tokens of a sequence: the kernels count up to some hundreds past the last in 32 bits.
+constexpr int64_t kMaxTokens = kInt31 - 1024;
 
 bool is_half(int dt) { return dt == QK_F16 || dt == QK_BF16; }
 
@@ -92,7 +94,7 @@ int check_attention_sizes(const char* op, int64_t tokens, int64_t batch, int64_t
     if (tokens > kInt31 || batch > kInt31 || tokens > kInt31 / q_heads || batch > kInt31 / q_heads)
         return fail(QK_ERR_UNSUPPORTED, "%s: %lld rows of %lld heads exceed the launch limit", op,
                     (long long)(tokens > batch ? tokens : batch), (long long)q_heads);
-    if (table_width > kInt31 / c->page_size)
+    if (c->page_size > kMaxTokens || table_width > kMaxTokens / c->page_size)
         return fail(QK_ERR_UNSUPPORTED, "%s: a table of %lld pages of %lld tokens exceeds 31 bits", op,
                     (long long)table_width, (long long)c->page_size);
     return QK_OK;
