@@ -6,7 +6,7 @@
 // step, one of 131072, some 200 GB of a 32-layer cache, at most 32).  So the same calls give the same pages,
 // whatever the order of workgroups, and freeing is a subtraction.
 //
-// What moves bytes is one kernel: items of (pair of pages, tensor, 32 KB piece) handed to workgroups in turn, eight
+// What moves bytes is one kernel: items of (pair of pages, tensor, 16 KB piece) handed to workgroups in turn, four
 // 16-byte loads in flight per lane before the stores.  Bound by HBM: each byte is read and written once.
 #include "attention.h"
 
@@ -16,7 +16,7 @@ namespace {
 constexpr int kPlan = 1024;   // threads of a planning workgroup
 constexpr int kWaves = kPlan / 64;
 constexpr int kCopy = 256;    // threads of a copying workgroup
-constexpr int64_t kPiece = 32768;
+constexpr int64_t kPiece = 16384;
 constexpr int kTensors = 120; // tensors per launch: 2880 bytes of arguments
 
 struct PageList {
@@ -86,7 +86,7 @@ __device__ __forceinline__ int32_t length_of(const PoolArgs& p, int64_t seq) {
 
 template <typename T>
 __device__ __forceinline__ void copy_piece(const char* s, char* d, int64_t bytes) {
-    constexpr int kDeep = 8;
+    constexpr int kDeep = 4;
     const int64_t n = bytes / (int64_t)sizeof(T);
     const T* from = (const T*)s;
     T* to = (T*)d;

@@ -421,15 +421,32 @@ at::Tensor npu_mrope_scatter_kv_meta(const at::Tensor& positions, const at::Tens
 
 // ---------------------------------------------------------------- pages
 
+// A page (the dimensions behind the first) fills its bytes, in whatever order.  From the sizes and strides alone: a view per tensor
+// would cost more than the launch.
+bool page_is_dense(const at::Tensor& t) {
+    const auto sizes = t.sizes(), strides = t.strides();
+    int64_t next = 1;
+    uint64_t done = 0;
+    for (int64_t left = t.dim() - 1; left > 0; --left) {
+        int64_t found = 0;  // the dimension whose stride is the product of those before it
+        for (int64_t d = 1; d < t.dim() && !found; ++d)
+            if (!(done >> d & 1) && (sizes[d] == 1 || strides[d] == next)) found = d;
+        if (!found) return false;
+        done |= (uint64_t)1 << found;
+        next *= sizes[found];
+    }
+    return true;
+}
+
 std::vector<qk_pages> page_list(const char* op, at::TensorList caches, int64_t num_pages, const at::Tensor& like) {
     std::vector<qk_pages> list;
     list.reserve(caches.size());
     for (const at::Tensor& t : caches) {
-        TORCH_CHECK(t.dim() >= 1 && t.size(0) == num_pages, op, ": every cache tensor must have ", num_pages,
+        TORCH_CHECK(t.dim() >= 1 && t.dim() <= 64 && t.size(0) == num_pages, op, ": every cache tensor must have ", num_pages,
                     " pages in its first dimension, got ", t.sizes());
         check_device(op, "a cache tensor", t, like);
         if (t.numel() == 0) continue;
-        TORCH_CHECK(t.select(0, 0).is_non_overlapping_and_dense(), op, ": a page of a cache tensor must be dense, got sizes ",
+        TORCH_CHECK(page_is_dense(t), op, ": a page of a cache tensor must be dense, got sizes ",
                     t.sizes(), " and strides ", t.strides());
         const int64_t bytes = t.numel() / num_pages * t.element_size();
         TORCH_CHECK(num_pages == 1 || t.stride(0) * t.element_size() >= bytes, op, ": pages of a cache tensor overlap");
