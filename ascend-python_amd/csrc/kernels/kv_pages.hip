@@ -151,9 +151,9 @@ hipError_t for_lists(const qk_pages* pages, int64_t tensors, F launch) {
     return hipSuccess;
 }
 
-// Workgroups for a number of items that may be large: eight per CU take them in turn.
+// Workgroups for a number of items that may be large: as many as are resident four times over take them in turn (2048: 2 % slower).
 unsigned copy_grid(int64_t items) {
-    const int64_t most = 2048;
+    const int64_t most = 8192;
     return (unsigned)(items < 1 ? 1 : items < most ? items : most);
 }
 

@@ -142,9 +142,9 @@ __device__ __forceinline__ u32x4 pack8(const float (&v)[8], int dtype) {
 }
 
 // Pieces of 16 bytes: a unit is two pieces of the first rotary_dim elements (interleaved: one), then one piece of the
-// rest.  `lanes` (a power of two, at most 32) lanes hold a head.  The rows of kAhead passes are asked for before the
-// factors, whose addresses wait for the positions.
-constexpr int kAhead = 4;
+// rest.  `lanes` (a power of two, at most 32) lanes hold a head.  The first pass's rows are asked for before the
+// factors, whose addresses wait for the positions; more passes ahead cost registers, and with them waves (4099 tokens with
+// three axes: none ahead but the first 22.0 us, 4.6 TB/s; two 24.0; four 25.9).
 template <bool INTER>
 __global__ __launch_bounds__(kThreads) void mrope_vec(MropeArgs a, int lanes, int units, int heads, int passes, bool whole) {
     constexpr int N = INTER ? 4 : 8;  // pairs of a lane
@@ -157,81 +157,73 @@ __global__ __launch_bounds__(kThreads) void mrope_vec(MropeArgs a, int lanes, in
     const int second = first + half;  // read only where `two`
     const int per_pass = per * gridDim.y, h0 = blockIdx.y * per + threadIdx.x / lanes;
 
-    u32x4 in0[kAhead], in1[kAhead];
-    auto ask = [&](int pass) {
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const int h = h0 + (pass + k) * per_pass;
-            in0[k] = in1[k] = (u32x4){0, 0, 0, 0};
-            if (pass + k < passes && h < heads && u < units) {
-                const uint16_t* const from = source_of(a, t, h);
-                in0[k] = *(const u32x4*)(from + first);
-                if (two) in1[k] = *(const u32x4*)(from + second);
-            }
+    u32x4 in0, in1;
+    auto ask = [&](int h) {
+        in0 = in1 = (u32x4){0, 0, 0, 0};
+        if (h < heads && u < units) {
+            const uint16_t* const from = source_of(a, t, h);
+            in0 = *(const u32x4*)(from + first);
+            if (two) in1 = *(const u32x4*)(from + second);
         }
     };
-    ask(0);
+    ask(h0);
     const Place place = place_of(a, t);
     float c[N], s[N];
     if (u < turning) turns_of<N>(a, t, N * u, whole, c, s);
 
-    for (int pass = 0; pass < passes; pass += kAhead) {
-        if (pass) ask(pass);
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const int h = h0 + (pass + k) * per_pass;
-            if (pass + k >= passes) break;
-            const bool on = h < heads && u < units;
-            Head hd = {};
-            float x[8] = {}, y[8] = {};
-            u32x4 w0 = in0[k], w1 = in1[k];
-            if (on) {
-                hd = head_of(a, t, h, place);
-                if (h < a.q_heads + a.kv_heads && u < turning) {
-                    unpack8(w0, a.dtype, x);
-                    if constexpr (!INTER) {
-                        unpack8(w1, a.dtype, y);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float x0 = x[i], x1 = y[i];
-                            x[i] = x0 * c[i] - x1 * s[i];
-                            y[i] = x1 * c[i] + x0 * s[i];
-                        }
-                        w1 = pack8(y, a.dtype);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x0 = x[2 * i], x1 = x[2 * i + 1];
-                            x[2 * i] = x0 * c[i] - x1 * s[i];
-                            x[2 * i + 1] = x1 * c[i] + x0 * s[i];
-                        }
-                    }
-                    w0 = pack8(x, a.dtype);
-                }
-                if (hd.out) {
-                    *(u32x4*)(hd.out + first) = w0;
-                    if (two) *(u32x4*)(hd.out + second) = w1;
-                }
-                if (hd.out2) {
-                    *(u32x4*)(hd.out2 + first) = w0;
-                    if (two) *(u32x4*)(hd.out2 + second) = w1;
-                }
-            }
-            if (a.cached && a.c.dtype == QK_I8) {
-                float amax = 0.0f;
-                if (hd.quant) {
-                    unpack8(w0, a.dtype, x);
+    for (int pass = 0; pass < passes; ++pass) {
+        const int h = h0 + pass * per_pass;
+        if (pass) ask(h);
+        const bool on = h < heads && u < units;
+        Head hd = {};
+        float x[8] = {}, y[8] = {};
+        u32x4 w0 = in0, w1 = in1;
+        if (on) {
+            hd = head_of(a, t, h, place);
+            if (h < a.q_heads + a.kv_heads && u < turning) {
+                unpack8(w0, a.dtype, x);
+                if constexpr (!INTER) {
                     unpack8(w1, a.dtype, y);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(fabsf(x[i]), two ? fabsf(y[i]) : 0.0f));
+                    for (int i = 0; i < 8; ++i) {
+                        const float x0 = x[i], x1 = y[i];
+                        x[i] = x0 * c[i] - x1 * s[i];
+                        y[i] = x1 * c[i] + x0 * s[i];
+                    }
+                    w1 = pack8(y, a.dtype);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x0 = x[2 * i], x1 = x[2 * i + 1];
+                        x[2 * i] = x0 * c[i] - x1 * s[i];
+                        x[2 * i + 1] = x1 * c[i] + x0 * s[i];
+                    }
                 }
-                for (int d = 1; d < lanes; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
-                if (hd.quant) {
-                    const RowQuant rq = row_quant(amax / 127.0f);
-                    *(u32x2*)(hd.quant + first) = quant8(x, rq);
-                    if (two) *(u32x2*)(hd.quant + second) = quant8(y, rq);
-                    if (u == 0) *hd.quant_scale = rq.s;
-                }
+                w0 = pack8(x, a.dtype);
+            }
+            if (hd.out) {
+                *(u32x4*)(hd.out + first) = w0;
+                if (two) *(u32x4*)(hd.out + second) = w1;
+            }
+            if (hd.out2) {
+                *(u32x4*)(hd.out2 + first) = w0;
+                if (two) *(u32x4*)(hd.out2 + second) = w1;
+            }
+        }
+        if (a.cached && a.c.dtype == QK_I8) {
+            float amax = 0.0f;
+            if (hd.quant) {
+                unpack8(w0, a.dtype, x);
+                unpack8(w1, a.dtype, y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(fabsf(x[i]), two ? fabsf(y[i]) : 0.0f));
+            }
+            for (int d = 1; d < lanes; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
+            if (hd.quant) {
+                const RowQuant rq = row_quant(amax / 127.0f);
+                *(u32x2*)(hd.quant + first) = quant8(x, rq);
+                if (two) *(u32x2*)(hd.quant + second) = quant8(y, rq);
+                if (u == 0) *hd.quant_scale = rq.s;
             }
         }
     }
