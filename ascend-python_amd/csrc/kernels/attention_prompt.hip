@@ -406,8 +406,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         bool edge = false;  // some row of the workgroup does not see some key of the tile at hand
         int32_t j0 = 0;     // the tile's first key
         uint64_t ok = 0;    // which of its keys exist
-        auto look = [&](int tile) INLINE {
-            ok = uniform64(info_ok[tile & 7]);
+        auto look = [&](int tile, uint64_t which) INLINE {
+            ok = uniform64(which);
             const int32_t last = tile * kKeys + kKeys - 1, j1 = last + (last < sinks ? 0 : gap);
             j0 = tile * kKeys + (tile * kKeys < sinks ? 0 : gap);
             edge = ~ok != 0 || j1 > p_first || (a.window && j1 >= a.sinks && p_last - j0 >= a.window);
@@ -486,8 +486,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         };
 
         // Looks at the tile whose scores x are there, `top` a lane's largest: hides what is not seen, moves the maximum.
-        auto prepare = [&](int tile, f32x16 (&x)[2], float top) INLINE {
-            look(tile);
+        auto prepare = [&](int tile, uint64_t which, f32x16 (&x)[2], float top) INLINE {
+            look(tile, which);
             if (no_rows) return;
             mine = ~0ull;
             if (__builtin_expect(edge, 0)) {
@@ -536,7 +536,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 behind_barrier(it);
                 load_tile(it + 2, 0);
                 load_tile(it + 1, 1);
-                look(it + 1);
+                look(it + 1, info_ok[it + 1 & 7]);
                 return;
             }
             const uint32_t k_from = lds0 + 2 * (it + 1 & 1) * TILE + here(k_at);
@@ -557,6 +557,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
 #pragma unroll
                 for (int i = 0; i < SENDS; ++i) from[i] = address(i < DMAS ? it + 2 : it + 1, i / DMAS, i % DMAS);
             }
+            const uint64_t ok_next = info_ok[it + 1 & 7];  // asked for here, used at the step's end
             const uint32_t v_from = lds0 + (2 * (it & 1) + 1) * TILE + here(v_at);
             auto v_operand = [&](int i) INLINE {
                 const uint32_t from = v_from ^ (i % NB) << 6;
@@ -659,12 +660,12 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (!Q8) l += (part[0] + part[1]) + (part[2] + part[3]);
             }
-            prepare(it + 1, y, top);
+            prepare(it + 1, ok_next, y, top);
         };
 
         f32x16 xa[2], xb[2];
         if (!no_rows) scores(tile0, xa);
-        prepare(tile0, xa, largest(xa));
+        prepare(tile0, info_ok[tile0 & 7], xa, largest(xa));
         for (int it = tile0; it < tiles; it += 2) {
             step(it, xa, xb);
             if (it + 1 < tiles) step(it + 1, xb, xa);
