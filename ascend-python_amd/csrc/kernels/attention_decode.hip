@@ -152,6 +152,14 @@ __global__ __launch_bounds__(kThreads, KS <= 4 ? 3 : KS <= 6 ? 2 : 1) void atten
     char* const v_lds = lds + wave * WAVE_LDS;
     float* const s_lds = (float*)(v_lds + kTile * VROW);  // 32 key scales (with the scores' factor), value scales, their log2
     const float factor = a.scale * kLog2e;
+    // What finds the rows reads its arguments from memory again each time: some thirty scalar registers, which would otherwise be
+    // kept in lanes of vector registers and moved through the vector unit.
+    auto args = []() {
+        const __attribute__((address_space(4))) DecodeArgs* from =
+            (const __attribute__((address_space(4))) DecodeArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(from));
+        return from;
+    };
     const Global zeros = global_address(kZeroRow);
 
     for (int64_t u0 = line.begin; u0 < line.end;) {
@@ -193,8 +201,6 @@ __global__ __launch_bounds__(kThreads, KS <= 4 ? 3 : KS <= 6 ? 2 : 1) void atten
         bool any = false;
 
         const int32_t* const table = a.kv.table + b * a.kv.table_stride;
-        const Global k_base = global_address(c.key) + kvh * c.key_head_stride * (Q8 ? 1 : 2) + 16 * kg;
-        const Global v_base = global_address(c.value) + kvh * c.value_head_stride * (Q8 ? 1 : 2) + 16 * kg;
         constexpr int ES = Q8 ? 1 : 2;
 
         // page of this lane's key of each half tile (-1: none), and the key's slot
@@ -215,7 +221,11 @@ __global__ __launch_bounds__(kThreads, KS <= 4 ? 3 : KS <= 6 ? 2 : 1) void atten
         u32x4 kr[2][LOADS], vr[2][LOADS];
         float ksc[2], vsc[2];
         uint32_t ok[2];  // which of the tile's keys are seen: 16 bits each
-        auto load_tile = [&](const int32_t (&page)[2], const int32_t (&slot)[2]) {
+        auto load_tile = [&](const int32_t (&page)[2], const int32_t (&slot)[2]) __attribute__((always_inline)) {
+            const auto* g = args();
+            const auto& c = g->a.kv.c;
+            const Global k_base = global_address(c.key) + kvh * c.key_head_stride * ES + 16 * kg;
+            const Global v_base = global_address(c.value) + kvh * c.value_head_stride * ES + 16 * kg;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const bool valid = page[t] >= 0 && page[t] < c.num_pages;
