@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     
     // the keys that any row sees, without a gap: key j is place j or, past the sinks, j - gap
     int32_t low = 0, sinks = 0;
-    if (a.window && p_first - a.window + 1 > 0) {
+    if (a.window && p_first >= a.window) {  // (a tile may begin before the first key: a difference could pass 32 bits)
         low = p_first - a.window + 1;
         sinks = a.sinks < low ? a.sinks : low;
     }
