@@ -28,6 +28,9 @@ constexpr int64_t kMaxTokens = kInt31 - 1024;
 
 bool is_half(int dt) { return dt == QK_F16 || dt == QK_BF16; }
 
+// A window, and its first tokens that stay visible, as the kernels and their plans take them: past 31 bits is without end.
+int32_t cut31(int64_t v) { return (int32_t)(v > kInt31 ? kInt31 : v); }
+
 int check_workspace(const char* op, size_t need, const void* workspace, size_t workspace_bytes) {
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(QK_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", op, need, workspace_bytes);
@@ -110,8 +113,6 @@ int check_query(const char* op, const void* query, int64_t token_stride, int64_t
     return QK_OK;
 }
 
-int32_t cut31(int64_t v) { return (int32_t)(v > kInt31 ? kInt31 : v); }
-
 qk::AttnArgs attention_args(const void* query, int dtype, int64_t tokens, int64_t batch, int64_t q_heads,
                             int64_t q_token_stride, int64_t q_head_stride, const qk_kv_cache* cache,
                             const int32_t* table, int64_t table_width, int64_t table_stride, const int32_t* lens,
@@ -183,7 +184,7 @@ int qk_paged_attention_workspace_size(int64_t batch, int64_t q_heads, const qk_k
     if (int rc = check_attention_sizes(op, batch, batch, q_heads, cache, cache && cache->dtype != QK_I8 ? cache->dtype : QK_BF16,
                                        table_width, window, sinks))
         return rc;
-    *bytes = qk::attention_decode_workspace(batch, q_heads, *cache, table_width, window, sinks);
+    *bytes = qk::attention_decode_workspace(batch, q_heads, *cache, table_width, cut31(window), cut31(sinks));
     return QK_OK;
 }
 
@@ -219,7 +220,7 @@ int qk_prompt_attention_workspace_size(int64_t tokens, int64_t batch, int64_t q_
     if (int rc = check_attention_sizes(op, tokens, batch, q_heads, cache, cache && cache->dtype != QK_I8 ? cache->dtype : QK_BF16,
                                        table_width, window, sinks))
         return rc;
-    *bytes = qk::attention_prompt_workspace(tokens, batch, q_heads, *cache, table_width, window, sinks);
+    *bytes = qk::attention_prompt_workspace(tokens, batch, q_heads, *cache, table_width, cut31(window), cut31(sinks));
     return QK_OK;
 }
 

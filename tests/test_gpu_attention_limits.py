@@ -24,3 +24,12 @@ def test_decode_window_without_end(ops, window):  # noqa: F811
     got = _run_decode(ops, [0, 1, 333], 4, 2, 64, 16, BF16, window=window, sinks=window)
     want = _run_decode(ops, [0, 1, 333], 4, 2, 64, 16, BF16)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("sinks", [2 ** 31 - 1, 2 ** 63 - 128, sys.maxsize])
+def test_prompt_sinks_without_end(ops, sinks, quant):  # noqa: F811
+    """With every key a sink a window hides nothing; few rows over a long past, so the keys are cut into parts."""
+    got = _run_prompt(ops, [3, 1], 4, 1, 64, past=[3000, 700], page=16, quant=quant, window=100, sinks=sinks)
+    want = _run_prompt(ops, [3, 1], 4, 1, 64, past=[3000, 700], page=16, quant=quant)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
