@@ -25,8 +25,9 @@ def quant_attention(x: torch.Tensor, gamma: torch.Tensor, w_qkv: torch.Tensor, s
                     eps: float = 1e-6) -> torch.Tensor:
     """x [T, H] fp16/bf16: the new tokens of sequences ``seqs``, cu_tokens[i] .. cu_tokens[i + 1] of the i-th; cu_tokens
     None: one token each.  slots and positions as ``cache.extend`` gave them (positions [axes, T] with ``sections`` for
-    images and video), once for all layers.  w_qkv int8 [H, (q_heads + 2 * kv_heads) * head_dim], w_o int8
-    [q_heads * head_dim, H], as quant_mlp takes its weights.  -> [T, H]."""
+    images and video), once for all layers.  A sequence number that ``extend`` passes over sees nothing: its rows are 0.
+    w_qkv int8 [H, (q_heads + 2 * kv_heads) * head_dim], w_o int8 [q_heads * head_dim, H], as quant_mlp takes its
+    weights.  -> [T, H]."""
     kv_heads, head_dim = cache.keys[layer].shape[2:]
     y, s, _ = npu_rms_norm_dynamic_quant(x, gamma, eps)
     qkv = npu_quant_matmul(y, w_qkv, s_qkv, pertoken_scale=s, output_dtype=x.dtype)
@@ -34,7 +35,7 @@ def quant_attention(x: torch.Tensor, gamma: torch.Tensor, w_qkv: torch.Tensor, s
     scales = dict(key_scale=cache.key_scales[layer], value_scale=cache.value_scales[layer])
     q = npu_mrope_scatter_kv(positions, q, k, v, cos_sin, cache.keys[layer], cache.values[layer], slots,
                              mrope_section=sections, rotary_mode=rotary_mode, **scales)
-    table, lens = cache.block_table[seqs], cache.context_lens[seqs]
+    table, lens = cache.rows(seqs)
     if cu_tokens is None:
         o, _ = npu_paged_attention(q, cache.keys[layer], cache.values[layer], table, lens, window=window, sinks=sinks, **scales)
     else:

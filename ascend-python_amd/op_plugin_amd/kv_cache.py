@@ -54,6 +54,15 @@ class PagedKVCache:
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         npu_kv_copy_pages(self._pools(), src, dst)
 
+    def rows(self, seqs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """The page table's rows and the lengths of seqs, as the attention ops take them.  A sequence number that the other
+        calls pass over (negative, or max_seqs and more: a batch's padding) has no tokens."""
+        if self.context_lens.numel() == 0:
+            return self.block_table.new_full((seqs.numel(), self.block_table.shape[1]), -1), self.context_lens.new_zeros(seqs.numel())
+        held = seqs.clamp(0, self.context_lens.numel() - 1)
+        at = held.long()
+        return self.block_table[at], self.context_lens[at].masked_fill_(held != seqs, 0)
+
     def compact(self) -> torch.Tensor:
         """Moves the pages in use to the front of the pool; how many moved, on the device."""
         self.block_table, self.ref_count, moved = npu_kv_compact(self._pools(), self.block_table, self.ref_count)

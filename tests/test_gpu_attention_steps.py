@@ -1,0 +1,66 @@
+"""quant_attention and the paged cache in a server's steps: padded batches."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+H, HQ, HKV, D, LAYERS = 256, 8, 2, 64, 2
+
+
+@pytest.fixture(scope="module")
+def mods():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from op_plugin_amd import attention, kv_cache
+    return attention, kv_cache
+
+
+def _ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+class Model:
+    """The weights of one attention block, and its steps over a cache."""
+
+    def __init__(self, mods, kind=torch.bfloat16, seed=0):
+        self.att, kvc = mods
+        self.g = torch.Generator().manual_seed(seed)
+        self.cache = kvc.PagedKVCache(LAYERS, 40, 16, HKV, D, max_seqs=6, max_len=200, dtype=kind, device=DEV)
+        int8 = lambda *shape: torch.randint(-127, 128, shape, generator=self.g, dtype=torch.int8).to(DEV)  # noqa: E731
+        self.w_qkv, self.w_o = int8(H, (HQ + 2 * HKV) * D), int8(HQ * D, H)
+        self.s_qkv, self.s_o = torch.full((self.w_qkv.shape[1],), 1e-3, device=DEV), torch.full((H,), 1e-3, device=DEV)
+        self.gamma = torch.ones(H, dtype=torch.bfloat16, device=DEV)
+        angle = torch.arange(256, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)
+        self.cos_sin = torch.cat([angle.cos(), angle.sin()], 1).float().to(DEV)
+
+    def input(self, tokens):
+        return torch.randn((tokens, H), generator=self.g).to(torch.bfloat16).to(DEV)
+
+    def step(self, x, seqs, cu, one_each=False, **kw):
+        """x through the block in every layer, each layer's own cache; the layers' outputs."""
+        slots, positions, missing = self.cache.extend(seqs, cu, x.shape[0])
+        return [self.att.quant_attention(x, self.gamma, self.w_qkv, self.s_qkv, self.w_o, self.s_o, self.cache, layer, seqs,
+                                         None if one_each else cu, slots, positions, self.cos_sin, HQ, **kw)
+                for layer in range(LAYERS)], missing
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.int8])
+def test_padded_batches(mods, kind):
+    """Sequence numbers outside the table are padding: their rows are 0, and the others what they are without."""
+    print(f"[case] padded batches {kind}", flush=True)
+    a, b = Model(mods, kind), Model(mods, kind)
+    x = a.input(37 + 5)
+    plain, _ = a.step(x, _ints([0, 5]), _ints([0, 37, 42]))
+    wide = torch.cat([a.input(3), x[:37], a.input(2), x[37:]])
+    padded, missing = b.step(wide, _ints([-1, 0, 6, 5]), _ints([0, 3, 40, 42, 47]))
+    assert int(missing) == 0
+    for p, w in zip(plain, padded):
+        assert torch.equal(p, torch.cat([w[3:40], w[42:]])) and (w[:3] == 0).all() and (w[40:42] == 0).all()
+    x = a.input(2)
+    plain, _ = a.step(x, _ints([5, 0]), _ints([0, 1, 2]), one_each=True)
+    wide = torch.cat([x[:1], a.input(2), x[1:], a.input(1)])
+    padded, missing = b.step(wide, _ints([5, -1, 2 ** 31 - 1, 0, 6]), _ints([0, 1, 2, 3, 4, 5]), one_each=True)
+    assert int(missing) == 0
+    for p, w in zip(plain, padded):
+        assert torch.equal(p, w[[0, 3]]) and (w[[1, 2, 4]] == 0).all()
+    assert torch.equal(a.cache.block_table, b.cache.block_table) and torch.equal(a.cache.context_lens, b.cache.context_lens)
