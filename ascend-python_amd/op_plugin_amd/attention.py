@@ -21,11 +21,12 @@ from .kv_cache import PagedKVCache
 def quant_attention(x: torch.Tensor, gamma: torch.Tensor, w_qkv: torch.Tensor, s_qkv: torch.Tensor, w_o: torch.Tensor,
                     s_o: torch.Tensor, cache: PagedKVCache, layer: int, seqs: torch.Tensor, cu_tokens: torch.Tensor | None,
                     slots: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, q_heads: int, *,
-                    sections: list[int] | None = None, rotary_mode: str = "half", window: int = 0, sinks: int = 0,
-                    eps: float = 1e-6) -> torch.Tensor:
+                    rows: tuple[torch.Tensor, torch.Tensor] | None = None, sections: list[int] | None = None,
+                    rotary_mode: str = "half", window: int = 0, sinks: int = 0, eps: float = 1e-6) -> torch.Tensor:
     """x [T, H] fp16/bf16: the new tokens of sequences ``seqs``, cu_tokens[i] .. cu_tokens[i + 1] of the i-th; cu_tokens
     None: one token each.  slots and positions as ``cache.extend`` gave them (positions [axes, T] with ``sections`` for
-    images and video), once for all layers.  A sequence number that ``extend`` passes over sees nothing: its rows are 0.
+    images and video), once for all layers, and so is rows, ``cache.rows(seqs)`` after ``extend`` (None: taken here, in
+    every layer again).  A sequence number that ``extend`` passes over sees nothing: its rows are 0.
     w_qkv int8 [H, (q_heads + 2 * kv_heads) * head_dim], w_o int8 [q_heads * head_dim, H], as quant_mlp takes its
     weights.  -> [T, H]."""
     kv_heads, head_dim = cache.keys[layer].shape[2:]
@@ -35,7 +36,7 @@ def quant_attention(x: torch.Tensor, gamma: torch.Tensor, w_qkv: torch.Tensor, s
     scales = dict(key_scale=cache.key_scales[layer], value_scale=cache.value_scales[layer])
     q = npu_mrope_scatter_kv(positions, q, k, v, cos_sin, cache.keys[layer], cache.values[layer], slots,
                              mrope_section=sections, rotary_mode=rotary_mode, **scales)
-    table, lens = cache.rows(seqs)
+    table, lens = rows if rows is not None else cache.rows(seqs)
     if cu_tokens is None:
         o, _ = npu_paged_attention(q, cache.keys[layer], cache.values[layer], table, lens, window=window, sinks=sinks, **scales)
     else:

@@ -64,3 +64,20 @@ def test_padded_batches(mods, kind):
     for p, w in zip(plain, padded):
         assert torch.equal(p, w[[0, 3]]) and (w[[1, 2, 4]] == 0).all()
     assert torch.equal(a.cache.block_table, b.cache.block_table) and torch.equal(a.cache.context_lens, b.cache.context_lens)
+
+
+@pytest.mark.parametrize("one_each", [False, True])
+def test_rows_taken_once(mods, one_each, monkeypatch):
+    """The table's rows taken once for all layers give the bits of rows taken in each layer."""
+    print(f"[case] rows taken once one_each={one_each}", flush=True)
+    a, b = Model(mods), Model(mods)
+    seqs, cu = _ints([3, -1, 0]), _ints([0, 1, 2, 3] if one_each else [0, 20, 21, 60])
+    x = a.input(3 if one_each else 60)
+    want, _ = a.step(x, seqs, cu, one_each)
+    slots, positions, _ = b.cache.extend(seqs, cu, x.shape[0])
+    rows = b.cache.rows(seqs)
+    monkeypatch.setattr(b.cache, "rows", None)  # no layer takes them again
+    for layer in range(LAYERS):
+        got = b.att.quant_attention(x, b.gamma, b.w_qkv, b.s_qkv, b.w_o, b.s_o, b.cache, layer, seqs, None if one_each else cu,
+                                    slots, positions, b.cos_sin, HQ, rows=rows)
+        assert torch.equal(got, want[layer])
