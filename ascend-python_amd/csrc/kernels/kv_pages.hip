@@ -25,18 +25,19 @@ struct PageList {
 };
 
 // Sum of v over the threads before this one, and over all (LDS: two barriers).
-__device__ __forceinline__ int32_t scan_before(int32_t v, int32_t& total, int32_t* sums) {
+template <typename T>
+__device__ __forceinline__ T scan_before(T v, T& total, T* sums) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int32_t in = v;
+    T in = v;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int32_t o = __shfl_up(in, d);
+        const T o = __shfl_up(in, d);
         if (lane >= d) in += o;
     }
     __syncthreads();  // the sums of the previous call have been read
     if (lane == 63) sums[wave] = in;
     __syncthreads();
-    int32_t before = 0, all = 0;
+    T before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         before += w < wave ? sums[w] : 0;
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(kPlan) void fork_plan(PoolArgs p, const int32_t* pa
             }
         }
         int32_t all;
-        const int32_t rank = need + scan_before(started, all, sums);
+        const int32_t rank = need + scan_before((int32_t)started, all, sums);
         need += all;
         if (i < n) {
             src[i] = page;
@@ -243,8 +244,8 @@ __global__ __launch_bounds__(kCopy) void free_seqs(PoolArgs p, const int32_t* se
 
 // ---------------------------------------------------------------- extend
 
-__device__ __forceinline__ int32_t grown_by(const int32_t* cu, int64_t i) {
-    const int32_t d = cu[i + 1] - cu[i];
+__device__ __forceinline__ int64_t grown_by(const int32_t* cu, int64_t i) {
+    const int64_t d = (int64_t)cu[i + 1] - cu[i];
     return d < 0 ? 0 : d;
 }
 
@@ -267,7 +268,7 @@ __device__ __forceinline__ void place_token(const PoolArgs& p, const int32_t* se
         const int64_t i = last_at_most(cu, n, (int32_t)t);
         const int32_t seq = seqs[i];
         if (seq >= 0 && seq < p.max_seqs) {
-            position = p.lens[seq] - grown_by(cu, i) + (int32_t)(t - cu[i]);
+            position = (int32_t)(p.lens[seq] - grown_by(cu, i) + (t - cu[i]));
             const int64_t at = position / p.page_size;
             if (position >= 0 && at < p.table_width)
                 slot = (int32_t)(p.table[seq * p.table_stride + at] * p.page_size + position % p.page_size);
@@ -282,31 +283,32 @@ __global__ __launch_bounds__(kPlan) void extend_plan(PoolArgs p, const int32_t* 
                                                      int64_t total, int32_t* slots, int32_t* positions, int32_t* missing,
                                                      int32_t* ws) {
     __shared__ int32_t sums[kWaves];
+    __shared__ int64_t wide[kWaves];
     int32_t *first = ws, *fresh = ws + n;
-    int32_t need = 0, over = 0;
+    // Sums over the sequences are of 64 bits: cu_tokens that fall, and rise again, ask for any number of pages.
+    int64_t need = 0, over = 0;
     for (int64_t base = 0; base < n; base += kPlan) {
         const int64_t i = base + threadIdx.x;
-        int32_t pages = 0, excess = 0;
+        int64_t pages = 0, excess = 0;
         if (i < n && seqs[i] >= 0 && seqs[i] < p.max_seqs) {
             const int64_t old = length_of(p, seqs[i]), len = old + grown_by(cu, i);
             const int64_t now = (len + p.page_size - 1) / p.page_size;
-            // (no sum of the excesses passes 31 bits, whatever cu holds)
-            if (now > p.table_width) excess = (int32_t)(now - p.table_width < 32767 ? now - p.table_width : 32767);
-            else pages = (int32_t)(now - (old + p.page_size - 1) / p.page_size);
+            if (now > p.table_width) excess = now - p.table_width;
+            else pages = now - (old + p.page_size - 1) / p.page_size;
         }
-        int32_t all;
-        const int32_t rank = need + scan_before(pages, all, sums);
+        int64_t all;
+        const int64_t rank = need + scan_before(pages, all, wide);
         need += all;
-        if (i < n) first[i] = rank;
-        scan_before(excess, all, sums);
+        if (i < n) first[i] = (int32_t)rank;  // read only where all ranks fit the pool
+        scan_before(excess, all, wide);
         over += all;
     }
-    int32_t lack = over;
+    int64_t lack = over;
     if (!lack) {
         const int32_t most = (int32_t)(need < p.num_pages ? need : p.num_pages);
         lack = need - lowest_free(p.count, p.num_pages, most, fresh, sums);
     }
-    if (threadIdx.x == 0) missing[0] = lack;
+    if (threadIdx.x == 0) missing[0] = (int32_t)(lack < 0x7fffffff ? lack : 0x7fffffff);
     __syncthreads();
     if (!lack) {
         for (int32_t r = threadIdx.x; r < need; r += kPlan) {
@@ -317,7 +319,7 @@ __global__ __launch_bounds__(kPlan) void extend_plan(PoolArgs p, const int32_t* 
         }
         __syncthreads();
         for (int64_t i = threadIdx.x; i < n; i += kPlan)
-            if (seqs[i] >= 0 && seqs[i] < p.max_seqs) p.lens[seqs[i]] = length_of(p, seqs[i]) + grown_by(cu, i);
+            if (seqs[i] >= 0 && seqs[i] < p.max_seqs) p.lens[seqs[i]] = (int32_t)(length_of(p, seqs[i]) + grown_by(cu, i));
         __syncthreads();
     }
     if (total <= kPlan && (int64_t)threadIdx.x < total)

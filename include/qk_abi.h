@@ -535,7 +535,7 @@ int qk_kv_free(int64_t num_pages, int64_t page_size, int32_t* block_table, int64
 /* npu_kv_extend: sequence seqs[i] (none twice) grows by cu_tokens[i + 1] - cu_tokens[i] tokens.  Pages are allocated in
  * the order of i; slots[t] and positions[t], t < total, are the cache slot and the position of each new token (-1
  * past cu_tokens[n], and for a sequence number that is passed over).  missing[0] = how many free pages, or table columns,
- * are missing: 0, or slots and positions are -1 and nothing else is written.  Workspace: see the query. */
+ * are missing (at most 2^31 - 1): 0, or slots and positions are -1 and nothing else is written.  Workspace: see the query. */
 int qk_kv_extend_workspace_size(int64_t n, int64_t num_pages, size_t* bytes);
 int qk_kv_extend(int64_t num_pages, int64_t page_size, int32_t* block_table, int64_t max_seqs, int64_t table_width,
                  int64_t table_stride, int32_t* context_lens, int32_t* ref_count, const int32_t* seqs,
