@@ -345,8 +345,8 @@ __global__ __launch_bounds__(kThreads, KS <= 4 ? 3 : KS <= 6 ? 2 : 1) void atten
             }
             const float top = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])),
                                     fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
-            if (__builtin_amdgcn_ballot_w64(top > m + kSlack)) {
-                const float m2 = fmaxf(m, quad_max(top));
+            if (__builtin_amdgcn_ballot_w64(top > m + (kBelow<PV> + kSlack))) {
+                const float m2 = fmaxf(m, quad_max(top) - kBelow<PV>);
                 const float keep = __builtin_amdgcn_exp2f(m - m2);
                 m = m2;
                 l *= keep;

@@ -420,8 +420,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         };
         // Moves the maximum where a score lies far above it; `top` is a lane's largest score (a NaN does not matter).
         auto raise = [&](float top) INLINE {
-            if (__builtin_expect(__builtin_amdgcn_ballot_w64(top * factor > m + kSlack) != 0, 0)) {
-                const float m2 = fmaxf(m, pair_max(top * factor));
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(top * factor > m + (kBelow<PV> + kSlack)) != 0, 0)) {
+                const float m2 = fmaxf(m, pair_max(top * factor) - kBelow<PV>);
                 const float keep = __builtin_amdgcn_exp2f(m - m2);
                 m = m2;
                 l *= keep;
