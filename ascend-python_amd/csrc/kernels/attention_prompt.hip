@@ -20,7 +20,8 @@
 // tokens 10 us.
 //
 // A masked weight is 0, but 0 times a NaN or an infinity in V is NaN: tiles that are masked for some rows look for such
-// values once they are staged, and the values are added apart, for the rows that see them.
+// values once they are staged, and the values are added apart, for the rows that see them, with the weight that the products
+// would take: an infinity whose weight rounds to 0 gives NaN in every tile.
 #include <type_traits>
 
 #include "attention_device.h"
@@ -616,7 +617,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) w = own == 32 * n + 8 * (e >> 2) + (e & 3) ? x[n][e] : w;
-                    w = pair_sum(w);
+                    w = load_half_bits(pack2<DT>(pair_sum(w), 0.0f) & 0xffffu, DT);  // as the products round it
                     const bool sees = pair_max(own >= 0 && !(own & 4) && (mine >> (own & 63) & 1) ? 1.0f : 0.0f) != 0.0f;
                     const Global row = (Global)(uintptr_t)info[it & 7][key][1];
 #pragma unroll
