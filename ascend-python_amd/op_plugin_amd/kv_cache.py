@@ -65,5 +65,8 @@ class PagedKVCache:
 
     def compact(self) -> torch.Tensor:
         """Moves the pages in use to the front of the pool; how many moved, on the device."""
-        self.block_table, self.ref_count, moved = npu_kv_compact(self._pools(), self.block_table, self.ref_count)
+        table, count, moved = npu_kv_compact(self._pools(), self.block_table, self.ref_count)
+        # into the tensors that captured graphs and other holders of the state read
+        self.block_table.copy_(table)
+        self.ref_count.copy_(count)
         return moved

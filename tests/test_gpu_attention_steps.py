@@ -81,3 +81,43 @@ def test_rows_taken_once(mods, one_each, monkeypatch):
         got = b.att.quant_attention(x, b.gamma, b.w_qkv, b.s_qkv, b.w_o, b.s_o, b.cache, layer, seqs, None if one_each else cu,
                                     slots, positions, b.cos_sin, HQ, rows=rows)
         assert torch.equal(got, want[layer])
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.int8])
+def test_graph_of_a_step_across_compact(mods, kind):
+    """A decode step captured before a compaction works on the compacted cache: the same bits as eager steps, every time."""
+    print(f"[case] graph across compact {kind}", flush=True)
+    a, b = Model(mods, kind), Model(mods, kind)  # a: eager; b: the captured step
+    seqs, cu, x = _ints([0, 3, 5]), _ints([0, 1, 2, 3]), a.input(3)
+    first = a.input(90)
+    for m in (a, b):
+        m.step(first, _ints([0, 1, 3, 5]), _ints([0, 20, 57, 60, 90]))
+        m.step(x, seqs, cu, one_each=True)  # the libraries' and the allocator's first use, outside the capture
+    held = [t.data_ptr() for t in (b.cache.block_table, b.cache.context_lens, b.cache.ref_count)]
+    graph, given = torch.cuda.CUDAGraph(), x.clone()
+    with torch.cuda.graph(graph):
+        got, missing = b.step(given, seqs, cu, one_each=True)
+    torch.cuda.synchronize()
+
+    def same(what):
+        xs = a.input(3)
+        given.copy_(xs)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, _ = a.step(xs, seqs, cu, one_each=True)
+        assert int(missing) == 0 and all(torch.equal(w, g) for w, g in zip(want, got)), what
+        for s, t in ((a.cache.block_table, b.cache.block_table), (a.cache.context_lens, b.cache.context_lens),
+                     (a.cache.ref_count, b.cache.ref_count)):
+            assert torch.equal(s, t), what
+
+    same("before")
+    for m in (a, b):
+        m.cache.free(_ints([1]))
+        assert int(m.cache.compact()) > 0
+    assert held == [t.data_ptr() for t in (b.cache.block_table, b.cache.context_lens, b.cache.ref_count)]
+    used = int((b.cache.ref_count > 0).sum())
+    assert (b.cache.ref_count[:used] > 0).all() and int(b.cache.block_table.max()) < used
+    for i in range(20):  # past the pages' ends: new ones are taken from behind those that moved
+        same(f"after, step {i}")
+        garbage = [torch.full_like(b.cache.block_table, 10 ** 6) for _ in range(4)]  # what an old table's memory may become
+        del garbage
