@@ -144,7 +144,8 @@ void check_query(const char* op, const at::Tensor& q, const qk_kv_cache* c) {
 
 double scale_or_default(const char* op, std::optional<double> scale, int64_t head_dim) {
     const double s = scale.value_or(1.0 / std::sqrt((double)head_dim));
-    TORCH_CHECK(std::isfinite(s), op, ": scale must be finite, got ", s);
+    // the kernels hold it, times log2 e, in 32 bits
+    TORCH_CHECK(std::isfinite((float)s * (float)M_LOG2E), op, ": scale must be finite, and at most 2.3e38, got ", s);
     return s;
 }
 

@@ -1,5 +1,6 @@
 // extern "C" entry points of the attention and cache functions (declared in include/qk_abi.h): the checks of their plain
 // arguments, and the kernels' launches on the caller's stream.  Nothing here allocates or synchronises.
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 
@@ -113,6 +114,12 @@ int check_query(const char* op, const void* query, int64_t token_stride, int64_t
     return QK_OK;
 }
 
+// The kernels hold the scale times log2 e.
+int check_scale(const char* op, float scale) {
+    if (!std::isfinite(scale * (float)M_LOG2E)) return fail(QK_ERR_ARG, "%s: scale must be finite, and at most 2.3e38 (got %g)", op, scale);
+    return QK_OK;
+}
+
 qk::AttnArgs attention_args(const void* query, int dtype, int64_t tokens, int64_t batch, int64_t q_heads,
                             int64_t q_token_stride, int64_t q_head_stride, const qk_kv_cache* cache,
                             const int32_t* table, int64_t table_width, int64_t table_stride, const int32_t* lens,
@@ -198,6 +205,7 @@ int qk_paged_attention(const void* query, int dtype, int64_t batch, int64_t q_he
     if (int rc = check_attention_sizes(op, batch, batch, q_heads, cache, dtype, table_width, window, sinks)) return rc;
     if (batch == 0) return QK_OK;
     if (int rc = check_query(op, query, q_token_stride, q_head_stride, out)) return rc;
+    if (int rc = check_scale(op, scale)) return rc;
     if (cache->num_pages > 0)
         if (int rc = check_cache_data(op, cache)) return rc;
     if (!context_lens || (table_width > 0 && !block_table)) return fail(QK_ERR_ARG, "%s: null pointer", op);
@@ -235,6 +243,7 @@ int qk_prompt_attention(const void* query, int dtype, int64_t tokens, int64_t ba
     if (int rc = check_attention_sizes(op, tokens, batch, q_heads, cache, dtype, table_width, window, sinks)) return rc;
     if (tokens == 0) return QK_OK;
     if (int rc = check_query(op, query, q_token_stride, q_head_stride, out)) return rc;
+    if (int rc = check_scale(op, scale)) return rc;
     if (!cu_seqlens_q) return fail(QK_ERR_ARG, "%s: null pointer", op);
     if (batch == 0) return fail(QK_ERR_ARG, "%s: rows without a sequence", op);
     static const int32_t no_table = 0;

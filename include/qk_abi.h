@@ -442,10 +442,10 @@ typedef struct qk_kv_cache {
  * newest included, token j in slot j % page_size of page block_table[b * table_stride + j / page_size].  The query
  * stands at the last of them, p, and sees the keys j <= p with p - j < window (window 0: all) or j < sinks.
  *   s_j = scale * q . k_j,  out = sum exp(s_j - m) v_j / sum exp(s_j - m),  lse = m + ln sum exp(s_j - m)
- * in fp32, m the largest s_j; out: [batch][q_heads][head_dim] of dtype, lse: [batch][q_heads] fp32 or NULL.  A sequence
- * without a visible key (length 0) gives out = 0 and lse = -inf.  Lengths are cut to table_width * page_size; a token
- * whose page id is outside [0, num_pages) is not seen.  Workspace: partial results where the keys of a sequence are
- * split over workgroups.
+ * in fp32, m the largest s_j, scale finite and at most 2.3e38; out: [batch][q_heads][head_dim] of dtype, lse:
+ * [batch][q_heads] fp32 or NULL.  A sequence without a visible key (length 0) gives out = 0 and lse = -inf.  Lengths are
+ * cut to table_width * page_size; a token whose page id is outside [0, num_pages) is not seen.  Workspace: partial
+ * results where the keys of a sequence are split over workgroups.
  */
 int qk_paged_attention_workspace_size(int64_t batch, int64_t q_heads, const qk_kv_cache* cache, int64_t table_width,
                                       int64_t window, int64_t sinks, size_t* bytes);
