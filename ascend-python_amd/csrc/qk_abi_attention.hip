@@ -308,7 +308,7 @@ int qk_mrope(const void* query, const void* key, const void* value, int dtype, i
     const int64_t strides[] = {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride};
     for (int64_t s : strides)
         if (s < 0) return fail(QK_ERR_ARG, "%s: negative stride", op);
-    if ((q_heads > 0 && (!query || !out_query)) || (kv_heads > 0 && (!key || (!out_key && !cache))) || !positions || !cos_sin)
+    if ((q_heads > 0 && !query) || (kv_heads > 0 && !key) || !positions || !cos_sin)
         return fail(QK_ERR_ARG, "%s: null pointer", op);
     if (cache && cache->num_pages > 0) {
         if (!slots) return fail(QK_ERR_ARG, "%s: null pointer", op);
