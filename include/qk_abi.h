@@ -518,8 +518,8 @@ int qk_kv_copy_pages(const qk_pages* pages, int64_t tensors, int64_t num_pages, 
 /* npu_kv_fork: sequence children[i] becomes a copy of parents[i].  Whole pages are shared (count + 1); a last page that
  * is not full goes to a new page (count 1), whose bytes are copied in each of the tensors, so no writable page is
  * shared.  A child's former pages are not released (qk_kv_free does that before); no child may be a parent or occur
- * twice.  missing[0] = how many free pages are missing: 0, or nothing but missing[0] is written.  Workspace: n + 1 int32
- * pairs. */
+ * twice.  missing[0] = how many free pages are missing: 0, or nothing but missing[0] is written.  Workspace: see the
+ * query. */
 int qk_kv_fork_workspace_size(int64_t n, size_t* bytes);
 int qk_kv_fork(const qk_pages* pages, int64_t tensors, int64_t num_pages, int64_t page_size, int32_t* block_table,
                int64_t max_seqs, int64_t table_width, int64_t table_stride, int32_t* context_lens, int32_t* ref_count,

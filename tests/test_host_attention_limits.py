@@ -48,3 +48,13 @@ def test_scales_that_it_can(scale):
     k, v = _cache()
     q.npu_paged_attention(_m((3, 8, 64)), k, v, _m((3, 5), I32), _m((3,), I32), scale=scale)
     q.npu_prompt_attention(_m((30, 8, 64)), _m((30, 2, 64)), _m((30, 2, 64)), _m((4,), I32), scale=scale)
+
+
+@pytest.mark.parametrize("n", [0, 1, 2, 1000])
+def test_fork_workspace(n):
+    """A byte less than the query says is refused (checked before any launch)."""
+    L, fake, size = q.abi(), ctypes.c_void_p(4096), ctypes.c_size_t(0)
+    assert L.qk_kv_fork_workspace_size(n, ctypes.byref(size)) == q.QK_OK
+    assert size.value == 4 * (3 * n + 1)  # sources, destinations, the new pages, and whether there are enough
+    assert L.qk_kv_fork(None, 0, 5, 16, fake, 4, 8, 8, fake, fake, fake, fake, n, fake, fake, size.value - 1,
+                        None) == q.QK_ERR_WORKSPACE and str(size.value) in q.last_error()
