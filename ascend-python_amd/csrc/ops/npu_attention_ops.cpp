@@ -11,6 +11,7 @@
 #include <torch/library.h>
 
 #include <cmath>
+#include <limits>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -133,6 +134,24 @@ void cache_data(qk_kv_cache& c, const at::Tensor& key, const at::Tensor& value, 
     c.value_scale = value_scale.has_value() ? const_cast<float*>(value_scale->const_data_ptr<float>()) : nullptr;
 }
 
+// What the C ABI refuses of a cache, for Meta calls, which do not reach it.  paged: read or written where it lies (contiguous
+// keys are copied where their rows are not whole pieces).
+void check_cache_limits(const char* op, const qk_kv_cache& c, const at::Tensor& key, const at::Tensor& value, bool paged) {
+    const int64_t piece = c.dtype == QK_I8 ? 16 : 8, int31 = std::numeric_limits<int32_t>::max();
+    TORCH_CHECK(c.head_dim > 0 && c.head_dim <= 256 && c.head_dim % piece == 0, op, ": head_dim must be a multiple of ", piece,
+                " up to 256 (got ", c.head_dim, ")");
+    TORCH_CHECK(c.kv_heads > 0 && c.kv_heads <= 65535, op, ": need kv_heads in 1..65535 (got ", c.kv_heads, ")");
+    TORCH_CHECK(c.page_size <= int31 && c.num_pages <= int31 / c.page_size, op, ": a cache of ", c.num_pages, " pages of ",
+                c.page_size, " tokens has slots past 31 bits");
+    if (!paged || c.num_pages == 0) return;
+    for (const at::Tensor* t : {&key, &value}) {
+        for (int64_t d = 0; d + 1 < t->dim(); ++d)
+            TORCH_CHECK(stride_of(*t, d) * t->element_size() % 16 == 0, op,
+                        ": the cache's strides must be multiples of 16 bytes (got ", stride_of(*t, d) * t->element_size(), ")");
+        TORCH_CHECK(t->storage_offset() * t->element_size() % 16 == 0, op, ": the cache must be 16-byte aligned");
+    }
+}
+
 void check_query(const char* op, const at::Tensor& q, const qk_kv_cache* c) {
     TORCH_CHECK(is_half(q), op, ": query must be float16 or bfloat16, got ", q.scalar_type());
     TORCH_CHECK(q.dim() == 3, op, ": query must be [tokens, heads, head_dim], got ", q.sizes());
@@ -211,6 +230,9 @@ std::tuple<at::Tensor, at::Tensor> npu_paged_attention_meta(const at::Tensor& qu
     const qk_kv_cache c = paged_attention_check(op, query, key_cache, value_cache, block_table, context_lens, key_scale,
                                                 value_scale, window, sinks);
     scale_or_default(op, scale, c.head_dim);
+    check_cache_limits(op, c, key_cache, value_cache, true);
+    size_t ws_bytes = 0;  // the query looks at the sizes as the launch does
+    check_rc(qk_paged_attention_workspace_size(query.size(0), query.size(1), &c, block_table.size(1), window, sinks, &ws_bytes), op);
     return attention_outputs(query);
 }
 
@@ -290,10 +312,17 @@ std::tuple<at::Tensor, at::Tensor> npu_prompt_attention_meta(const at::Tensor& q
                                                              int64_t window, int64_t sinks) {
     const char* op = "npu_prompt_attention";
     const bool paged = block_table.has_value();
-    const auto fit = [&](const at::Tensor& t) { return paged || last_is_dense(t) ? t : t.contiguous(); };
+    const auto fit = [&](const at::Tensor& t) { return paged || t.dim() != 3 || last_is_dense(t) ? t : t.contiguous(); };
     const qk_kv_cache c = prompt_attention_check(op, query, fit(key), fit(value), cu_seqlens_q, cu_seqlens_k, block_table,
                                                  context_lens, key_scale, value_scale, window, sinks);
     scale_or_default(op, scale, c.head_dim);
+    if (query.size(0) > 0) {
+        check_cache_limits(op, c, key, value, paged);
+        size_t ws_bytes = 0;
+        check_rc(qk_prompt_attention_workspace_size(query.size(0), cu_seqlens_q.size(0) - 1, query.size(1), &c,
+                                                    paged ? block_table->size(1) : 0, window, sinks, &ws_bytes),
+                 op);
+    }
     return attention_outputs(query);
 }
 
@@ -343,6 +372,12 @@ Mrope mrope_check(const char* op, const at::Tensor& positions, const at::Tensor&
     return m;
 }
 
+// What the C ABI refuses of the heads, for Meta calls.
+void check_mrope_limits(const char* op, const at::Tensor& q, const at::Tensor& k) {
+    TORCH_CHECK(q.size(2) <= 256, op, ": head_dim must be 1..256 (got ", q.size(2), ")");
+    TORCH_CHECK(q.size(1) <= 65535 && k.size(1) <= 65535, op, ": invalid size q_heads=", q.size(1), " kv_heads=", k.size(1));
+}
+
 void mrope_launch(const char* op, const Mrope& m, const at::Tensor& positions_in, const at::Tensor& q_in,
                   const at::Tensor& k_in, const at::Tensor* v_in, const at::Tensor& cos_sin_in, const at::Tensor& out_q,
                   const at::Tensor* out_k, const qk_kv_cache* c, const int32_t* slots) {
@@ -375,6 +410,7 @@ std::tuple<at::Tensor, at::Tensor> npu_mrope_meta(const at::Tensor& positions, c
                                                   const at::Tensor& key, const at::Tensor& cos_sin_cache,
                                                   at::OptionalIntArrayRef mrope_section, c10::string_view rotary_mode) {
     mrope_check("npu_mrope", positions, query, key, cos_sin_cache, mrope_section, rotary_mode);
+    if (query.size(0) > 0) check_mrope_limits("npu_mrope", query, key);
     return {at::empty(query.sizes(), query.options()), at::empty(key.sizes(), key.options())};
 }
 
@@ -416,7 +452,11 @@ at::Tensor npu_mrope_scatter_kv_meta(const at::Tensor& positions, const at::Tens
                                      at::OptionalIntArrayRef mrope_section, c10::string_view rotary_mode) {
     const char* op = "npu_mrope_scatter_kv";
     mrope_check(op, positions, query, key, cos_sin_cache, mrope_section, rotary_mode);
-    scatter_check(op, query, key, value, key_cache, value_cache, slot_mapping, key_scale, value_scale);
+    const qk_kv_cache c = scatter_check(op, query, key, value, key_cache, value_cache, slot_mapping, key_scale, value_scale);
+    if (query.size(0) > 0) {
+        check_mrope_limits(op, query, key);
+        check_cache_limits(op, c, key_cache, value_cache, true);
+    }
     return at::empty(query.sizes(), query.options());
 }
 
@@ -454,6 +494,15 @@ std::vector<qk_pages> page_list(const char* op, at::TensorList caches, int64_t n
         list.push_back({t.is_meta() ? nullptr : t.data_ptr(), num_pages == 1 ? bytes : t.stride(0) * t.element_size(), bytes});
     }
     return list;
+}
+
+void check_seqs(const char* op, const at::Tensor& seqs) {
+    TORCH_CHECK(seqs.numel() <= QK_MAX_SEQS, op, ": ", seqs.numel(), " sequences (at most ", QK_MAX_SEQS, " a call)");
+}
+
+void check_slots(const char* op, const at::Tensor& table, const at::Tensor& count, int64_t page_size) {
+    const int64_t most = std::numeric_limits<int32_t>::max() / page_size;
+    TORCH_CHECK(count.size(0) <= most && table.size(1) <= most, op, ": sizes past 31 bits");
 }
 
 void check_pool(const char* op, const at::Tensor& table, const at::Tensor& lens, const at::Tensor& count) {
@@ -502,6 +551,8 @@ void fork_check(const char* op, const at::Tensor& table, const at::Tensor& lens,
     TORCH_CHECK(parents.sizes() == children.sizes(), op, ": parents and children must have one length, got ",
                 parents.sizes(), " and ", children.sizes());
     TORCH_CHECK(page_size > 0, op, ": page_size must be positive, got ", page_size);
+    check_seqs(op, parents);
+    check_slots(op, table, count, page_size);
 }
 
 at::Tensor npu_kv_fork(at::TensorList caches, const at::Tensor& table, const at::Tensor& lens, const at::Tensor& count,
@@ -535,6 +586,8 @@ void free_check(const char* op, const at::Tensor& table, const at::Tensor& lens,
     check_pool(op, table, lens, count);
     check_index(op, "seqs", seqs, 1, table);
     TORCH_CHECK(page_size > 0, op, ": page_size must be positive, got ", page_size);
+    check_seqs(op, seqs);
+    check_slots(op, table, count, page_size);
 }
 
 void npu_kv_free(const at::Tensor& table, const at::Tensor& lens, const at::Tensor& count, const at::Tensor& seqs_in,
@@ -560,6 +613,7 @@ void extend_check(const char* op, const at::Tensor& table, const at::Tensor& len
     TORCH_CHECK(cu.size(0) == seqs.size(0) + 1, op, ": cu_tokens must have one value more than seqs, got ", cu.sizes(),
                 " and ", seqs.sizes());
     TORCH_CHECK(total >= 0, op, ": total_tokens must not be negative, got ", total);
+    TORCH_CHECK(total <= std::numeric_limits<int32_t>::max(), op, ": invalid number of tokens ", total);
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> npu_kv_extend(const at::Tensor& table, const at::Tensor& lens,
@@ -592,6 +646,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> npu_kv_extend_meta(const at::Tens
 void compact_check(const char* op, const at::Tensor& table, const at::Tensor& count) {
     check_index(op, "block_table", table, 2, table);
     check_index(op, "ref_count", count, 1, table);
+    check_slots(op, table, count, 1);
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> npu_kv_compact(at::TensorList caches, const at::Tensor& table_in,
