@@ -28,8 +28,9 @@ class PagedKVCache:
         self.keys = [torch.empty(shape, dtype=dtype, device=device) for _ in range(layers)]
         self.values = [torch.empty(shape, dtype=dtype, device=device) for _ in range(layers)]
         quant = dtype == torch.int8
-        self.key_scales = [torch.empty(shape[:3], device=device) if quant else None for _ in range(layers)]
-        self.value_scales = [torch.empty(shape[:3], device=device) if quant else None for _ in range(layers)]
+        scales = lambda: torch.empty(shape[:3], dtype=torch.float32, device=device) if quant else None  # noqa: E731
+        self.key_scales = [scales() for _ in range(layers)]
+        self.value_scales = [scales() for _ in range(layers)]
         width = -(-max_len // page_size)
         self.block_table = torch.full((max_seqs, width), -1, dtype=torch.int32, device=device)
         self.context_lens = torch.zeros(max_seqs, dtype=torch.int32, device=device)
