@@ -9,7 +9,8 @@ namespace qk {
 void abi_begin();
 int abi_error(int code, const char* message);
 
-// q = j / d for 0 <= j < 2^31 and a divisor fixed per launch (a page's size): (j * m) >> s with m = ceil(2^s / d),
+// q = j / d for 0 <= j < 2^31 and a divisor fixed per launch (a page's size), by multiplication (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994): (j * m) >> s with m = ceil(2^s / d),
 // s = 31 + ceil(log2 d).  The error of m, below d, adds j * d / (d * 2^s) < 1 / d to the quotient, too little to reach the
 // next whole number; m < 2^32 as d > 2^(s - 32).
 struct Div31 {

@@ -18,7 +18,7 @@
 // maximum is that of score plus log2 value_scale, so that the weights with their scales stay in fp16's range.
 //
 // Measured on one MI355X, inputs that change: 4 x 131072 keys under 64 heads on 8 (2.1 GB) 402 us, 5.3 TB/s; 48 sequences up to
-// 8191 (227 MB) 63 us, 3.6 TB/s; 96 on an int8 cache with a window of 4096 (159 MB) 51 us; 997 keys of one sequence 12 us.
+// 8191 (227 MB) 63 us, 3.6 TB/s; 96 on an int8 cache with a window of 4096 (159 MB) 53 us; 997 keys of one sequence 12 us.
 #include "attention_device.h"
 
 namespace qk {

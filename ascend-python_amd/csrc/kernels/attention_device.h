@@ -11,10 +11,12 @@ constexpr float kLowest = -3.0e38f;
 // A running maximum stays until a score passes it by this much: weights reach 2^8, which neither 16-bit type nor the fp32
 // sums mind, and most tiles rescale nothing.
 constexpr float kSlack = 8.0f;
-// What weights are rounded to 16 bits for, the right operand of the second product's matrix instruction, costs float16 (DT:
-// their type) its small ones: below 2^-14 they lose bits and below 2^-25 all, while their sum keeps them, and 100000 of them
-// can be a share of the result that shows.  So the running "maximum" lies this far below the largest score there: weights
-// reach 2^(7 + 8), still finite, keep all their bits down to 2^-21 of the largest and are rounded to multiples of 2^-31 of it below.
+// Weights are rounded once to 16 bits, half a step each: the second product's matrix instruction takes operands of one 16-bit
+// type, and a second one for what the rounding leaves would be half as much matrix work again, for an error of the size that
+// V's own 16 bits have.  bf16 keeps its relative step whatever the weight; float16 (DT: the weights' type) loses bits below
+// 2^-14 and everything below 2^-25, while the weights' fp32 sum does not, and 100000 small weights can be a share of the
+// result that shows.  So the running "maximum" lies 7 below the largest score there: weights reach 2^(7 + 8), still finite,
+// keep all their bits down to 2^-21 of the largest, and are rounded to multiples of 2^-31 of it below that.
 template <int DT>
 constexpr float kBelow = DT == QK_F16 ? 7.0f : 0.0f;
 

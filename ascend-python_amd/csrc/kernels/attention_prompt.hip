@@ -15,9 +15,9 @@
 // The next tile's scores are made between the exponentials of this one, so that a wave keeps both pipes busy.  The running
 // maximum moves only where a score lies far above it: most tiles rescale nothing and need no exchange between lanes.
 //
-// Measured on one MI355X: 8192 tokens under 32 heads on 8 550 us, 1.0 PFLOP/s (on random data the card is held back by its power:
-// 500 us on zeros); 2048 tokens 56 us; 1023 tokens over 12000 with a window of 2048 57 us; 4 tokens over 12000 33 us; 77
-// tokens 10 us.
+// Measured on one MI355X: 8192 tokens under 32 heads on 8 540 us, 1.0 PFLOP/s (on random data the card is held back by its power:
+// 500 us on zeros); 2048 tokens 54 us; six chunks up to 1023 tokens over 12000 with a window of 2048 56 us; 4 tokens over
+// 12000 33 us; 77 tokens 10 us.
 //
 // A masked weight is 0, but 0 times a NaN or an infinity in V is NaN: tiles that are masked for some rows look for such
 // values once they are staged, and the values are added apart, for the rows that see them, with the weight that the products

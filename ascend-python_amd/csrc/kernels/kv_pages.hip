@@ -8,7 +8,7 @@
 //
 // What moves bytes is one kernel: items of (pair of pages, tensor, 16 KB piece) handed to workgroups in turn, four
 // 16-byte loads in flight per lane before the stores.  Bound by HBM: each byte is read and written once
-// (a pool of 1024 pages of 1 MB packed: 74 us, 4.5 TB/s; pieces of 32 KB, eight loads in flight: 97 us).
+// (a pool of 1024 pages of 1 MB packed: 75 us, 4.5 TB/s; pieces of 32 KB, eight loads in flight: 97 us).
 #include "attention.h"
 
 namespace qk {
