@@ -59,6 +59,16 @@ size_t attention_prompt_workspace(int64_t tokens, int64_t batch, int64_t q_heads
                                   int64_t window, int64_t sinks);
 hipError_t launch_attention_prompt(const AttnArgs& a, void* workspace, hipStream_t stream);
 
+// What the rows of trees see of their own tree: bit k of row t is bit k % 64 of words[t * stride + k / 64].
+struct TreeMask {
+    const uint64_t* words;
+    int64_t stride;
+    int32_t count;  // words of a row
+};
+// Ragged trees (cu_q != nullptr), keys in pages.
+size_t attention_tree_workspace(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache& c, int64_t table_width);
+hipError_t launch_attention_tree(const AttnArgs& a, const TreeMask& mask, void* workspace, hipStream_t stream);
+
 struct MropeArgs {
     const void *q, *k, *v;
     int dtype;

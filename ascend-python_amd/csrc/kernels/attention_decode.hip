@@ -65,17 +65,6 @@ __device__ __forceinline__ int64_t worker_of(int64_t total, int64_t workers, int
     return quotient((u + 1) * workers + total - 1, total) - 1;
 }
 
-// Sum over the lanes up to this one, by moves within rows of 16 lanes and from a row's last lane to those behind.
-__device__ __forceinline__ int32_t wave_scan(int32_t v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);
-    return v;
-}
-
 __device__ __forceinline__ int32_t length_of(const AttnArgs& a, int64_t b) {
     const int64_t most = a.kv.table_width * a.kv.c.page_size, n = a.kv.lens[b];
     return (int32_t)(n < 0 ? 0 : n > most ? most : n);

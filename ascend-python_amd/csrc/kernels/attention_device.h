@@ -89,6 +89,17 @@ __device__ __forceinline__ uint64_t uniform64(uint64_t v) {
     return (uint64_t)hi << 32 | lo;
 }
 
+// Sum over the lanes up to this one, by moves within rows of 16 lanes and from a row's last lane to those behind.
+__device__ __forceinline__ int32_t wave_scan(int32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);
+    return v;
+}
+
 // The keys that a position sees, without a gap: the first `sinks` of them, then those from `low` on.
 struct Seen {
     int32_t count, sinks, gap;

@@ -1,0 +1,66 @@
+// Trees of drafted tokens over a cache in pages: the kernel of attention_prompt.h, with rows that see the whole context and, of
+// their own tree, what their masks say.  A row's place among the keys plays no part but in a window, which is held against the
+// depth in the tree.
+//
+// Between a token and a prompt: n rows of a group of G query heads make 4 * head_dim * n * G operations for 4 * head_dim bytes of a key
+// and value, so small trees are bound by HBM and trees past some 190 / G rows by the matrix cores.  There are few tiles (a tree of 32 rows under a
+// group of four is one) over contexts of any length, so the keys of all tiles are cut into parts that fill the card once; the
+// lengths are on the device only, and every workgroup finds its part from them (tree_work).
+#include "attention_prompt.h"
+
+namespace qk {
+namespace {
+
+struct Plan {
+    int64_t grid, arrivals_bytes, part_bytes, parts, tiles;
+    int room;
+};
+
+Plan plan(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache& c, int64_t table_width) {
+    Plan p = {};
+    const int64_t some = batch < tokens ? batch : tokens;
+    // at most, of a key-value head: row tiles, and parts of a tile
+    const int64_t tiles = p.tiles = tokens * (q_heads / c.kv_heads) / kRows + some + 1;
+    const int64_t parts = table_width * c.page_size / kKeys / kTreeSteps + 1;
+    // cut tiles fill the card's places once; heads wider than 128 leave one workgroup per CU
+    const int64_t room = (c.head_dim <= 128 ? kResident : kResident / 2) / c.kv_heads;
+    p.room = room < 1 ? 1 : (int)room;
+    // How many tiles there are is known on the device only: tiles that are not cut, or parts that fill the room.  Workgroups without
+    // a part end at once.
+    const int64_t ranks = tiles > p.room ? tiles : tiles * parts < p.room ? tiles * parts : p.room;
+    p.grid = ranks * c.kv_heads;
+    if (p.room > 1 && parts > 1) {
+        p.parts = (ranks < p.room ? ranks : p.room) * c.kv_heads;
+        p.arrivals_bytes = (tiles * c.kv_heads * 8 + 255) / 256 * 256;
+        p.part_bytes = kRows * (padded_width(c) + 2) * 4;
+    }
+    return p;
+}
+
+}  // namespace
+
+size_t attention_tree_workspace(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache& c, int64_t table_width) {
+    if (tokens == 0) return 0;
+    const Plan p = plan(tokens, batch, q_heads, c, table_width);
+    return (size_t)(p.arrivals_bytes + p.parts * p.part_bytes);
+}
+
+hipError_t launch_attention_tree(const AttnArgs& a, const TreeMask& mask, void* workspace, hipStream_t stream) {
+    const Plan p = plan(a.tokens, a.batch, a.q_heads, a.kv.c, a.kv.table_width);
+    PromptArgs g = {};
+    g.a = a;
+    g.group_div = div31((uint32_t)(a.q_heads / a.kv.c.kv_heads));
+    g.splits = p.room;
+    g.mask = mask;
+    g.most_tiles = p.tiles;
+    if (p.parts > 0) {
+        g.tag = next_split_tag();
+        g.arrivals = (uint64_t*)workspace;
+        g.parts = (float*)((char*)workspace + p.arrivals_bytes);
+        g.part_bytes = p.part_bytes;
+    }
+    launch_form<true>(g, p.grid, stream);
+    return hipGetLastError();
+}
+
+}  // namespace qk

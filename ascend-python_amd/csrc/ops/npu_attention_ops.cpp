@@ -326,6 +326,70 @@ std::tuple<at::Tensor, at::Tensor> npu_prompt_attention_meta(const at::Tensor& q
     return attention_outputs(query);
 }
 
+// ---------------------------------------------------------------- npu_tree_attention
+
+qk_kv_cache tree_attention_check(const char* op, const at::Tensor& q, const at::Tensor& key, const at::Tensor& value,
+                                 const at::Tensor& cu_q, const at::Tensor& table, const at::Tensor& lens, const at::Tensor& mask,
+                                 const OptTensor& key_scale, const OptTensor& value_scale, int64_t window, int64_t sinks) {
+    qk_kv_cache c = prompt_attention_check(op, q, key, value, cu_q, std::nullopt, table, lens, key_scale, value_scale, window, sinks);
+    TORCH_CHECK(mask.scalar_type() == at::kLong && mask.dim() == 2 && mask.size(0) == q.size(0) && mask.size(1) >= 1, op,
+                ": tree_mask must be int64 [tokens, words] with a word at least, got ", mask.scalar_type(), " ", mask.sizes(),
+                " for ", q.size(0), " tokens");
+    TORCH_CHECK(mask.size(1) <= std::numeric_limits<int32_t>::max() / 64, op, ": masks of at most ",
+                std::numeric_limits<int32_t>::max() / 64, " words, got ", mask.size(1));
+    check_device(op, "tree_mask", mask, q);
+    return c;
+}
+
+std::tuple<at::Tensor, at::Tensor> npu_tree_attention(const at::Tensor& query, const at::Tensor& key_cache,
+                                                      const at::Tensor& value_cache, const at::Tensor& cu_seqlens_q,
+                                                      const at::Tensor& block_table, const at::Tensor& context_lens,
+                                                      const at::Tensor& tree_mask, const OptTensor& key_scale,
+                                                      const OptTensor& value_scale, std::optional<double> scale, int64_t window,
+                                                      int64_t sinks) {
+    const char* op = "npu_tree_attention";
+    qk_kv_cache c = tree_attention_check(op, query, key_cache, value_cache, cu_seqlens_q, block_table, context_lens, tree_mask,
+                                         key_scale, value_scale, window, sinks);
+    const double s = scale_or_default(op, scale, c.head_dim);
+    const c10::DeviceGuard guard(query.device());
+    const auto q = whole_rows(query);
+    const auto cu_q = cu_seqlens_q.contiguous(), table = dense_table(block_table), lens = context_lens.contiguous();
+    const auto mask = last_is_dense(tree_mask) ? tree_mask : tree_mask.contiguous();
+    cache_data(c, key_cache, value_cache, key_scale, value_scale);
+    auto [out, lse] = attention_outputs(q);
+    if (q.size(0) == 0) return {out, lse};
+    const int64_t width = table.size(1), batch = cu_q.size(0) - 1;
+    size_t ws_bytes = 0;
+    check_rc(qk_tree_attention_workspace_size(q.size(0), batch, q.size(1), &c, width, window, sinks, &ws_bytes), op);
+    const auto ws = workspace_for(q, ws_bytes);
+    check_rc(qk_tree_attention(q.const_data_ptr(), qk_dtype_of(q.scalar_type()), q.size(0), batch, q.size(1), stride_of(q, 0),
+                               stride_of(q, 1), index_data(cu_q), &c, index_data(table), width, stride_of(table, 0),
+                               index_data(lens), mask.const_data_ptr<int64_t>(), mask.size(1), stride_of(mask, 0), (float)s, window,
+                               sinks, out.data_ptr(), lse.data_ptr<float>(), ws.data_ptr(), ws_bytes, current_stream(q)),
+             op);
+    return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor> npu_tree_attention_meta(const at::Tensor& query, const at::Tensor& key_cache,
+                                                           const at::Tensor& value_cache, const at::Tensor& cu_seqlens_q,
+                                                           const at::Tensor& block_table, const at::Tensor& context_lens,
+                                                           const at::Tensor& tree_mask, const OptTensor& key_scale,
+                                                           const OptTensor& value_scale, std::optional<double> scale,
+                                                           int64_t window, int64_t sinks) {
+    const char* op = "npu_tree_attention";
+    const qk_kv_cache c = tree_attention_check(op, query, key_cache, value_cache, cu_seqlens_q, block_table, context_lens, tree_mask,
+                                               key_scale, value_scale, window, sinks);
+    scale_or_default(op, scale, c.head_dim);
+    if (query.size(0) > 0) {
+        check_cache_limits(op, c, key_cache, value_cache, true);
+        size_t ws_bytes = 0;
+        check_rc(qk_tree_attention_workspace_size(query.size(0), cu_seqlens_q.size(0) - 1, query.size(1), &c, block_table.size(1),
+                                                  window, sinks, &ws_bytes),
+                 op);
+    }
+    return attention_outputs(query);
+}
+
 // ---------------------------------------------------------------- npu_mrope, npu_mrope_scatter_kv
 
 struct Mrope {
@@ -685,6 +749,9 @@ TORCH_LIBRARY_FRAGMENT(npu, m) {
     m.def("npu_prompt_attention(Tensor query, Tensor key, Tensor value, Tensor cu_seqlens_q, *, Tensor? cu_seqlens_k=None, "
           "Tensor? block_table=None, Tensor? context_lens=None, Tensor? key_scale=None, Tensor? value_scale=None, "
           "float? scale=None, int window=0, int sinks=0) -> (Tensor, Tensor)");
+    m.def("npu_tree_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor cu_seqlens_q, Tensor block_table, "
+          "Tensor context_lens, Tensor tree_mask, *, Tensor? key_scale=None, Tensor? value_scale=None, float? scale=None, "
+          "int window=0, int sinks=0) -> (Tensor, Tensor)");
     m.def("npu_mrope(Tensor positions, Tensor query, Tensor key, Tensor cos_sin_cache, *, int[]? mrope_section=None, "
           "str rotary_mode='half') -> (Tensor, Tensor)");
     m.def("npu_mrope_scatter_kv(Tensor positions, Tensor query, Tensor key, Tensor value, Tensor cos_sin_cache, "
@@ -703,6 +770,7 @@ TORCH_LIBRARY_FRAGMENT(npu, m) {
 TORCH_LIBRARY_IMPL(npu, CUDA, m) {
     m.impl("npu_paged_attention", &npu_paged_attention);
     m.impl("npu_prompt_attention", &npu_prompt_attention);
+    m.impl("npu_tree_attention", &npu_tree_attention);
     m.impl("npu_mrope", &npu_mrope);
     m.impl("npu_mrope_scatter_kv", &npu_mrope_scatter_kv);
     m.impl("npu_kv_copy_pages", &npu_kv_copy_pages);
@@ -715,6 +783,7 @@ TORCH_LIBRARY_IMPL(npu, CUDA, m) {
 TORCH_LIBRARY_IMPL(npu, Meta, m) {
     m.impl("npu_paged_attention", &npu_paged_attention_meta);
     m.impl("npu_prompt_attention", &npu_prompt_attention_meta);
+    m.impl("npu_tree_attention", &npu_tree_attention_meta);
     m.impl("npu_mrope", &npu_mrope_meta);
     m.impl("npu_mrope_scatter_kv", &npu_mrope_scatter_kv_meta);
     m.impl("npu_kv_copy_pages", &npu_kv_copy_pages_meta);

@@ -269,6 +269,51 @@ int qk_prompt_attention(const void* query, int dtype, int64_t tokens, int64_t ba
     return launched(qk::launch_attention_prompt(a, workspace, (hipStream_t)stream), op);
 }
 
+int qk_tree_attention_workspace_size(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache* cache,
+                                     int64_t table_width, int64_t window, int64_t sinks, size_t* bytes) {
+    qk::abi_begin();
+    const char* op = "npu_tree_attention";
+    if (!bytes) return fail(QK_ERR_ARG, "%s: null pointer", op);
+    if (int rc = check_attention_sizes(op, tokens, batch, q_heads, cache, cache && cache->dtype != QK_I8 ? cache->dtype : QK_BF16,
+                                       table_width, window, sinks))
+        return rc;
+    *bytes = qk::attention_tree_workspace(tokens, batch, q_heads, *cache, table_width);
+    return QK_OK;
+}
+
+int qk_tree_attention(const void* query, int dtype, int64_t tokens, int64_t batch, int64_t q_heads, int64_t q_token_stride,
+                      int64_t q_head_stride, const int32_t* cu_seqlens_q, const qk_kv_cache* cache, const int32_t* block_table,
+                      int64_t table_width, int64_t table_stride, const int32_t* context_lens, const int64_t* tree_mask,
+                      int64_t mask_words, int64_t mask_stride, float scale, int64_t window, int64_t sinks, void* out, float* lse,
+                      void* workspace, size_t workspace_bytes, qk_stream_t stream) {
+    qk::abi_begin();
+    const char* op = "npu_tree_attention";
+    if (int rc = check_attention_sizes(op, tokens, batch, q_heads, cache, dtype, table_width, window, sinks)) return rc;
+    if (tokens == 0) return QK_OK;
+    if (int rc = check_query(op, query, q_token_stride, q_head_stride, out)) return rc;
+    if (int rc = check_scale(op, scale)) return rc;
+    if (!cu_seqlens_q || !tree_mask) return fail(QK_ERR_ARG, "%s: null pointer", op);
+    if (batch == 0) return fail(QK_ERR_ARG, "%s: rows without a sequence", op);
+    if (mask_words < 1 || mask_words > kInt31 / 64 || mask_stride < 0)
+        return fail(QK_ERR_ARG, "%s: masks of 1 to %lld words, a stride not negative (got %lld and %lld)", op, (long long)kInt31 / 64,
+                    (long long)mask_words, (long long)mask_stride);
+    if ((uintptr_t)tree_mask % 8 != 0) return fail(QK_ERR_ARG, "%s: tree_mask must be 8-byte aligned", op);
+    if (!context_lens || (table_width > 0 && !block_table)) return fail(QK_ERR_ARG, "%s: null pointer", op);
+    if (table_stride < 0) return fail(QK_ERR_ARG, "%s: negative stride of the table", op);
+    if (cache->num_pages > 0)
+        if (int rc = check_cache_data(op, cache)) return rc;
+    static const int32_t no_table = 0;
+    qk::AttnArgs a = attention_args(query, dtype, tokens, batch, q_heads, q_token_stride, q_head_stride, cache,
+                                    block_table ? block_table : &no_table, table_width, table_stride, context_lens, scale, window,
+                                    sinks, out, lse);
+    a.cu_q = cu_seqlens_q;
+    const qk::TreeMask mask = {(const uint64_t*)tree_mask, mask_stride, (int32_t)mask_words};
+    size_t need = 0;
+    if (int rc = qk_tree_attention_workspace_size(tokens, batch, q_heads, cache, table_width, window, sinks, &need)) return rc;
+    if (int rc = check_workspace(op, need, workspace, workspace_bytes)) return rc;
+    return launched(qk::launch_attention_tree(a, mask, workspace, (hipStream_t)stream), op);
+}
+
 int qk_mrope(const void* query, const void* key, const void* value, int dtype, int64_t tokens, int64_t q_heads,
              int64_t kv_heads, int64_t head_dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
              int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const int32_t* positions,

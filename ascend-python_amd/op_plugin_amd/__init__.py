@@ -33,7 +33,10 @@ Importing this package loads ``_npu_ops.so``, which registers
   value_scale=None, scale=None, window=0, sinks=0) -> (out, lse)`` (one new token per sequence),
   ``torch.ops.npu.npu_prompt_attention(query, key, value, cu_seqlens_q, *, cu_seqlens_k=None, block_table=None,
   context_lens=None, key_scale=None, value_scale=None, scale=None, window=0, sinks=0) -> (out, lse)`` (ragged prompts or
-  prompt chunks, causal, keys contiguous or paged)
+  prompt chunks, causal, keys contiguous or paged),
+  ``torch.ops.npu.npu_tree_attention(query, key_cache, value_cache, cu_seqlens_q, block_table, context_lens, tree_mask, *,
+  key_scale=None, value_scale=None, scale=None, window=0, sinks=0) -> (out, lse)`` (trees of drafted tokens: a row sees the
+  context and the rows of its own tree whose bits its mask [tokens, words] int64 has set)
 * ``torch.ops.npu.npu_mrope(positions, query, key, cos_sin_cache, *, mrope_section=None, rotary_mode="half") -> (query,
   key)`` and ``torch.ops.npu.npu_mrope_scatter_kv(positions, query, key, value, cos_sin_cache, key_cache, value_cache,
   slot_mapping, *, key_scale=None, value_scale=None, mrope_section=None, rotary_mode="half") -> query``: rotary
@@ -84,6 +87,7 @@ npu_quant_matmul_swiglu = torch.ops.npu.npu_quant_matmul_swiglu
 npu_quant_matmul_swiglu_quant = torch.ops.npu.npu_quant_matmul_swiglu_quant
 npu_paged_attention = torch.ops.npu.npu_paged_attention
 npu_prompt_attention = torch.ops.npu.npu_prompt_attention
+npu_tree_attention = torch.ops.npu.npu_tree_attention
 npu_mrope = torch.ops.npu.npu_mrope
 npu_mrope_scatter_kv = torch.ops.npu.npu_mrope_scatter_kv
 npu_kv_copy_pages = torch.ops.npu.npu_kv_copy_pages
@@ -105,7 +109,8 @@ ABI_SYMBOLS = (
     "qk_quantize_per_tensor", "qk_quantize_per_channel", "qk_dequantize", "qk_rms_norm", "qk_rms_norm_quant",
     "qk_swiglu", "qk_swiglu_quant", "qk_quant_matmul_swiglu", "qk_quant_matmul_swiglu_quant_workspace_size",
     "qk_quant_matmul_swiglu_quant", "qk_paged_attention_workspace_size", "qk_paged_attention",
-    "qk_prompt_attention_workspace_size", "qk_prompt_attention", "qk_mrope", "qk_kv_copy_pages",
+    "qk_prompt_attention_workspace_size", "qk_prompt_attention", "qk_tree_attention_workspace_size", "qk_tree_attention",
+    "qk_mrope", "qk_kv_copy_pages",
     "qk_kv_fork_workspace_size", "qk_kv_fork", "qk_kv_free", "qk_kv_extend_workspace_size", "qk_kv_extend",
     "qk_kv_compact_workspace_size", "qk_kv_compact",
 )
@@ -167,6 +172,9 @@ def abi() -> ctypes.CDLL:
         L.qk_prompt_attention_workspace_size.argtypes = [I64, I64, I64, C, I64, I64, I64, Z]
         L.qk_prompt_attention.argtypes = [P, I, I64, I64, I64, I64, I64, P, C, P, P, I64, I64, P, F, I64, I64, P, P, P,
                                           SZ, P]
+        L.qk_tree_attention_workspace_size.argtypes = [I64, I64, I64, C, I64, I64, I64, Z]
+        L.qk_tree_attention.argtypes = [P, I, I64, I64, I64, I64, I64, P, C, P, I64, I64, P, P, I64, I64, F, I64, I64, P, P,
+                                        P, SZ, P]
         L.qk_mrope.argtypes = [P, P, P, I] + [I64] * 10 + [P, I64, I64, P, P, I, I64, I64, I, P, P, C, P, P]
         L.qk_kv_copy_pages.argtypes = [G, I64, I64, P, P, I64, P]
         L.qk_kv_fork_workspace_size.argtypes = [I64, Z]
@@ -208,6 +216,6 @@ __all__ = [
     "npu_convert_weight_to_int4pack", "npu_format_cast", "get_npu_format", "quantize_per_tensor",
     "quantize_per_channel", "dequantize", "npu_rms_norm", "npu_swiglu", "npu_rms_norm_dynamic_quant",
     "npu_swiglu_dynamic_quant", "npu_quant_matmul_swiglu", "npu_quant_matmul_swiglu_quant", "npu_paged_attention",
-    "npu_prompt_attention", "npu_mrope", "npu_mrope_scatter_kv", "npu_kv_copy_pages", "npu_kv_fork", "npu_kv_free",
+    "npu_prompt_attention", "npu_tree_attention", "npu_mrope", "npu_mrope_scatter_kv", "npu_kv_copy_pages", "npu_kv_fork", "npu_kv_free",
     "npu_kv_extend", "npu_kv_compact", "abi", "last_error", "debug_set_plan", "LIB_PATH", "OPS_PATH",
 ]

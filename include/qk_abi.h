@@ -475,6 +475,25 @@ int qk_prompt_attention(const void* query, int dtype, int64_t tokens, int64_t ba
                         qk_stream_t stream);
 
 /*
+ * npu_tree_attention -- attention of drafted tokens, a tree of them per sequence, over its pages (decoding with drafts: a
+ * third phase between the two of the reference's fused attention, several rows of which no two need see each other).
+ * query: [tokens][q_heads][head_dim], sequence b's rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] as above.  Sequence b holds
+ * context_lens[b] tokens in pages, the last n of them the rows' own, n being their number; before them x =
+ * context_lens[b] - n.  Row t sees the keys j < x, and key x + k for every k < n whose bit, k % 64 of
+ * tree_mask[t * mask_stride + k / 64], is set (itself only if its own bit is; past mask_words words there are none).  With
+ * a window it sees of the keys j < x those with p - j < window or j < sinks, p = x - 1 + the number of its bits set below n, so that
+ * a row whose bits are its ancestors and itself stands at its depth; the tree's own keys go by the mask alone.  Same formula, outputs and
+ * rules as qk_paged_attention; a row that sees no key, and a row past the last sequence, gives out = 0 and lse = -inf.
+ */
+int qk_tree_attention_workspace_size(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache* cache,
+                                     int64_t table_width, int64_t window, int64_t sinks, size_t* bytes);
+int qk_tree_attention(const void* query, int dtype, int64_t tokens, int64_t batch, int64_t q_heads, int64_t q_token_stride,
+                      int64_t q_head_stride, const int32_t* cu_seqlens_q, const qk_kv_cache* cache,
+                      const int32_t* block_table, int64_t table_width, int64_t table_stride, const int32_t* context_lens,
+                      const int64_t* tree_mask, int64_t mask_words, int64_t mask_stride, float scale, int64_t window,
+                      int64_t sinks, void* out, float* lse, void* workspace, size_t workspace_bytes, qk_stream_t stream);
+
+/*
  * npu_mrope, npu_mrope_scatter_kv -- rotary positions of one to four axes (time, height, width of an image's or a
  * video's tokens), alone or with the write of the new keys and values into the cache.  query: [tokens][q_heads]
  * [head_dim], key, value: [tokens][kv_heads][head_dim] of dtype (QK_F16 / QK_BF16) through strides in elements.
