@@ -707,6 +707,92 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> npu_kv_extend_meta(const at::Tens
     return {at::empty({total}, table.options()), at::empty({total}, table.options()), at::empty({1}, table.options())};
 }
 
+// A token's row in each cache tensor: its dimensions behind pages and tokens, as pieces of whole bytes that lie one apart.
+std::vector<qk_rows> row_list(const char* op, at::TensorList caches, int64_t num_pages, int64_t page_size, const at::Tensor& like) {
+    std::vector<qk_rows> list;
+    list.reserve(caches.size());
+    for (const at::Tensor& t : caches) {
+        TORCH_CHECK(t.dim() >= 2 && t.dim() <= 64 && t.size(0) == num_pages && t.size(1) == page_size, op,
+                    ": every cache tensor must be [", num_pages, ", ", page_size, ", ...], got ", t.sizes());
+        check_device(op, "a cache tensor", t, like);
+        if (t.numel() == 0) continue;
+        const int64_t size = t.element_size();
+        qk_rows r = {t.is_meta() ? nullptr : t.data_ptr(), stride_of(t, 0) * size, stride_of(t, 1) * size, 0, 1, size};
+        uint64_t done = 3;
+        for (int64_t left = t.dim() - 2; left > 0; --left) {  // the dimension of the smallest stride next; those of one element anywhere
+            int64_t d = -1;
+            for (int64_t i = 2; i < t.dim(); ++i)
+                if (!(done >> i & 1) && (d < 0 || stride_of(t, i) < stride_of(t, d))) d = i;
+            done |= (uint64_t)1 << d;
+            if (t.size(d) == 1) continue;
+            const int64_t step = t.stride(d) * size;
+            if (r.pieces == 1 && step == r.piece_bytes) {
+                r.piece_bytes *= t.size(d);
+            } else {
+                TORCH_CHECK(step > 0 && (r.pieces == 1 ? step > r.piece_bytes : step == r.pieces * r.piece_stride), op,
+                            ": a token of a cache tensor must be dense, or pieces at one distance, got sizes ", t.sizes(), " and strides ",
+                            t.strides());
+                if (r.pieces == 1) r.piece_stride = step;
+                r.pieces *= t.size(d);
+            }
+        }
+        TORCH_CHECK((num_pages == 1 || t.stride(0) > 0) && (page_size == 1 || t.stride(1) > 0), op, ": tokens of a cache tensor overlap");
+        list.push_back(r);
+    }
+    return list;
+}
+
+void accept_check(const char* op, const at::Tensor& table, const at::Tensor& lens, const at::Tensor& count, const at::Tensor& seqs,
+                  const at::Tensor& cu, const at::Tensor& tokens, const at::Tensor& parents, const at::Tensor& sampled,
+                  int64_t page_size) {
+    free_check(op, table, lens, count, seqs, page_size);
+    check_index(op, "cu_tokens", cu, 1, table);
+    TORCH_CHECK(cu.size(0) == seqs.size(0) + 1, op, ": cu_tokens must have one value more than seqs, got ", cu.sizes(),
+                " and ", seqs.sizes());
+    check_index(op, "tokens", tokens, 1, table);
+    check_index(op, "parents", parents, 1, table);
+    check_index(op, "sampled", sampled, 1, table);
+    TORCH_CHECK(parents.sizes() == tokens.sizes() && sampled.sizes() == tokens.sizes(), op,
+                ": tokens, parents and sampled must have one length, got ", tokens.sizes(), ", ", parents.sizes(), " and ", sampled.sizes());
+    TORCH_CHECK(tokens.size(0) <= std::numeric_limits<int32_t>::max(), op, ": invalid number of tokens ", tokens.size(0));
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> accept_outputs(const at::Tensor& tokens, const at::Tensor& seqs) {
+    return {at::empty(tokens.sizes(), tokens.options()), at::empty(seqs.sizes(), tokens.options()),
+            at::empty(seqs.sizes(), tokens.options())};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> npu_kv_accept(at::TensorList caches, const at::Tensor& table, const at::Tensor& lens,
+                                                             const at::Tensor& count, const at::Tensor& seqs_in,
+                                                             const at::Tensor& cu_in, const at::Tensor& tokens_in,
+                                                             const at::Tensor& parents_in, const at::Tensor& sampled_in,
+                                                             int64_t page_size) {
+    const char* op = "npu_kv_accept";
+    accept_check(op, table, lens, count, seqs_in, cu_in, tokens_in, parents_in, sampled_in, page_size);
+    const c10::DeviceGuard guard(table.device());
+    const auto list = row_list(op, caches, count.size(0), page_size, table);
+    const auto seqs = seqs_in.contiguous(), cu = cu_in.contiguous(), tokens = tokens_in.contiguous(), parents = parents_in.contiguous(),
+               sampled = sampled_in.contiguous();
+    auto [path, accepted, next] = accept_outputs(tokens, seqs);
+    check_rc(qk_kv_accept(list.data(), (int64_t)list.size(), count.size(0), page_size, written(table), table.size(0), table.size(1),
+                          stride_of(table, 0), written(lens), written(count), index_data(seqs), index_data(cu), seqs.numel(),
+                          tokens.numel(), index_data(tokens), index_data(parents), index_data(sampled), written(path),
+                          written(accepted), written(next), current_stream(table)),
+             op);
+    return {path, accepted, next};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> npu_kv_accept_meta(at::TensorList caches, const at::Tensor& table,
+                                                                  const at::Tensor& lens, const at::Tensor& count,
+                                                                  const at::Tensor& seqs, const at::Tensor& cu,
+                                                                  const at::Tensor& tokens, const at::Tensor& parents,
+                                                                  const at::Tensor& sampled, int64_t page_size) {
+    const char* op = "npu_kv_accept";
+    accept_check(op, table, lens, count, seqs, cu, tokens, parents, sampled, page_size);
+    row_list(op, caches, count.size(0), page_size, table);
+    return accept_outputs(tokens, seqs);
+}
+
 void compact_check(const char* op, const at::Tensor& table, const at::Tensor& count) {
     check_index(op, "block_table", table, 2, table);
     check_index(op, "ref_count", count, 1, table);
@@ -764,6 +850,9 @@ TORCH_LIBRARY_FRAGMENT(npu, m) {
           "int page_size) -> ()");
     m.def("npu_kv_extend(Tensor(a!) block_table, Tensor(b!) context_lens, Tensor(c!) ref_count, Tensor seqs, "
           "Tensor cu_tokens, int total_tokens, int page_size) -> (Tensor, Tensor, Tensor)");
+    m.def("npu_kv_accept(Tensor(a!)[] caches, Tensor(b!) block_table, Tensor(c!) context_lens, Tensor(d!) ref_count, "
+          "Tensor seqs, Tensor cu_tokens, Tensor tokens, Tensor parents, Tensor sampled, int page_size) -> "
+          "(Tensor, Tensor, Tensor)");
     m.def("npu_kv_compact(Tensor(a!)[] caches, Tensor block_table, Tensor ref_count) -> (Tensor, Tensor, Tensor)");
 }
 
@@ -777,6 +866,7 @@ TORCH_LIBRARY_IMPL(npu, CUDA, m) {
     m.impl("npu_kv_fork", &npu_kv_fork);
     m.impl("npu_kv_free", &npu_kv_free);
     m.impl("npu_kv_extend", &npu_kv_extend);
+    m.impl("npu_kv_accept", &npu_kv_accept);
     m.impl("npu_kv_compact", &npu_kv_compact);
 }
 
@@ -790,5 +880,6 @@ TORCH_LIBRARY_IMPL(npu, Meta, m) {
     m.impl("npu_kv_fork", &npu_kv_fork_meta);
     m.impl("npu_kv_free", &npu_kv_free_meta);
     m.impl("npu_kv_extend", &npu_kv_extend_meta);
+    m.impl("npu_kv_accept", &npu_kv_accept_meta);
     m.impl("npu_kv_compact", &npu_kv_compact_meta);
 }

@@ -464,6 +464,35 @@ int qk_kv_extend(int64_t num_pages, int64_t page_size, int32_t* block_table, int
     return launched(qk::launch_kv_extend(p, seqs, cu_tokens, n, total, slots, positions, missing, workspace, (hipStream_t)stream), op);
 }
 
+int qk_kv_accept(const qk_rows* rows, int64_t tensors, int64_t num_pages, int64_t page_size, int32_t* block_table,
+                 int64_t max_seqs, int64_t table_width, int64_t table_stride, int32_t* context_lens, int32_t* ref_count,
+                 const int32_t* seqs, const int32_t* cu_tokens, int64_t n, int64_t total, const int32_t* tokens,
+                 const int32_t* parents, const int32_t* sampled, int32_t* path, int32_t* accepted, int32_t* next,
+                 qk_stream_t stream) {
+    qk::abi_begin();
+    const char* op = "npu_kv_accept";
+    if (int rc = check_pool(op, num_pages, page_size, block_table, max_seqs, table_width, table_stride, context_lens, ref_count)) return rc;
+    if (tensors < 0 || tensors > (1 << 20)) return fail(QK_ERR_ARG, "%s: invalid number of tensors %lld", op, (long long)tensors);
+    if (tensors > 0 && !rows) return fail(QK_ERR_ARG, "%s: null pointer", op);
+    for (int64_t i = 0; i < tensors; ++i) {
+        const qk_rows& t = rows[i];
+        if (t.pieces < 0 || t.piece_bytes < 0 || t.pieces > kInt31 || t.piece_bytes > kInt31 || t.page_stride < 0 || t.token_stride < 0 ||
+            t.piece_stride < 0)
+            return fail(QK_ERR_ARG, "%s: tensor %lld: invalid size or stride", op, (long long)i);
+        if (t.pieces > 0 && t.piece_bytes > 0 && num_pages > 0 && !t.base) return fail(QK_ERR_ARG, "%s: null pointer", op);
+        if (t.pieces > 1 && t.piece_stride < t.piece_bytes) return fail(QK_ERR_ARG, "%s: tensor %lld: pieces overlap", op, (long long)i);
+    }
+    if (int rc = check_seqs(op, n)) return rc;
+    if (total < 0 || total > kInt31) return fail(QK_ERR_ARG, "%s: invalid number of tokens %lld", op, (long long)total);
+    if ((n > 0 && (!seqs || !cu_tokens || !accepted || !next)) || (total > 0 && (!tokens || !parents || !sampled || !path)))
+        return fail(QK_ERR_ARG, "%s: null pointer", op);
+    if (n == 0 && total == 0) return QK_OK;
+    const qk::PoolArgs p = {num_pages, page_size, block_table, max_seqs, table_width, table_stride, context_lens, ref_count};
+    return launched(qk::launch_kv_accept(rows, tensors, p, seqs, cu_tokens, n, total, tokens, parents, sampled, path, accepted, next,
+                                         (hipStream_t)stream),
+                    op);
+}
+
 int qk_kv_compact_workspace_size(int64_t num_pages, size_t* bytes) {
     qk::abi_begin();
     if (!bytes) return fail(QK_ERR_ARG, "npu_kv_compact: null pointer");

@@ -42,7 +42,11 @@ Importing this package loads ``_npu_ops.so``, which registers
   slot_mapping, *, key_scale=None, value_scale=None, mrope_section=None, rotary_mode="half") -> query``: rotary
   positions of one to four axes, alone or with the write into the cache (int8 with scales per token and head)
 * the cache's pages: ``npu_kv_extend``, ``npu_kv_fork``, ``npu_kv_free``, ``npu_kv_copy_pages``, ``npu_kv_compact``
-  (``op_plugin_amd.kv_cache.PagedKVCache`` holds their state)
+  (``op_plugin_amd.kv_cache.PagedKVCache`` holds their state), and ``torch.ops.npu.npu_kv_accept(caches, block_table,
+  context_lens, ref_count, seqs, cu_tokens, tokens, parents, sampled, page_size) -> (path, accepted, next_tokens)``: of trees
+  of drafted tokens the way that was drawn stays in the cache
+* ``torch.ops.npu.npu_sample(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=None) -> (tokens,
+  logprobs)``: a token per row of logits from given uniform numbers, with settings per row
 
 and exposes the same callables here, so code written as
 ``torch_npu.npu_quant_matmul(...)`` runs as ``op_plugin_amd.npu_quant_matmul(...)``
@@ -95,6 +99,8 @@ npu_kv_fork = torch.ops.npu.npu_kv_fork
 npu_kv_free = torch.ops.npu.npu_kv_free
 npu_kv_extend = torch.ops.npu.npu_kv_extend
 npu_kv_compact = torch.ops.npu.npu_kv_compact
+npu_kv_accept = torch.ops.npu.npu_kv_accept
+npu_sample = torch.ops.npu.npu_sample
 
 # qk_abi.h constants
 QK_F16, QK_BF16, QK_F32, QK_I8, QK_I32, QK_U8, QK_I4_NZ, QK_I8_NZ, QK_I8_NK = 1, 2, 3, 4, 5, 6, 16, 17, 18
@@ -112,7 +118,7 @@ ABI_SYMBOLS = (
     "qk_prompt_attention_workspace_size", "qk_prompt_attention", "qk_tree_attention_workspace_size", "qk_tree_attention",
     "qk_mrope", "qk_kv_copy_pages",
     "qk_kv_fork_workspace_size", "qk_kv_fork", "qk_kv_free", "qk_kv_extend_workspace_size", "qk_kv_extend",
-    "qk_kv_compact_workspace_size", "qk_kv_compact",
+    "qk_kv_compact_workspace_size", "qk_kv_compact", "qk_kv_accept", "qk_sample_workspace_size", "qk_sample",
 )
 
 
@@ -125,6 +131,12 @@ class KvCache(ctypes.Structure):
                    "key_scale_page_stride", "key_scale_token_stride", "key_scale_head_stride",
                    "value_scale_page_stride", "value_scale_token_stride", "value_scale_head_stride")] + \
                [("dtype", ctypes.c_int)]
+
+
+class Rows(ctypes.Structure):
+    """qk_rows: where the rows of a cache tensor's tokens lie, in bytes."""
+    _fields_ = [("base", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in (
+        "page_stride", "token_stride", "piece_stride", "pieces", "piece_bytes")]
 
 
 class Pages(ctypes.Structure):
@@ -184,6 +196,10 @@ def abi() -> ctypes.CDLL:
         L.qk_kv_extend.argtypes = [I64, I64, P, I64, I64, I64, P, P, P, P, I64, I64, P, P, P, P, SZ, P]
         L.qk_kv_compact_workspace_size.argtypes = [I64, Z]
         L.qk_kv_compact.argtypes = [G, I64, I64, P, I64, I64, I64, P, P, P, P, P, SZ, P]
+        L.qk_kv_accept.argtypes = [ctypes.POINTER(Rows), I64, I64, I64, P, I64, I64, I64, P, P, P, P, I64, I64, P, P, P, P, P, P,
+                                   P]
+        L.qk_sample_workspace_size.argtypes = [I64, I64, I, I, Z]
+        L.qk_sample.argtypes = [P, I, I64, I64, I64, P, P, P, P, P, P, P, P, SZ, P]
         for name in ABI_SYMBOLS:
             getattr(L, name).restype = I if name != "qk_last_error" else ctypes.c_char_p
         _abi = L
@@ -217,5 +233,5 @@ __all__ = [
     "quantize_per_channel", "dequantize", "npu_rms_norm", "npu_swiglu", "npu_rms_norm_dynamic_quant",
     "npu_swiglu_dynamic_quant", "npu_quant_matmul_swiglu", "npu_quant_matmul_swiglu_quant", "npu_paged_attention",
     "npu_prompt_attention", "npu_tree_attention", "npu_mrope", "npu_mrope_scatter_kv", "npu_kv_copy_pages", "npu_kv_fork", "npu_kv_free",
-    "npu_kv_extend", "npu_kv_compact", "abi", "last_error", "debug_set_plan", "LIB_PATH", "OPS_PATH",
+    "npu_kv_extend", "npu_kv_compact", "npu_kv_accept", "npu_sample", "abi", "last_error", "debug_set_plan", "LIB_PATH", "OPS_PATH",
 ]

@@ -571,6 +571,50 @@ int qk_kv_compact(const qk_pages* pages, int64_t tensors, int64_t num_pages, con
                   int32_t* new_table, int32_t* new_count, int32_t* moved, void* workspace, size_t workspace_bytes,
                   qk_stream_t stream);
 
+/* npu_kv_accept: the end of a step of decoding with drafts.  Sequence seqs[i] (none twice) ends in the tokens of a tree, rows
+ * first = cu_tokens[i] .. cu_tokens[i + 1] of tokens, parents and sampled: n of them, as qk_kv_extend placed them, behind
+ * x = context_lens[seq] - n others.  Row 0 is the root, the token drawn last; the others are drafted, parents[first + k] < k
+ * being the row of the tree that row k follows (rows without such a parent are reached by none).  sampled[first + k] is the
+ * token that was drawn at row k.  From the root the way goes to the lowest of a row's children whose token (not negative) is the one
+ * drawn at the row, until there is none: kept rows 0 = r_0 < r_1 < ... < r_{a-1}.  path[first + j] = first + r_j for j < a, -1
+ * behind; accepted[i] = a (at least 1); next[i] = sampled[first + r_{a-1}], the token that the next tree begins with.
+ * In every tensor the cache's row of token x + r_j moves to x + j (a page id outside [0, num_pages) is not followed); then
+ * context_lens[seq] = x + a, and the pages behind it lose a count and their table entries become -1.  The tree's pages
+ * must not be shared.  A sequence number outside [0, max_seqs), an empty tree, and one larger than the sequence are passed over:
+ * accepted 0, next and path -1.  path [total], accepted and next [n].
+ * A cache tensor is described by qk_rows: the row of the token at place s of page p is `pieces` pieces of piece_bytes bytes,
+ * piece_stride apart, from base + p * page_stride + s * token_stride on (all in bytes).  No workspace. */
+typedef struct qk_rows {
+    void* base;
+    int64_t page_stride, token_stride, piece_stride;
+    int64_t pieces, piece_bytes;
+} qk_rows;
+int qk_kv_accept(const qk_rows* rows, int64_t tensors, int64_t num_pages, int64_t page_size, int32_t* block_table,
+                 int64_t max_seqs, int64_t table_width, int64_t table_stride, int32_t* context_lens, int32_t* ref_count,
+                 const int32_t* seqs, const int32_t* cu_tokens, int64_t n, int64_t total, const int32_t* tokens,
+                 const int32_t* parents, const int32_t* sampled, int32_t* path, int32_t* accepted, int32_t* next,
+                 qk_stream_t stream);
+
+/* ------------------------------------------------------------------ a token per row of logits
+ *
+ * npu_sample -- temperature, top-k, top-p and min-p, and a draw from a given uniform number (the reference leaves sampling
+ * to the framework's own sort, cumsum and multinomial).  logits: [rows][vocab] QK_F16, QK_BF16 or QK_F32, rows row_stride
+ * elements apart, vocab 1 .. QK_MAX_VOCAB.  The others are [rows] on the device; all but uniform may be NULL.
+ *   w_i = exp((x_i - max x) / temperature[r])       (NULL: 1)
+ * The row's tokens in order of x, falling, ties by index.  top_k[r] > 0 keeps the first so many.  top_p[r] < 1 keeps of
+ * those the ones before which less than top_p of their sum of w lies.  min_p[r] > 0 keeps those with w_i >= min_p (above 1:
+ * as 1).  The first is always kept.  S = the sum of the kept w; tokens[r] is the lowest kept i at which the kept w up to and
+ * including i sum to more than uniform[r] * S (uniform cut to [0, 1)), logprobs[r] = ln(w_i / S).  A temperature that is
+ * not above 0 takes the first, logprob 0.  A logit -inf or NaN is never drawn; a row without another gives token -1, logprob
+ * -inf.  Among infinite logits all weight is theirs, in equal parts.  Weights are multiples of 2^-F of the largest, F = 62 -
+ * ceil(log2 vocab), at most 50, and sums of them exact: the result does not depend on how the work is split.
+ */
+#define QK_MAX_VOCAB (1 << 24)
+int qk_sample_workspace_size(int64_t rows, int64_t vocab, int dtype, int filters, size_t* bytes);
+int qk_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride, const float* uniform,
+              const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens,
+              float* logprobs, void* workspace, size_t workspace_bytes, qk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
