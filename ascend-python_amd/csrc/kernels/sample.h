@@ -17,7 +17,7 @@ struct SampleArgs {
     int32_t* tokens;
     float* logprobs;
 };
-size_t sample_workspace(int64_t rows, int64_t vocab, int dtype, bool filters);
+size_t sample_workspace(int64_t rows, int64_t vocab, int dtype);
 hipError_t launch_sample(const SampleArgs& a, void* workspace, hipStream_t stream);
 
 }  // namespace qk

@@ -61,7 +61,7 @@ std::tuple<at::Tensor, at::Tensor> npu_sample(const at::Tensor& logits, const at
     const auto *p = (const float*)setting(2, top_p), *m = (const float*)setting(3, min_p);
     const int dtype = qk_dtype_of(x.scalar_type());
     size_t ws_bytes = 0;
-    check_rc(qk_sample_workspace_size(rows, vocab, dtype, k || p || m, &ws_bytes));
+    check_rc(qk_sample_workspace_size(rows, vocab, dtype, &ws_bytes));
     const auto ws = at::empty({(int64_t)ws_bytes}, x.options().dtype(at::kByte));
     check_rc(qk_sample(x.const_data_ptr(), dtype, rows, vocab, rows > 1 ? x.stride(0) : 0, uniform.const_data_ptr<float>(), t, k, p, m,
                        tokens.data_ptr<int32_t>(), logprobs.data_ptr<float>(), ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,

@@ -32,11 +32,11 @@ int check_sizes(int64_t rows, int64_t vocab, int dtype) {
 
 extern "C" {
 
-int qk_sample_workspace_size(int64_t rows, int64_t vocab, int dtype, int filters, size_t* bytes) {
+int qk_sample_workspace_size(int64_t rows, int64_t vocab, int dtype, size_t* bytes) {
     qk::abi_begin();
     if (!bytes) return fail(QK_ERR_ARG, "%s: null pointer", kOp);
     if (int rc = check_sizes(rows, vocab, dtype)) return rc;
-    *bytes = qk::sample_workspace(rows, vocab, dtype, filters != 0);
+    *bytes = qk::sample_workspace(rows, vocab, dtype);
     return QK_OK;
 }
 
@@ -50,7 +50,7 @@ int qk_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_
     if (row_stride < 0) return fail(QK_ERR_ARG, "%s: negative stride", kOp);
     if ((uintptr_t)logits % (dtype == QK_F32 ? 4 : 2) != 0) return fail(QK_ERR_ARG, "%s: logits that are not whole elements", kOp);
     const qk::SampleArgs a = {logits, dtype, rows, vocab, row_stride, uniform, temperature, top_k, top_p, min_p, tokens, logprobs};
-    const size_t need = qk::sample_workspace(rows, vocab, dtype, top_k || top_p || min_p);
+    const size_t need = qk::sample_workspace(rows, vocab, dtype);
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(QK_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", kOp, need, workspace_bytes);
     if (need > 0 && (uintptr_t)workspace % 256 != 0) return fail(QK_ERR_WORKSPACE, "%s: the workspace must be 256-byte aligned", kOp);

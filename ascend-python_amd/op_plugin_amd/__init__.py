@@ -198,7 +198,7 @@ def abi() -> ctypes.CDLL:
         L.qk_kv_compact.argtypes = [G, I64, I64, P, I64, I64, I64, P, P, P, P, P, SZ, P]
         L.qk_kv_accept.argtypes = [ctypes.POINTER(Rows), I64, I64, I64, P, I64, I64, I64, P, P, P, P, I64, I64, P, P, P, P, P, P,
                                    P]
-        L.qk_sample_workspace_size.argtypes = [I64, I64, I, I, Z]
+        L.qk_sample_workspace_size.argtypes = [I64, I64, I, Z]
         L.qk_sample.argtypes = [P, I, I64, I64, I64, P, P, P, P, P, P, P, P, SZ, P]
         for name in ABI_SYMBOLS:
             getattr(L, name).restype = I if name != "qk_last_error" else ctypes.c_char_p

@@ -610,7 +610,7 @@ int qk_kv_accept(const qk_rows* rows, int64_t tensors, int64_t num_pages, int64_
  * ceil(log2 vocab), at most 50, and sums of them exact: the result does not depend on how the work is split.
  */
 #define QK_MAX_VOCAB (1 << 24)
-int qk_sample_workspace_size(int64_t rows, int64_t vocab, int dtype, int filters, size_t* bytes);
+int qk_sample_workspace_size(int64_t rows, int64_t vocab, int dtype, size_t* bytes);
 int qk_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride, const float* uniform,
               const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens,
               float* logprobs, void* workspace, size_t workspace_bytes, qk_stream_t stream);
