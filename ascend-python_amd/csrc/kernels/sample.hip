@@ -24,6 +24,7 @@ constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;      // of the histograms
 constexpr int kPerUnit = 64;     // bins per temperature
+constexpr float kSlope = 0.0155038f;  // 1 - e^(-1 / 64): what a weight falls in a bin
 constexpr int kList = 4096;      // tokens in the border's bins
 constexpr int kSegmentVectors = 256;
 constexpr int kSegments = 1024;  // of a row at most
@@ -47,118 +48,126 @@ __device__ __forceinline__ float load_logit(const void* row, int64_t i) {
     else return load_half_bits(((const uint16_t*)row)[i], DT);
 }
 
-// 2^t for -64 <= t <= 0: 2^n times the Taylor series of e^(f ln 2), |f| <= 1/2, whose terms past the 13th are below 2^-56.
-__device__ __forceinline__ double pow2(double t) {
-    const double n = __builtin_rint(t), z = (t - n) * 0.693147180559945309417;
-    double p = 1.0 / 479001600.0;
-    p = __builtin_fma(p, z, 1.0 / 39916800.0);
-    p = __builtin_fma(p, z, 1.0 / 3628800.0);
-    p = __builtin_fma(p, z, 1.0 / 362880.0);
-    p = __builtin_fma(p, z, 1.0 / 40320.0);
-    p = __builtin_fma(p, z, 1.0 / 5040.0);
-    p = __builtin_fma(p, z, 1.0 / 720.0);
-    p = __builtin_fma(p, z, 1.0 / 120.0);
-    p = __builtin_fma(p, z, 1.0 / 24.0);
-    p = __builtin_fma(p, z, 1.0 / 6.0);
-    p = __builtin_fma(p, z, 0.5);
-    p = __builtin_fma(p, z, 1.0);
-    p = __builtin_fma(p, z, 1.0);
-    return __builtin_ldexp(p, (int)n);
+// a * b + c with c in scalar registers: by itself the compiler copies such a c into the result's registers first, once per product.
+__device__ __forceinline__ double fma_scalar(double a, double b, double c) {
+    double d;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+    return d;
+}
+// 2^t times 2^bits as a whole number, 0 where t is below -60 or NaN (t <= 0): 2^n times a polynomial in f = t - n, |f| <= 1/2, that
+// meets 2^f in the 11 Chebyshev nodes and stays within 2^-51 of it; rounded by adding 2^(52 - bits), in whose last bits the number
+// then stands.
+__device__ __forceinline__ uint64_t weight_of_log2(double t, int bits) {
+    double c, p;
+    asm("v_max_f64 %0, %1, %2" : "=v"(c) : "v"(t), "s"(-60.0));
+    const double n = __builtin_rint(c), f = c - n;
+    p = fma_scalar(0x1.e6063f7217bc6p-28, f, 0x1.b675bca4eeebbp-24);
+    p = fma_scalar(p, f, 0x1.62bfd47773353p-20);
+    p = fma_scalar(p, f, 0x1.ffcb54062e698p-17);
+    p = fma_scalar(p, f, 0x1.430913096fd9fp-13);
+    p = fma_scalar(p, f, 0x1.5d87fe9d7a584p-10);
+    p = fma_scalar(p, f, 0x1.3b2ab6fba1ddap-7);
+    p = fma_scalar(p, f, 0x1.c6b08d703ce49p-5);
+    p = fma_scalar(p, f, 0x1.ebfbdff82c598p-3);
+    p = fma_scalar(p, f, 0x1.62e42fefa3a19p-1);
+    p = __builtin_fma(p, f, 1.0);
+    return __builtin_bit_cast(uint64_t, __builtin_ldexp(p, (int)n) + __builtin_ldexp(1.0, 52 - bits)) & 0xfffffffffffffull;
 }
 
 // Weights of a row whose largest logit is `top`.
 struct Weights {
     double top, factor;  // log2 e / temperature
-    double one;          // 2^F, the largest weight
+    int bits;            // F: the largest weight is 2^F
     bool infinite;       // top is: equal weights for its like, none for the others
 
-    // log2 of the weight of a logit that is not below the lowest finite one
+    // log2 of a logit's weight in a row without an infinite one (-inf: -inf, or NaN where the temperature is infinite)
+    __device__ __forceinline__ double finite_log2(float x) const { return ((double)x - top) * factor; }
+    __device__ __forceinline__ uint64_t finite(float x) const { return weight_of_log2(finite_log2(x), bits); }
+    // ... in any row
     __device__ __forceinline__ double log2_of(float x) const {
         if (infinite) return x == __builtin_inff() ? 0.0 : -__builtin_inf();
-        return ((double)x - top) * factor;
+        return finite_log2(x);
     }
-    __device__ __forceinline__ uint64_t of_log2(double t) const {
-        if (!(t >= -60.0)) return 0;
-        // rounded to a whole number by adding 2^52, in whose last bits it then stands
-        return __builtin_bit_cast(uint64_t, pow2(t) * one + 0x1p52) & 0xfffffffffffffull;
-    }
-    __device__ __forceinline__ uint64_t of(uint32_t key) const { return key < kLeast ? 0 : of_log2(log2_of(value_of(key))); }
+    __device__ __forceinline__ uint64_t of(uint32_t key) const { return key < kLeast ? 0 : weight_of_log2(log2_of(value_of(key)), bits); }
 };
 
 // ---------------------------------------------------------------- sums over a workgroup
 
-struct Sums {
-    uint32_t count;
-    uint64_t weight;
+// v of the lane that the move `DPP` names, 0 where there is none
+template <int DPP, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, DPP, ROWS, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), DPP, ROWS, 0xf, true);
+    return (uint64_t)hi << 32 | lo;
+}
+// Sum over the lanes up to this one: within rows of 16 lanes, then from a row's last lane to those behind.
+__device__ __forceinline__ uint64_t wave_upto(uint64_t v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    v += moved<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
+}
+
+// Sums, maxima and minima over the workgroup, each with one barrier: calls take the two halves of the space in turn, so that
+// one may write while the one before is still read.
+struct Group {
+    struct Space {
+        uint64_t of[2][kWaves];
+    };
+    Space& sh;
+    int turn = 0;
+
+    __device__ __forceinline__ const uint64_t* exchange(uint64_t of_wave, bool writes) {
+        turn ^= 1;
+        if (writes) sh.of[turn][threadIdx.x >> 6] = of_wave;
+        __syncthreads();
+        return sh.of[turn];
+    }
+    // Sum over the threads before this one, and over all.
+    __device__ __forceinline__ uint64_t before(uint64_t v, uint64_t& all) {
+        const int wave = threadIdx.x >> 6;
+        const uint64_t upto = wave_upto(v);
+        const uint64_t* const of = exchange(upto, (threadIdx.x & 63) == 63);
+        uint64_t sum = upto - v;
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            sum += w < wave ? of[w] : 0;
+            all += of[w];
+        }
+        return sum;
+    }
+    __device__ __forceinline__ uint64_t sum(uint64_t v) {
+        uint64_t all;
+        before(v, all);
+        return all;
+    }
+    __device__ __forceinline__ float max(float v) {
+        const uint64_t* const of = exchange(__float_as_uint(wave_max(v)), (threadIdx.x & 63) == 0);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) v = fmaxf(v, __uint_as_float((uint32_t)of[w]));
+        return v;
+    }
+    __device__ __forceinline__ uint32_t min(uint32_t v) {
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_xor(v, d);
+            v = o < v ? o : v;
+        }
+        const uint64_t* const of = exchange(v, (threadIdx.x & 63) == 0);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) v = (uint32_t)of[w] < v ? (uint32_t)of[w] : v;
+        return v;
+    }
 };
 
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
-    return (uint64_t)__shfl_up((uint32_t)(v >> 32), d) << 32 | __shfl_up((uint32_t)v, d);
-}
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-    for (int d = 1; d < 64; d <<= 1) v += (uint64_t)__shfl_xor((uint32_t)(v >> 32), d) << 32 | __shfl_xor((uint32_t)v, d);
-    return v;
-}
-
-struct Scan {
-    uint64_t weight[kWaves];
-    uint32_t count[kWaves];
-};
-
-// Sums over the threads before this one, and over all.
-__device__ __forceinline__ Sums scan_before(Sums v, Sums& all, Scan& sh) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    Sums in = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t w = shfl_up64(in.weight, d);
-        const uint32_t c = __shfl_up(in.count, d);
-        if (lane >= d) {
-            in.weight += w;
-            in.count += c;
-        }
-    }
-    __syncthreads();  // what an earlier call left has been read
-    if (lane == 63) {
-        sh.weight[wave] = in.weight;
-        sh.count[wave] = in.count;
-    }
-    __syncthreads();
-    Sums before = {in.count - v.count, in.weight - v.weight};
-    all = {0, 0};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) {
-            before.weight += sh.weight[w];
-            before.count += sh.count[w];
-        }
-        all.weight += sh.weight[w];
-        all.count += sh.count[w];
-    }
-    return before;
-}
-
-__device__ __forceinline__ float block_max(float v, Scan& sh) {
-    v = wave_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.count[threadIdx.x >> 6] = __float_as_uint(v);
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) v = fmaxf(v, __uint_as_float(sh.count[w]));
-    return v;
-}
-__device__ __forceinline__ uint32_t block_min(uint32_t v, Scan& sh) {
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_xor(v, d);
-        v = o < v ? o : v;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.count[threadIdx.x >> 6] = v;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) v = sh.count[w] < v ? sh.count[w] : v;
-    return v;
-}
+// (one of it in a kernel, not one at each use)
+__device__ __attribute__((noinline)) double log2_of_double(double v) { return ::log2(v); }
 
 // ---------------------------------------------------------------- what a row is asked for
 
@@ -178,12 +187,11 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int64_t r) 
     return s;
 }
 __device__ __forceinline__ Weights weights_of(const Settings& s, float top, int bits) {
-    return {(double)top, s.greedy ? 0.0 : 1.44269504088896340736 / (double)s.temperature, __builtin_ldexp(1.0, bits),
-            top == __builtin_inff()};
+    return {(double)top, s.greedy ? 0.0 : 1.44269504088896340736 / (double)s.temperature, bits, top == __builtin_inff()};
 }
 // The least log2 of a weight that min_p keeps
 __device__ __forceinline__ double least_of(const Settings& s) {
-    return s.min_p > 0.0f ? ::log2((double)(s.min_p < 1.0f ? s.min_p : 1.0f)) : -__builtin_inf();
+    return s.min_p > 0.0f ? log2_of_double((double)(s.min_p < 1.0f ? s.min_p : 1.0f)) : -__builtin_inf();
 }
 // The weight that the kept ones reach first, of a whole of `total`: at least 1, so that the first token stays
 __device__ __forceinline__ uint64_t top_p_goal(const Settings& s, uint64_t total) {
@@ -192,7 +200,7 @@ __device__ __forceinline__ uint64_t top_p_goal(const Settings& s, uint64_t total
 }
 __device__ __forceinline__ void write_token(const SampleArgs& a, int64_t r, int64_t i, float x, const Weights& w, int bits, uint64_t total) {
     a.tokens[r] = (int32_t)i;
-    a.logprobs[r] = (float)((w.log2_of(x) + (double)bits - ::log2((double)total)) * 0.693147180559945309417);
+    a.logprobs[r] = (float)((w.log2_of(x) + (double)bits - log2_of_double((double)total)) * 0.693147180559945309417);
 }
 
 // ---------------------------------------------------------------- one workgroup, border by border
@@ -212,9 +220,10 @@ struct Border {
 
 // Where the count (by_weight: the weight) of the sorted row reaches `goal`, which all of it does reach.
 template <int DT>
-__device__ Border find_border(const void* row, int64_t n, const Weights& w, bool by_weight, uint64_t goal, Digits& sh, Scan& scan) {
+__device__ Border find_border(const void* row, int64_t n, const Weights& w, bool by_weight, uint64_t goal, Digits& sh, Group& group) {
     uint32_t prefix = 0, count_above = 0, equal = 0;
     uint64_t weight_above = 0;
+#pragma nounroll
     for (int level = 0; level < 3; ++level) {
         const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
         for (int i = threadIdx.x; i < kBins; i += kThreads) {
@@ -233,27 +242,23 @@ __device__ Border find_border(const void* row, int64_t n, const Weights& w, bool
         // a thread has some bins, the highest first
         constexpr int kOwn = kBins / kThreads;
         const int hi = kBins - 1 - kOwn * (int)threadIdx.x;
-        Sums own = {0, 0}, all;
-#pragma unroll
+        uint64_t count = 0, weight = 0, all;
         for (int k = 0; k < kOwn; ++k) {
-            own.count += sh.count[hi - k];
-            own.weight += sh.weight[hi - k];
+            count += sh.count[hi - k];
+            weight += sh.weight[hi - k];
         }
-        Sums before = scan_before(own, all, scan);
-        before.count += count_above;
-        before.weight += weight_above;
-#pragma unroll
+        count = count_above + group.before(count, all);
+        weight = weight_above + group.before(weight, all);
         for (int k = 0; k < kOwn; ++k) {
-            const Sums bin = {sh.count[hi - k], sh.weight[hi - k]};
-            const uint64_t from = by_weight ? before.weight : before.count, to = from + (by_weight ? bin.weight : bin.count);
+            const uint64_t from = by_weight ? weight : count, to = from + (by_weight ? sh.weight[hi - k] : sh.count[hi - k]);
             if (from < goal && goal <= to) {
                 sh.found_bin = hi - k;
-                sh.found_count = before.count;
-                sh.found_weight = before.weight;
-                sh.found_in_bin = bin.count;
+                sh.found_count = (uint32_t)count;
+                sh.found_weight = weight;
+                sh.found_in_bin = sh.count[hi - k];
             }
-            before.count += bin.count;
-            before.weight += bin.weight;
+            count += sh.count[hi - k];
+            weight += sh.weight[hi - k];
         }
         __syncthreads();
         prefix = prefix << bits | sh.found_bin;
@@ -274,42 +279,44 @@ __device__ Border find_border(const void* row, int64_t n, const Weights& w, bool
 
 // A row whose largest logit is `top`, above -inf.
 template <int DT>
-__device__ void draw_alone(const SampleArgs& a, int64_t r, const void* row, const Settings& s, float top, int bits, Digits& sh, Scan& scan) {
+__device__ __forceinline__ void draw_alone(const SampleArgs& a, int64_t r, const void* row, const Settings& s, float top, int bits, Digits& sh,
+                                           Group& group) {
     const int tid = threadIdx.x;
     const int64_t n = a.vocab;
     const Weights w = weights_of(s, top, bits);
     const double least = least_of(s);
+    __syncthreads();  // what the space held has been read
     // the kept: down to `border`, of whose ties those up to index `last`, and of those the ones of log2 weight `least` and more
     Border border = {kLeast, 0, 0, 0};
     bool cut = false;
-    Sums all, mine = {0, 0};
     if ((s.top_k > 0 && s.top_k < n) || s.top_p < 1.0f) {
+        uint64_t count = 0, total = 0;
         for (int64_t i = tid; i < n; i += kThreads) {
             const uint32_t key = key_of(load_logit<DT>(row, i));
-            mine.count += key >= kLeast;
-            mine.weight += w.of(key);
+            count += key >= kLeast;
+            total += w.of(key);
         }
-        scan_before(mine, all, scan);
-        uint64_t total = all.weight;
-        if (s.top_k > 0 && (uint32_t)s.top_k < all.count) {
-            border = find_border<DT>(row, n, w, false, (uint64_t)s.top_k, sh, scan);
+        count = group.sum(count);
+        total = group.sum(total);
+        if (s.top_k > 0 && (uint64_t)s.top_k < count) {
+            border = find_border<DT>(row, n, w, false, (uint64_t)s.top_k, sh, group);
             cut = true;
             total = border.above + border.ties * w.of(border.key);
         }
         if (s.top_p < 1.0f) {
-            border = find_border<DT>(row, n, w, true, top_p_goal(s, total), sh, scan);
+            border = find_border<DT>(row, n, w, true, top_p_goal(s, total), sh, group);
             cut = true;
         }
     }
     int64_t last = n - 1;
     if (cut && border.ties < border.equal) {
-        uint32_t seen = 0;
+        uint64_t seen = 0, all;
         for (int64_t base = 0; base < n && seen < border.ties; base += kThreads) {
             const int64_t i = base + tid;
             const bool tie = i < n && key_of(load_logit<DT>(row, i)) == border.key;
-            const Sums before = scan_before({tie, 0}, all, scan);
-            if (tie && seen + before.count == border.ties - 1) sh.found_weight = (uint64_t)i;
-            seen += all.count;
+            const uint64_t before = group.before(tie, all);
+            if (tie && seen + before == border.ties - 1) sh.found_weight = (uint64_t)i;
+            seen += all;
         }
         __syncthreads();
         last = (int64_t)sh.found_weight;
@@ -320,16 +327,15 @@ __device__ void draw_alone(const SampleArgs& a, int64_t r, const void* row, cons
         if (key < border.key || (key == border.key && i > last) || key < kLeast || w.log2_of(value_of(key)) < least) return 0;
         return w.of(key);
     };
-    mine = {0, 0};
-    for (int64_t i = tid; i < n; i += kThreads) mine.weight += kept(i);
-    scan_before(mine, all, scan);
-    const uint64_t total = all.weight, goal = (uint64_t)((double)s.uniform * (double)total) + 1;  // at most total
-    uint64_t passed = 0;
+    uint64_t total = 0;
+    for (int64_t i = tid; i < n; i += kThreads) total += kept(i);
+    total = group.sum(total);
+    const uint64_t goal = (uint64_t)((double)s.uniform * (double)total) + 1;  // at most total
+    uint64_t passed = 0, all;
     for (int64_t base = 0; base < n && passed < goal; base += kThreads) {
-        const uint64_t v = kept(base + tid);
-        const uint64_t from = passed + scan_before({0, v}, all, scan).weight;
+        const uint64_t v = kept(base + tid), from = passed + group.before(v, all);
         if (from < goal && goal <= from + v) write_token(a, r, base + tid, load_logit<DT>(row, base + tid), w, bits, total);
-        passed += all.weight;
+        passed += all;
     }
 }
 
@@ -356,46 +362,70 @@ struct Row {
         n = (int32_t)a.vocab;
         count = (n + offset + kPer - 1) / kPer;
     }
-    // A lane's vectors of a segment (past the row: of what comes first, not used)
-    __device__ __forceinline__ void load(int32_t segment, int lane, u32x4 (&v)[kSteps]) const {
+    // f(first token, logits) for a lane's vectors of a segment, -inf for what is not the row's
+    template <typename F>
+    __device__ __forceinline__ void each(int32_t segment, int lane, F f) const {
+        u32x4 v[kSteps];
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
             const int32_t at = segment * kSegmentVectors + k * 64 + lane;
             v[k] = vectors[at < count ? at : 0];
         }
-    }
-    // f(token, logit) for its elements, -inf past the row's
-    template <typename F>
-    __device__ __forceinline__ void each(int32_t segment, int lane, const u32x4 (&v)[kSteps], F f) const {
-#pragma unroll
+        const bool inside = segment * kSegmentVectors * kPer >= offset && (segment + 1) * kSegmentVectors * kPer - offset <= n;
+        // (the vectors move up instead of the loop being written out: a workgroup runs it a few times, and fetching its code costs more)
+#pragma nounroll
         for (int k = 0; k < kSteps; ++k) {
             const int32_t first = (segment * kSegmentVectors + k * 64 + lane) * kPer - offset;
+            float x[kPer];
 #pragma unroll
             for (int e = 0; e < kPer; ++e) {
-                float x;
-                if constexpr (DT == QK_F32) x = __uint_as_float(v[k][e]);
-                else x = load_half_bits(v[k][e >> 1] >> (16 * (e & 1)) & 0xffffu, DT);
-                f(first + e, (uint32_t)(first + e) < (uint32_t)n ? x : -__builtin_inff());
+                if constexpr (DT == QK_F32) x[e] = __uint_as_float(v[0][e]);
+                else x[e] = load_half_bits(v[0][e >> 1] >> (16 * (e & 1)) & 0xffffu, DT);
             }
+#pragma unroll
+            for (int i = 1; i < kSteps; ++i) v[i - 1] = v[i];
+            if (!inside) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) x[e] = (uint32_t)(first + e) < (uint32_t)n ? x[e] : -__builtin_inff();
+            }
+            f(first, x);
         }
     }
     __device__ __forceinline__ int32_t segment_of(uint32_t token) const { return (int32_t)(token + offset) / (kPer * kSegmentVectors); }
 };
 
-// The bin of a logit: below the one of `top` by so many.  Falls where the logit rises, as every step of it does.
+// The number of a logit's bin, cut to 32 bits: it rises with the logit, as every step of it does.
 __device__ __forceinline__ int32_t bin_at(float x, float per_bin) {
-    return (int32_t)__builtin_floorf(fminf(fmaxf(x * per_bin, -0x1p29f), 0x1p29f));
+    int32_t at;
+    asm("v_cvt_flr_i32_f32 %0, %1" : "=v"(at) : "v"(x * per_bin));
+    return at;
+}
+// The least logit for which `is` holds, which does not hold again below it; +inf where it holds for no finite one.  A wave's lanes
+// try 64 at a time.
+template <typename F>
+__device__ __forceinline__ float least_logit(F is) {
+    uint32_t low = kLeast, high = 0xff800000u;  // of -FLT_MAX and of +inf
+    while (low < high) {
+        const uint32_t step = (high - low + 63) / 64;
+        uint32_t at = low + (threadIdx.x & 63) * step;
+        at = at < high ? at : high;
+        const uint64_t held = __builtin_amdgcn_ballot_w64(at == high || is(value_of(at)));
+        const int first = held ? __builtin_ctzll(held) : 64;
+        const uint32_t next = low + first * step;
+        if (first > 0) low = next - step + 1;
+        if (first < 64 && next < high) high = next;
+    }
+    return value_of(__builtin_amdgcn_readfirstlane((int)low));
 }
 
 // What the look at a row found: it is done (greedy, or nothing to draw), it is done by one workgroup, no filter cuts it, or the border of
-// the kept tokens lies in bins low .. high, counted from the one of `top` (kBins: all past the histogram), `above` tokens before
-// them; top_k: 0 where that does not cut.
+// the kept tokens lies among the logits from `listed` to `above`, at which those begin that are kept for certain, `count` of them;
+// top_k: 0 where that does not cut; keep: the least logit that min_p keeps.
 constexpr int kDone = 0, kAlone = 1, kWhole = 2, kCut = 3;
 struct Plan {
-    int32_t mode;
-    float top;
-    int32_t top_bin, low, high, top_k;
-    uint32_t above;
+    int32_t mode, top_k;
+    uint32_t count;
+    float top, above, listed, keep;
 };
 // What a workgroup's look at its part found: the largest logit, the first token that has it (greedy rows), how many could be drawn
 // (rows with a histogram).
@@ -424,81 +454,100 @@ union Space {
     Digits digits;
 };
 
-// A part of a row: its largest logit and, where a filter cuts, its histogram.  The weight of a logit in units of that of its bin's upper
-// end, 1 - z + z^2 / 2 for e^-z below 1/64: it only has to lead to the border.
+// A part of a row: its largest logit and, where a filter cuts, its histogram.  Weights there are in units of that of the bin's upper
+// end, and near enough: they only have to lead to the border.
 template <int DT>
-__device__ Part look_at(const Row<DT>& row, const Settings& s, bool histogram, int32_t seg0, int32_t seg1, Look& sh, Scan& scan) {
+__device__ Part look_at(const Row<DT>& row, const Settings& s, bool histogram, int32_t seg0, int32_t seg1, Look& sh, Group& group) {
+    constexpr int kPer = Row<DT>::kPer;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    u32x4 v[Row<DT>::kSteps];
     Part part = {-__builtin_inff(), 0xffffffffu, 0};
-    for (int32_t g = seg0 + wave; g < seg1; g += kWaves) {
-        row.load(g, lane, v);
-        row.each(g, lane, v, [&](int32_t, float x) { part.top = fmaxf(part.top, x); });
-    }
+    for (int32_t g = seg0 + wave; g < seg1; g += kWaves)
+        row.each(g, lane, [&](int32_t, const float (&x)[kPer]) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) part.top = fmaxf(part.top, x[e]);
+        });
     if (histogram)
         for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
-    part.top = block_max(part.top, scan);
+    part.top = group.max(part.top);
     if (s.greedy) {
-        for (int32_t g = seg0 + wave; g < seg1; g += kWaves) {
-            row.load(g, lane, v);
-            row.each(g, lane, v, [&](int32_t i, float x) { part.first = x == part.top && (uint32_t)i < part.first ? (uint32_t)i : part.first; });
-        }
-        part.first = block_min(part.first, scan);
+        for (int32_t g = seg0 + wave; g < seg1; g += kWaves)
+            row.each(g, lane, [&](int32_t first, const float (&x)[kPer]) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e)
+                    if (x[e] == part.top && (uint32_t)(first + e) < part.first) part.first = first + e;
+            });
+        part.first = group.min(part.first);
     }
     if (histogram) {
         const float per_bin = (float)kPerUnit / s.temperature;
         const int32_t top_bin = bin_at(part.top, per_bin);
-        for (int32_t g = seg0 + wave; g < seg1; g += kWaves) {
-            row.load(g, lane, v);
-            row.each(g, lane, v, [&](int32_t, float x) {
-                if (x > -__builtin_inff()) {
-                    ++part.valid;
-                    const int32_t at = bin_at(x, per_bin), bin = top_bin - at;
-                    const float z = fminf(fmaxf((float)at + 1.0f - x * per_bin, 0.0f), 1.0f) * (1.0f / kPerUnit);
-                    if (bin < kBins)
-                        atomicAdd((unsigned long long*)&sh.bins[bin], 1ull << 40 | (uint32_t)((1.0f - z + 0.5f * z * z) * 0x1p20f));
+        for (int32_t g = seg0 + wave; g < seg1; g += kWaves)
+            row.each(g, lane, [&](int32_t, const float (&x)[kPer]) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    const bool valid = x[e] > -__builtin_inff();
+                    part.valid += valid;
+                    const uint32_t bin = (uint32_t)top_bin - (uint32_t)bin_at(x[e], per_bin);
+                    // e^-z, z = (1 - f) / 64: on the line that passes it by 2^-15 at most
+                    const float f = __builtin_amdgcn_fractf(x[e] * per_bin);
+                    if (valid && bin < (uint32_t)kBins)
+                        atomicAdd((unsigned long long*)&sh.bins[bin], 1ull << 40 | (uint32_t)__builtin_fmaf(f, 0x1p20f * kSlope, 0x1p20f * (0.99998f - kSlope)));
                 }
             });
-        }
-        Sums all;
-        scan_before({part.valid, 0}, all, scan);  // (its barriers: the histogram is whole behind them)
-        part.valid = all.count;
+        part.valid = (uint32_t)group.sum(part.valid);  // (its barrier: the histogram is whole behind it)
     }
     return part;
 }
 
+// The plan of a row that no filter but min_p cuts.
+__device__ __forceinline__ Plan plan_of(const Settings& s, float top, int bits) {
+    Plan p = {kWhole, 0, 0, top, value_of(kLeast), value_of(kLeast), value_of(kLeast)};
+    if (s.min_p > 0.0f) {
+        const Weights w = weights_of(s, top, bits);
+        const double least = least_of(s);
+        p.keep = least_logit([&](float x) { return w.finite_log2(x) >= least; });
+    }
+    return p;
+}
+
 // The border's bins of a row; bin(b, count, weight) gives the histogram's bin b, its weight in units of its own upper end.
 template <typename F>
-__device__ Plan plan_row(const Settings& s, float top, uint32_t valid, Look& sh, Scan& scan, F bin) {
+__device__ Plan plan_row(const Settings& s, float top, int bits, uint32_t valid, Look& sh, Group& group, F bin) {
     constexpr int kOwn = kBins / kThreads;
     const int first = kOwn * threadIdx.x;
-    Sums own[kOwn], sum = {0, 0}, all;
+    // counts, and weights in units of 2^-22 of the top bin's upper end, as count << 43 | weight
+    constexpr int kCount = 43;
+    struct Sums {
+        uint32_t count;
+        uint64_t weight;
+    };
+    auto apart = [](uint64_t v) { return Sums{(uint32_t)(v >> kCount), v & (((uint64_t)1 << kCount) - 1)}; };
+    uint64_t own[kOwn], sum = 0, all;
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
+        uint32_t count;
         float weight;
-        bin(first + k, own[k].count, weight);
-        // in units of 2^-24 of the top bin's upper end
-        own[k].weight = (uint64_t)(weight * __builtin_amdgcn_exp2f((float)(first + k) * (-1.44269504f / kPerUnit)) * 0x1p24f);
-        sum.count += own[k].count;
-        sum.weight += own[k].weight;
+        bin(first + k, count, weight);
+        weight *= __builtin_amdgcn_exp2f((float)(first + k) * (-1.44269504f / kPerUnit)) * 0x1p22f;
+        own[k] = (uint64_t)count << kCount | (uint64_t)weight;
+        sum += own[k];
     }
-    const Sums before = scan_before(sum, all, scan);
+    const uint64_t before = group.before(sum, all);
     const bool cuts = s.top_k > 0 && (uint32_t)s.top_k < valid;
     if (threadIdx.x == 0) {
         sh.found[0] = sh.found[1] = sh.found[2] = kBins;
-        sh.weight[0] = sh.weight[1] = all.weight;
-        sh.above = all.count;
+        sh.weight[0] = sh.weight[1] = apart(all).weight;
+        sh.above = apart(all).count;
         sh.upto = valid;
     }
     __syncthreads();
     // visit(b, sums before the bin, the bin's): this thread's bins
     auto each = [&](auto visit) {
-        Sums at = before;
+        uint64_t at = before;
 #pragma unroll
         for (int k = 0; k < kOwn; ++k) {
-            visit(first + k, at, own[k]);
-            at.count += own[k].count;
-            at.weight += own[k].weight;
+            visit(first + k, apart(at), apart(own[k]));
+            at += own[k];
         }
     };
     if (cuts)
@@ -520,78 +569,90 @@ __device__ Plan plan_row(const Settings& s, float top, uint32_t valid, Look& sh,
         });
     }
     __syncthreads();
-    Plan p = {kCut, top, bin_at(top, (float)kPerUnit / s.temperature), 0, 0, cuts ? s.top_k : 0, 0};
-    p.low = s.top_p < 1.0f && sh.found[0] < sh.found[2] ? sh.found[0] : sh.found[2];
-    p.high = cuts ? sh.found[2] : sh.found[1];
-    if (p.high < p.low) p.high = p.low;
+    const int32_t low = s.top_p < 1.0f && sh.found[0] < sh.found[2] ? sh.found[0] : sh.found[2];
+    int32_t high = cuts ? sh.found[2] : sh.found[1];
+    if (high < low) high = low;
     each([&](int b, const Sums& at, const Sums& in) {
-        if (b == p.low) sh.above = at.count;
-        if (b == p.high) sh.upto = at.count + in.count;
+        if (b == low) sh.above = at.count;
+        if (b == high) sh.upto = at.count + in.count;
     });
     __syncthreads();
-    p.above = sh.above;
-    if (!cuts && !(s.top_p < 1.0f)) p.mode = kWhole;
-    else if (sh.upto - sh.above > (uint32_t)kList) p.mode = kAlone;
+    Plan p = plan_of(s, top, bits);
+    if (!cuts && !(s.top_p < 1.0f)) return p;
+    p.mode = sh.upto - sh.above > (uint32_t)kList ? kAlone : kCut;
+    p.top_k = cuts ? s.top_k : 0;
+    p.count = sh.above;
+    // bins as logits (a bin's number below the top one's by so many; there is none below the last of the 32 bits)
+    const float per_bin = (float)kPerUnit / s.temperature;
+    const int64_t top_bin = bin_at(top, per_bin);
+    p.above = least_logit([&](float x) { return bin_at(x, per_bin) > top_bin - low; });
+    p.listed = high == kBins ? value_of(kLeast) : least_logit([&](float x) { return bin_at(x, per_bin) >= top_bin - high; });
     return p;
 }
 
-// A part of a row: exact sums of the weights above the border's bins (`all`: of all weights), by segment of those that min_p keeps,
-// and the tokens in the border's bins, in any order.
+// A part of a row: exact sums of the weights from `above` on (`all`: of all weights, where top_p asks for them), by segment of those that
+// min_p keeps, and the tokens from `listed` up to there, in any order.
 struct Drawn {
     uint64_t all, above;
 };
 template <int DT, typename F>
-__device__ Drawn draw_part(const Row<DT>& row, const Settings& s, const Weights& w, const Plan& p, int32_t seg0, int32_t seg1, Draw& sh,
-                           Scan& scan, F segment_sum) {
+__device__ __forceinline__ Drawn draw_part(const Row<DT>& row, const Settings& s, const Weights& w, const Plan& p, int32_t seg0, int32_t seg1,
+                                           Draw& sh, Group& group, F segment_sum) {
+    constexpr int kPer = Row<DT>::kPer;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    const bool cut = p.mode == kCut, whole_sum = cut && s.top_p < 1.0f && p.top_k == 0;
-    const float per_bin = cut ? (float)kPerUnit / s.temperature : 0.0f;
-    const double least = least_of(s);
-    u32x4 v[Row<DT>::kSteps];
+    const bool whole_sum = p.mode == kCut && s.top_p < 1.0f && p.top_k == 0, min_p = s.min_p > 0.0f;
+    const float keep = fmaxf(p.keep, p.above);
     Drawn d = {0, 0};
     for (int32_t g = seg0 + wave; g < seg1; g += kWaves) {
-        uint64_t kept = 0;
-        row.load(g, lane, v);
-        row.each(g, lane, v, [&](int32_t i, float x) {
-            if (x > -__builtin_inff()) {
-                int32_t bin = cut ? p.top_bin - bin_at(x, per_bin) : -1;
-                bin = bin < kBins ? bin : kBins;
-                const bool above = !cut || bin < p.low;
-                if (above || whole_sum) {
-                    const double t = w.log2_of(x);
-                    const uint64_t weight = w.of_log2(t);
-                    d.all += weight;
-                    if (above) {
-                        d.above += weight;
-                        kept += t >= least ? weight : 0;
-                    }
+        uint64_t above = 0, kept = 0;
+        row.each(g, lane, [&](int32_t first, const float (&x)[kPer]) {
+            bool some = whole_sum, listed = false;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                some |= x[e] >= p.above;
+                listed |= x[e] < p.above && x[e] >= p.listed;
+            }
+            if (__builtin_amdgcn_ballot_w64(some)) {
+                uint64_t weight[kPer];
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) weight[e] = w.finite(x[e]);
+                if (whole_sum) {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) d.all += weight[e];
                 }
-                if (!above && bin <= p.high) {
-                    const uint32_t at = atomicAdd(&sh.listed, 1u);
-                    if (at < (uint32_t)kList) sh.list[at] = place_of(key_of(x), (uint32_t)i);
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) above += x[e] >= p.above ? weight[e] : 0;
+                if (min_p) {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) kept += x[e] >= keep ? weight[e] : 0;
                 }
             }
+            if (listed) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e)
+                    if (x[e] < p.above && x[e] >= p.listed) {
+                        const uint32_t at = atomicAdd(&sh.listed, 1u);
+                        if (at < (uint32_t)kList) sh.list[at] = place_of(key_of(x[e]), (uint32_t)(first + e));
+                    }
+            }
         });
-        kept = wave_sum64(kept);
+        d.above += above;
+        kept = last_lane(wave_upto(min_p ? kept : above));
         if (lane == 0) segment_sum(g, kept);
     }
-    Sums all;
-    scan_before({0, d.all}, all, scan);
-    d.all = all.weight;
-    scan_before({0, d.above}, all, scan);
-    d.above = all.weight;
+    d.all = group.sum(d.all);
+    d.above = group.sum(d.above);
     return d;
 }
 
-// The token of a row whose parts are together: sh.list holds `listed` tokens, sh.kept the segments' sums.
+// The token of a row whose parts are together: sh.list holds `listed` tokens, sh.kept the segments' sums.  False: the border is not in
+// its bins.
 template <int DT>
-__device__ void draw_row(const SampleArgs& a, int64_t r, const Row<DT>& row, const Settings& s, const Weights& w, int bits, const Plan& p,
-                         const Drawn& d, int32_t segments, uint32_t listed, Space& space, Scan& scan) {
-    Draw& sh = space.draw;
+__device__ bool draw_row(const SampleArgs& a, int64_t r, const Row<DT>& row, const Settings& s, const Weights& w, int bits, const Plan& p,
+                         const Drawn& d, int32_t segments, uint32_t listed, Draw& sh, Group& group) {
     const int tid = threadIdx.x;
-    const double least = least_of(s);
     uint64_t border = ~0ull;  // the last kept token in the sorted row
     if (p.mode == kCut) {
         // the list in order: a bitonic sort
@@ -615,69 +676,54 @@ __device__ void draw_row(const SampleArgs& a, int64_t r, const Row<DT>& row, con
             sh.found_weight = d.all;
         }
         __syncthreads();
-        constexpr int kOwn = kList / kThreads;
-        uint64_t own[kOwn], sum = 0;
-#pragma unroll
-        for (int k = 0; k < kOwn; ++k) {
-            const uint32_t i = tid * kOwn + k;
-            own[k] = i < listed ? w.of(~(uint32_t)(sh.list[i] >> 32)) : 0;
-            sum += own[k];
-        }
-        Sums all;
-        const uint64_t before = d.above + scan_before({0, sum}, all, scan).weight;
-        if (p.top_k) {
-            uint64_t at = before;
-#pragma unroll
-            for (int k = 0; k < kOwn; ++k) {
-                const uint32_t i = tid * kOwn + k;
-                at += own[k];
-                if (i < listed && p.above + i + 1 == (uint32_t)p.top_k) {
-                    sh.found_k = (int32_t)i;
-                    sh.found_weight = at;
-                }
+        auto weight_at = [&](uint32_t i) { return i < listed ? w.finite(value_of(~(uint32_t)(sh.list[i] >> 32))) : 0; };
+        uint64_t all;
+        if (p.top_k) {  // the sum of the first top_k
+            const uint32_t length = (uint32_t)p.top_k - p.count;
+            uint64_t at = 0;
+            for (uint32_t i = tid; i < length; i += kThreads) at += weight_at(i);
+            at = group.sum(at);
+            if (tid == 0 && length > 0 && length <= listed) {
+                sh.found_k = (int32_t)length - 1;
+                sh.found_weight = d.above + at;
             }
+            __syncthreads();
         }
-        __syncthreads();
         int32_t last = p.top_k ? sh.found_k : (int32_t)listed - 1;
         bool held = last >= 0;
         if (s.top_p < 1.0f) {
             const uint64_t goal = top_p_goal(s, sh.found_weight);
-            uint64_t at = before;
-#pragma unroll
-            for (int k = 0; k < kOwn; ++k) {
-                if (at < goal && goal <= at + own[k]) sh.found_p = tid * kOwn + k;
-                at += own[k];
+            uint64_t passed = d.above;
+#pragma nounroll
+            for (uint32_t base = 0; base < listed; base += kThreads) {
+                const uint64_t v = weight_at(base + tid), at = passed + group.before(v, all);
+                if (at < goal && goal <= at + v) sh.found_p = base + tid;
+                passed += all;
             }
             __syncthreads();
             held = held && sh.found_p >= 0;
             last = sh.found_p < last ? sh.found_p : last;
         }
-        if (!held) {  // the border is not in these bins
-            __syncthreads();
-            draw_alone<DT>(a, r, row.start(), s, p.top, bits, space.digits, scan);
-            return;
-        }
+        if (!held) return false;
         border = sh.list[last];
-#pragma unroll
-        for (int k = 0; k < kOwn; ++k) {
-            const uint32_t i = tid * kOwn + k;
-            if ((int32_t)i <= last && w.log2_of(value_of(~(uint32_t)(sh.list[i] >> 32))) >= least)
-                atomicAdd((unsigned long long*)&sh.kept[row.segment_of((uint32_t)sh.list[i])], (unsigned long long)own[k]);
+        for (uint32_t i = tid; (int32_t)i <= last; i += kThreads) {
+            const uint64_t v = weight_at(i);
+            if (value_of(~(uint32_t)(sh.list[i] >> 32)) >= p.keep)
+                atomicAdd((unsigned long long*)&sh.kept[row.segment_of((uint32_t)sh.list[i])], (unsigned long long)v);
         }
     }
     __syncthreads();
     // the segment in which the drawn number falls
     constexpr int kOwn = kSegments / kThreads;
-    uint64_t own[kOwn], sum = 0;
+    uint64_t own[kOwn], sum = 0, total;
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
         const int32_t g = tid * kOwn + k;
         own[k] = g < segments ? sh.kept[g] : 0;
         sum += own[k];
     }
-    Sums all;
-    uint64_t at = scan_before({0, sum}, all, scan).weight;
-    const uint64_t total = all.weight, goal = (uint64_t)((double)s.uniform * (double)total) + 1;  // at most total
+    uint64_t at = group.before(sum, total);
+    const uint64_t goal = (uint64_t)((double)s.uniform * (double)total) + 1;  // at most total
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
         if (at < goal && goal <= at + own[k]) {
@@ -697,20 +743,17 @@ __device__ void draw_row(const SampleArgs& a, int64_t r, const Row<DT>& row, con
     for (int k = 0; k < kEach; ++k) {
         const int32_t i = first + k;
         x[k] = i >= 0 && i < row.n ? load_logit<DT>(row.start(), i) : -__builtin_inff();
-        weight[k] = 0;
-        if (x[k] > -__builtin_inff() && place_of(key_of(x[k]), (uint32_t)i) <= border) {
-            const double t = w.log2_of(x[k]);
-            if (t >= least) weight[k] = w.of_log2(t);
-        }
+        weight[k] = x[k] >= p.keep && place_of(key_of(x[k]), (uint32_t)i) <= border ? w.finite(x[k]) : 0;
         sum += weight[k];
     }
-    at = sh.found_weight;
-    at += scan_before({0, sum}, all, scan).weight;
+    uint64_t in_segment;
+    at = sh.found_weight + group.before(sum, in_segment);
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
         if (at < goal && goal <= at + weight[k]) write_token(a, r, first + k, x[k], w, bits, total);
         at += weight[k];
     }
+    return true;
 }
 
 __device__ __forceinline__ void write_plain(const SampleArgs& a, int64_t r, int32_t token) {
@@ -727,29 +770,36 @@ __device__ __forceinline__ bool cuts(const Settings& s, int64_t vocab) {
 
 // A workgroup a row, nothing kept between its steps but in LDS.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a, int bits, int32_t segments) {
+__global__ __launch_bounds__(kThreads, 4) void sample_rows(SampleArgs a, int bits, int32_t segments) {
     __shared__ Space space;
-    __shared__ Scan scan;
+    __shared__ Group::Space shared;
+    Group group = {shared};
     const int64_t r = blockIdx.x;
     const Row<DT> row(a, r);
     const Settings s = settings_of(a, r);
     const bool histogram = cuts(s, a.vocab) && segments > 0;
-    const Part part = look_at<DT>(row, s, histogram, 0, (row.count + kSegmentVectors - 1) / kSegmentVectors, space.look, scan);
+    const Part part = look_at<DT>(row, s, histogram, 0, (row.count + kSegmentVectors - 1) / kSegmentVectors, space.look, group);
     if (part.top == -__builtin_inff()) return write_plain(a, r, -1);
     if (s.greedy) return write_plain(a, r, (int32_t)part.first);
-    Plan p = {kWhole, part.top, 0, 0, 0, 0, 0};
-    if (part.top == __builtin_inff() || segments == 0) p.mode = kAlone;
-    else if (histogram)
-        p = plan_row(s, part.top, part.valid, space.look, scan, [&](int b, uint32_t& count, float& weight) {
+    Plan p = {kAlone, 0, 0, part.top, 0.0f, 0.0f, 0.0f};
+    if (part.top == __builtin_inff() || segments == 0) {
+    } else if (!histogram) {
+        p = plan_of(s, part.top, bits);
+    } else {
+        p = plan_row(s, part.top, bits, part.valid, space.look, group, [&](int b, uint32_t& count, float& weight) {
             const uint64_t v = space.look.bins[b];
             count = (uint32_t)(v >> 40);
             weight = (float)(v & ((1ull << 40) - 1)) * 0x1p-20f;
         });
+    }
     __syncthreads();  // of the histogram
-    if (p.mode == kAlone) return draw_alone<DT>(a, r, row.start(), s, p.top, bits, space.digits, scan);
-    const Weights w = weights_of(s, p.top, bits);
-    const Drawn d = draw_part<DT>(row, s, w, p, 0, segments, space.draw, scan, [&](int32_t g, uint64_t sum) { space.draw.kept[g] = sum; });
-    draw_row<DT>(a, r, row, s, w, bits, p, d, segments, space.draw.listed, space, scan);
+    bool alone = p.mode == kAlone;
+    if (!alone) {
+        const Weights w = weights_of(s, p.top, bits);
+        const Drawn d = draw_part<DT>(row, s, w, p, 0, segments, space.draw, group, [&](int32_t g, uint64_t sum) { space.draw.kept[g] = sum; });
+        alone = !draw_row<DT>(a, r, row, s, w, bits, p, d, segments, space.draw.listed, space.draw, group);
+    }
+    if (alone) draw_alone<DT>(a, r, row.start(), s, p.top, bits, space.digits, group);
 }
 
 struct SplitArgs {
@@ -780,45 +830,48 @@ __device__ __forceinline__ T get(const T* p) {
 template <int DT>
 __global__ __launch_bounds__(kThreads) void sample_look(SplitArgs g) {
     __shared__ Look sh;
-    __shared__ Scan scan;
+    __shared__ Group::Space shared;
+    Group group = {shared};
     const SampleArgs& a = g.a;
     const int64_t r = blockIdx.x / (uint32_t)g.groups;
-    const int group = (int)(blockIdx.x % (uint32_t)g.groups), tid = threadIdx.x;
+    const int which = (int)(blockIdx.x % (uint32_t)g.groups), tid = threadIdx.x;
     const Row<DT> row(a, r);
     const Settings s = settings_of(a, r);
     const bool histogram = cuts(s, a.vocab);
-    const int32_t seg0 = group * g.per_group, seg1 = seg0 + g.per_group < g.segments ? seg0 + g.per_group : g.segments;
-    const Part part = look_at<DT>(row, s, histogram, seg0, seg1, sh, scan);
+    const int32_t seg0 = which * g.per_group, seg1 = seg0 + g.per_group < g.segments ? seg0 + g.per_group : g.segments;
+    const Part part = look_at<DT>(row, s, histogram, seg0, seg1, sh, group);
     Part* const parts = g.parts + r * g.groups;
     uint64_t* const bins = g.bins + r * g.groups * kBins;
     if (tid == 0) {
-        put(&parts[group].top, part.top);
-        put(&parts[group].first, part.first);
-        put(&parts[group].valid, part.valid);
+        put(&parts[which].top, part.top);
+        put(&parts[which].first, part.first);
+        put(&parts[which].valid, part.valid);
     }
     if (histogram)
-        for (int i = tid; i < kBins; i += kThreads) put(bins + (int64_t)group * kBins + i, sh.bins[i]);
+        for (int i = tid; i < kBins; i += kThreads) put(bins + (int64_t)which * kBins + i, sh.bins[i]);
     if (!splitk_last(g.look_arrivals + r, (uint32_t)g.groups, g.tag)) return;
 
     // groups: at most a workgroup's threads
     const float own = tid < g.groups ? get(&parts[tid].top) : -__builtin_inff();
-    const float top = block_max(own, scan);
-    Plan p = {kDone, top, 0, 0, 0, 0, 0};
+    const float top = group.max(own);
+    Plan p = {kDone, 0, 0, top, 0.0f, 0.0f, 0.0f};
     if (top == -__builtin_inff()) {
         write_plain(a, r, -1);
     } else if (s.greedy) {
-        write_plain(a, r, (int32_t)block_min(own == top ? get(&parts[tid < g.groups ? tid : 0].first) : 0xffffffffu, scan));
+        write_plain(a, r, (int32_t)group.min(own == top ? get(&parts[tid < g.groups ? tid : 0].first) : 0xffffffffu));
     } else if (top == __builtin_inff()) {
         p.mode = kAlone;
     } else if (!histogram) {
-        p.mode = kWhole;
+        p = plan_of(s, top, g.bits);
     } else {
         const float per_bin = (float)kPerUnit / s.temperature;
         // how far a part's histogram lies below the row's (one without a logit: past it)
-        if (tid < g.groups) sh.shift[tid] = own > -__builtin_inff() ? bin_at(top, per_bin) - bin_at(own, per_bin) : kBins;
-        Sums all;
-        scan_before({tid < g.groups ? get(&parts[tid].valid) : 0, 0}, all, scan);
-        p = plan_row(s, top, all.count, sh, scan, [&](int b, uint32_t& count, float& weight) {
+        if (tid < g.groups) {
+            const uint32_t lower = (uint32_t)bin_at(top, per_bin) - (uint32_t)bin_at(own, per_bin);
+            sh.shift[tid] = own > -__builtin_inff() && lower < (uint32_t)kBins ? (int32_t)lower : kBins;
+        }
+        const uint32_t valid = (uint32_t)group.sum(tid < g.groups ? get(&parts[tid].valid) : 0);  // (its barrier: the shifts are there)
+        p = plan_row(s, top, g.bits, valid, sh, group, [&](int b, uint32_t& count, float& weight) {
             count = 0;
             weight = 0.0f;
             for (int c = 0; c < g.groups; ++c) {
@@ -837,28 +890,30 @@ __global__ __launch_bounds__(kThreads) void sample_look(SplitArgs g) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void sample_draw(SplitArgs g) {
+__global__ __launch_bounds__(kThreads, 4) void sample_draw(SplitArgs g) {
     __shared__ Space space;
-    __shared__ Scan scan;
+    __shared__ Group::Space shared;
+    Group group = {shared};
     Draw& sh = space.draw;
     const SampleArgs& a = g.a;
     const int64_t r = blockIdx.x / (uint32_t)g.groups;
-    const int group = (int)(blockIdx.x % (uint32_t)g.groups), tid = threadIdx.x;
+    const int which = (int)(blockIdx.x % (uint32_t)g.groups), tid = threadIdx.x;
     const Plan p = g.plans[r];
-    if (p.mode == kDone || (p.mode == kAlone && group > 0)) return;
+    if (p.mode == kDone || (p.mode == kAlone && which > 0)) return;
     const Row<DT> row(a, r);
     const Settings s = settings_of(a, r);
-    if (p.mode == kAlone) return draw_alone<DT>(a, r, row.start(), s, p.top, g.bits, space.digits, scan);
+    bool alone = p.mode == kAlone;
+    if (!alone) {
     const Weights w = weights_of(s, p.top, g.bits);
-    const int32_t seg0 = group * g.per_group, seg1 = seg0 + g.per_group < g.segments ? seg0 + g.per_group : g.segments;
+    const int32_t seg0 = which * g.per_group, seg1 = seg0 + g.per_group < g.segments ? seg0 + g.per_group : g.segments;
     uint64_t* const kept = g.kept + r * g.segments;
     uint64_t* const list = g.list + r * kList;
     Drawn* const sums = g.sums + r * g.groups;
-    Drawn d = draw_part<DT>(row, s, w, p, seg0, seg1, sh, scan, [&](int32_t at, uint64_t sum) { put(kept + at, sum); });
+    Drawn d = draw_part<DT>(row, s, w, p, seg0, seg1, sh, group, [&](int32_t at, uint64_t sum) { put(kept + at, sum); });
     const uint32_t own = sh.listed < (uint32_t)kList ? sh.listed : kList;
     if (tid == 0) {
-        put(&sums[group].all, d.all);
-        put(&sums[group].above, d.above);
+        put(&sums[which].all, d.all);
+        put(&sums[which].above, d.above);
         sh.base = own ? __hip_atomic_fetch_add(g.listed + r, own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
     }
     __syncthreads();
@@ -870,12 +925,11 @@ __global__ __launch_bounds__(kThreads) void sample_draw(SplitArgs g) {
     listed = listed < (uint32_t)kList ? listed : kList;
     for (uint32_t i = tid; i < listed; i += kThreads) sh.list[i] = get(list + i);
     for (int32_t i = tid; i < g.segments; i += kThreads) sh.kept[i] = get(kept + i);
-    Sums all;
-    scan_before({0, tid < g.groups ? get(&sums[tid].all) : 0}, all, scan);
-    d.all = all.weight;
-    scan_before({0, tid < g.groups ? get(&sums[tid].above) : 0}, all, scan);
-    d.above = all.weight;
-    draw_row<DT>(a, r, row, s, w, g.bits, p, d, g.segments, listed, space, scan);
+    d.all = group.sum(tid < g.groups ? get(&sums[tid].all) : 0);
+    d.above = group.sum(tid < g.groups ? get(&sums[tid].above) : 0);
+    alone = !draw_row<DT>(a, r, row, s, w, g.bits, p, d, g.segments, listed, sh, group);
+    }
+    if (alone) draw_alone<DT>(a, r, row.start(), s, p.top, g.bits, space.digits, group);
 }
 
 // ---------------------------------------------------------------- host
