@@ -20,13 +20,13 @@
 namespace qk {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;      // of the histograms
 constexpr int kPerUnit = 64;     // bins per temperature
 constexpr float kSlope = 0.0155038f;  // 1 - e^(-1 / 64): what a weight falls in a bin
 constexpr int kList = 4096;      // tokens in the border's bins
-constexpr int kSegmentVectors = 256;
+constexpr int kBatch = 4;        // 16-byte vectors that a lane asks for at a time
 constexpr int kSegments = 1024;  // of a row at most
 constexpr int64_t kMostTokens = 1 << 20;  // of a row that is split: a bin's count and weight share 64 bits
 
@@ -144,8 +144,10 @@ struct Group {
         return sum;
     }
     __device__ __forceinline__ uint64_t sum(uint64_t v) {
-        uint64_t all;
-        before(v, all);
+        const uint64_t* const of = exchange(last_lane(wave_upto(v)), (threadIdx.x & 63) == 0);
+        uint64_t all = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) all += of[w];
         return all;
     }
     __device__ __forceinline__ float max(float v) {
@@ -342,56 +344,72 @@ __device__ __forceinline__ void draw_alone(const SampleArgs& a, int64_t r, const
 // ---------------------------------------------------------------- look and draw
 
 // A row as vectors of 16 aligned bytes: token i is element i + offset of them.  (Elements of the first and the last vector that are
-// not the row's are read, and not used: a vector with one byte of a row lies in memory as a whole.)
-template <int DT>
+// not the row's are read, and not used: a vector with one byte of a row lies in memory as a whole.)  A segment is STEPS vectors of
+// each lane of a wave: what one sum is kept of.
+template <int DT, int STEPS>
 struct Row {
-    static constexpr int kPer = DT == QK_F32 ? 4 : 8;
-    static constexpr int kSteps = kSegmentVectors / 64;
+    static constexpr int kType = DT, kSize = DT == QK_F32 ? 4 : 2, kPer = 16 / kSize;
+    static constexpr int kSegment = STEPS * 64 * kPer;  // elements
     const u32x4* vectors;
     int32_t offset, n, count;  // count: of vectors
 
-    __device__ __forceinline__ const void* start() const {
-        return (const char*)vectors + offset * (DT == QK_F32 ? 4 : 2);
-    }
-
     __device__ __forceinline__ Row(const SampleArgs& a, int64_t r) {
-        constexpr int kSize = DT == QK_F32 ? 4 : 2;
         const uintptr_t at = (uintptr_t)a.x + r * a.row_stride * kSize;
         vectors = (const u32x4*)(at & ~(uintptr_t)15);
         offset = (int32_t)(at & 15) / kSize;
         n = (int32_t)a.vocab;
         count = (n + offset + kPer - 1) / kPer;
     }
-    // f(first token, logits) for a lane's vectors of a segment, -inf for what is not the row's
-    template <typename F>
-    __device__ __forceinline__ void each(int32_t segment, int lane, F f) const {
-        u32x4 v[kSteps];
+    __device__ __forceinline__ const void* start() const { return (const char*)vectors + offset * kSize; }
+    __device__ __forceinline__ int32_t segments() const { return (count + STEPS * 64 - 1) / (STEPS * 64); }
+    __device__ __forceinline__ int32_t segment_of(uint32_t token) const { return (int32_t)(token + offset) / kSegment; }
+
+    // This wave's segments of those from seg0 on: f(first token, logits) for each of a lane's vectors, -inf for what is not the row's, and
+    // end(segment) behind each segment.  The next vectors are on their way while some are worked on; the loop over those is not
+    // written out, as a workgroup runs it a few times only and fetching its code would cost more.
+    template <typename F, typename E>
+    __device__ __forceinline__ void each(int32_t seg0, int32_t seg1, F f, E end) const {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int32_t steps = (seg1 - seg0 - wave + kWaves - 1) / kWaves * STEPS;
+        auto segment = [&](int32_t q) { return seg0 + wave + kWaves * (q / STEPS); };
+        auto vector = [&](int32_t q) { return (segment(q) * STEPS + q % STEPS) * 64 + lane; };
+        auto load = [&](int32_t q, u32x4 (&v)[kBatch]) {
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            const int32_t at = segment * kSegmentVectors + k * 64 + lane;
-            v[k] = vectors[at < count ? at : 0];
-        }
-        const bool inside = segment * kSegmentVectors * kPer >= offset && (segment + 1) * kSegmentVectors * kPer - offset <= n;
-        // (the vectors move up instead of the loop being written out: a workgroup runs it a few times, and fetching its code costs more)
+            for (int k = 0; k < kBatch; ++k) {
+                const int32_t at = vector(q + k);
+                v[k] = vectors[q + k < steps && at < count ? at : 0];
+            }
+        };
+        u32x4 v[kBatch], next[kBatch];
+        load(0, next);
+        for (int32_t q0 = 0; q0 < steps; q0 += kBatch) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) v[k] = next[k];
+            if (q0 + kBatch < steps) load(q0 + kBatch, next);
 #pragma nounroll
-        for (int k = 0; k < kSteps; ++k) {
-            const int32_t first = (segment * kSegmentVectors + k * 64 + lane) * kPer - offset;
-            float x[kPer];
+            for (int32_t q = q0; q < q0 + kBatch && q < steps; ++q) {
+                const int32_t at = vector(q), first = at * kPer - offset, g = segment(q);
+                float x[kPer];
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                if constexpr (DT == QK_F32) x[e] = __uint_as_float(v[0][e]);
-                else x[e] = load_half_bits(v[0][e >> 1] >> (16 * (e & 1)) & 0xffffu, DT);
+                for (int e = 0; e < kPer; ++e) {
+                    if constexpr (DT == QK_F32) x[e] = __uint_as_float(v[0][e]);
+                    else x[e] = load_half_bits(v[0][e >> 1] >> (16 * (e & 1)) & 0xffffu, DT);
+                }
+#pragma unroll
+                for (int k = 1; k < kBatch; ++k) v[k - 1] = v[k];
+                if (!(g * kSegment >= offset && (g + 1) * kSegment - offset <= n)) {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) x[e] = (uint32_t)(first + e) < (uint32_t)n ? x[e] : -__builtin_inff();
+                }
+                f(first, x);
+                if (q % STEPS == STEPS - 1) end(g);
             }
-#pragma unroll
-            for (int i = 1; i < kSteps; ++i) v[i - 1] = v[i];
-            if (!inside) {
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) x[e] = (uint32_t)(first + e) < (uint32_t)n ? x[e] : -__builtin_inff();
-            }
-            f(first, x);
         }
     }
-    __device__ __forceinline__ int32_t segment_of(uint32_t token) const { return (int32_t)(token + offset) / (kPer * kSegmentVectors); }
+    template <typename F>
+    __device__ __forceinline__ void each(int32_t seg0, int32_t seg1, F f) const {
+        each(seg0, seg1, f, [](int32_t) {});
+    }
 };
 
 // The number of a logit's bin, cut to 32 bits: it rises with the logit, as every step of it does.
@@ -400,14 +418,23 @@ __device__ __forceinline__ int32_t bin_at(float x, float per_bin) {
     asm("v_cvt_flr_i32_f32 %0, %1" : "=v"(at) : "v"(x * per_bin));
     return at;
 }
-// The least logit for which `is` holds, which does not hold again below it; +inf where it holds for no finite one.  A wave's lanes
-// try 64 at a time.
+// The least logit for which `is` holds, which holds for all above it; +inf where it holds for no finite one.  A wave's lanes
+// try 64 at a time, first those around `guess`.
 template <typename F>
-__device__ __forceinline__ float least_logit(F is) {
-    uint32_t low = kLeast, high = 0xff800000u;  // of -FLT_MAX and of +inf
+__device__ __forceinline__ float least_logit(float guess, F is) {
+    constexpr uint32_t kMost = 0xff800000u;  // +inf
+    uint32_t low = kLeast, high = kMost, at = key_of(guess);
+    if (at >= kLeast + 64 && at <= kMost - 64) {
+        at = at - 32 + (threadIdx.x & 63);
+        const uint64_t held = __builtin_amdgcn_ballot_w64(is(value_of(at)));
+        at = __builtin_amdgcn_readfirstlane((int)at);
+        const int first = held ? __builtin_ctzll(held) : 64;
+        if (first > 0) low = at + first;
+        if (first < 64) high = at + first;
+    }
     while (low < high) {
         const uint32_t step = (high - low + 63) / 64;
-        uint32_t at = low + (threadIdx.x & 63) * step;
+        at = low + (threadIdx.x & 63) * step;
         at = at < high ? at : high;
         const uint64_t held = __builtin_amdgcn_ballot_w64(at == high || is(value_of(at)));
         const int first = held ? __builtin_ctzll(held) : 64;
@@ -417,6 +444,8 @@ __device__ __forceinline__ float least_logit(F is) {
     }
     return value_of(__builtin_amdgcn_readfirstlane((int)low));
 }
+// Bins per unit of a logit (near enough to 64 / temperature; the same wherever it is asked for)
+__device__ __forceinline__ float bins_per_logit(const Settings& s) { return (float)kPerUnit * __builtin_amdgcn_rcpf(s.temperature); }
 
 // What the look at a row found: it is done (greedy, or nothing to draw), it is done by one workgroup, no filter cuts it, or the border of
 // the kept tokens lies among the logits from `listed` to `above`, at which those begin that are kept for certain, `count` of them;
@@ -435,7 +464,7 @@ struct Part {
 };
 
 struct Look {
-    uint64_t bins[kBins];  // count << 40 | weight
+    uint64_t bins[kBins + 64];  // count << 40 | weight; behind them, a place for each lane: of what has no bin
     int32_t shift[kThreads];
     int32_t found[3];      // bins: the borders in the weights, from below and from above, and in the count
     uint64_t weight[2];
@@ -456,45 +485,45 @@ union Space {
 
 // A part of a row: its largest logit and, where a filter cuts, its histogram.  Weights there are in units of that of the bin's upper
 // end, and near enough: they only have to lead to the border.
-template <int DT>
-__device__ Part look_at(const Row<DT>& row, const Settings& s, bool histogram, int32_t seg0, int32_t seg1, Look& sh, Group& group) {
-    constexpr int kPer = Row<DT>::kPer;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <typename R>
+__device__ __forceinline__ Part look_at(const R& row, const Settings& s, bool histogram, int32_t seg0, int32_t seg1, Look& sh, Group& group) {
+    constexpr int kPer = R::kPer;
     Part part = {-__builtin_inff(), 0xffffffffu, 0};
-    for (int32_t g = seg0 + wave; g < seg1; g += kWaves)
-        row.each(g, lane, [&](int32_t, const float (&x)[kPer]) {
+    row.each(seg0, seg1, [&](int32_t, const float (&x)[kPer]) {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) part.top = fmaxf(part.top, x[e]);
-        });
+        for (int e = 0; e < kPer; ++e) part.top = fmaxf(part.top, x[e]);
+    });
     if (histogram)
         for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
     part.top = group.max(part.top);
     if (s.greedy) {
-        for (int32_t g = seg0 + wave; g < seg1; g += kWaves)
-            row.each(g, lane, [&](int32_t first, const float (&x)[kPer]) {
+        row.each(seg0, seg1, [&](int32_t first, const float (&x)[kPer]) {
 #pragma unroll
-                for (int e = 0; e < kPer; ++e)
-                    if (x[e] == part.top && (uint32_t)(first + e) < part.first) part.first = first + e;
-            });
+            for (int e = 0; e < kPer; ++e)
+                if (x[e] == part.top && (uint32_t)(first + e) < part.first) part.first = first + e;
+        });
         part.first = group.min(part.first);
     }
     if (histogram) {
-        const float per_bin = (float)kPerUnit / s.temperature;
+        const float per_bin = bins_per_logit(s);
         const int32_t top_bin = bin_at(part.top, per_bin);
-        for (int32_t g = seg0 + wave; g < seg1; g += kWaves)
-            row.each(g, lane, [&](int32_t, const float (&x)[kPer]) {
+        const uint32_t past = kBins + (threadIdx.x & 63);
+        uint32_t seen = 0, none = 0;  // of this wave
+        row.each(seg0, seg1, [&](int32_t, const float (&x)[kPer]) {
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    const bool valid = x[e] > -__builtin_inff();
-                    part.valid += valid;
-                    const uint32_t bin = (uint32_t)top_bin - (uint32_t)bin_at(x[e], per_bin);
-                    // e^-z, z = (1 - f) / 64: on the line that passes it by 2^-15 at most
-                    const float f = __builtin_amdgcn_fractf(x[e] * per_bin);
-                    if (valid && bin < (uint32_t)kBins)
-                        atomicAdd((unsigned long long*)&sh.bins[bin], 1ull << 40 | (uint32_t)__builtin_fmaf(f, 0x1p20f * kSlope, 0x1p20f * (0.99998f - kSlope)));
-                }
-            });
-        part.valid = (uint32_t)group.sum(part.valid);  // (its barrier: the histogram is whole behind it)
+            for (int e = 0; e < kPer; ++e) {
+                // (-inf and NaN come to the least number there is)
+                const float v = fmaxf(x[e], -__builtin_inff());
+                none += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v == -__builtin_inff()));
+                const uint32_t below = (uint32_t)top_bin - (uint32_t)bin_at(v, per_bin), bin = below < past ? below : past;
+                // e^-z, z = (1 - f) / 64: on the line that passes it by 2^-15 at most
+                const float f = __builtin_amdgcn_fractf(v * per_bin);
+                atomicAdd((unsigned long long*)&sh.bins[bin], 1ull << 40 | (uint32_t)__builtin_fmaf(f, 0x1p20f * kSlope, 0x1p20f * (0.99998f - kSlope)));
+            }
+            seen += 64 * kPer;
+        });
+        // (the barrier: the histogram is whole behind it)
+        part.valid = (uint32_t)group.sum((threadIdx.x & 63) == 0 ? seen - none : 0);
     }
     return part;
 }
@@ -505,7 +534,7 @@ __device__ __forceinline__ Plan plan_of(const Settings& s, float top, int bits) 
     if (s.min_p > 0.0f) {
         const Weights w = weights_of(s, top, bits);
         const double least = least_of(s);
-        p.keep = least_logit([&](float x) { return w.finite_log2(x) >= least; });
+        p.keep = least_logit(top + s.temperature * (float)least * 0.693147181f, [&](float x) { return w.finite_log2(x) >= least; });
     }
     return p;
 }
@@ -579,14 +608,17 @@ __device__ Plan plan_row(const Settings& s, float top, int bits, uint32_t valid,
     __syncthreads();
     Plan p = plan_of(s, top, bits);
     if (!cuts && !(s.top_p < 1.0f)) return p;
-    p.mode = sh.upto - sh.above > (uint32_t)kList ? kAlone : kCut;
+    // (at the end of the numbers there is, -inf shares a bin with logits)
+    const float per_bin = bins_per_logit(s);
+    const int64_t top_bin = bin_at(top, per_bin);
+    p.mode = sh.upto - sh.above > (uint32_t)kList || top_bin < -(1 << 30) ? kAlone : kCut;
     p.top_k = cuts ? s.top_k : 0;
     p.count = sh.above;
     // bins as logits (a bin's number below the top one's by so many; there is none below the last of the 32 bits)
-    const float per_bin = (float)kPerUnit / s.temperature;
-    const int64_t top_bin = bin_at(top, per_bin);
-    p.above = least_logit([&](float x) { return bin_at(x, per_bin) > top_bin - low; });
-    p.listed = high == kBins ? value_of(kLeast) : least_logit([&](float x) { return bin_at(x, per_bin) >= top_bin - high; });
+    const float per = s.temperature * (1.0f / kPerUnit);
+    p.above = least_logit((float)(top_bin - low + 1) * per, [&](float x) { return bin_at(x, per_bin) > top_bin - low; });
+    p.listed = high == kBins ? value_of(kLeast)
+                             : least_logit((float)(top_bin - high) * per, [&](float x) { return bin_at(x, per_bin) >= top_bin - high; });
     return p;
 }
 
@@ -595,19 +627,19 @@ __device__ Plan plan_row(const Settings& s, float top, int bits, uint32_t valid,
 struct Drawn {
     uint64_t all, above;
 };
-template <int DT, typename F>
-__device__ __forceinline__ Drawn draw_part(const Row<DT>& row, const Settings& s, const Weights& w, const Plan& p, int32_t seg0, int32_t seg1,
-                                           Draw& sh, Group& group, F segment_sum) {
-    constexpr int kPer = Row<DT>::kPer;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <typename R, typename F>
+__device__ __forceinline__ Drawn draw_part(const R& row, const Settings& s, const Weights& w, const Plan& p, int32_t seg0, int32_t seg1, Draw& sh,
+                                           Group& group, F segment_sum) {
+    constexpr int kPer = R::kPer;
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     const bool whole_sum = p.mode == kCut && s.top_p < 1.0f && p.top_k == 0, min_p = s.min_p > 0.0f;
     const float keep = fmaxf(p.keep, p.above);
     Drawn d = {0, 0};
-    for (int32_t g = seg0 + wave; g < seg1; g += kWaves) {
-        uint64_t above = 0, kept = 0;
-        row.each(g, lane, [&](int32_t first, const float (&x)[kPer]) {
+    uint64_t above = 0, kept = 0;
+    row.each(
+        seg0, seg1,
+        [&](int32_t first, const float (&x)[kPer]) {
             bool some = whole_sum, listed = false;
 #pragma unroll
             for (int e = 0; e < kPer; ++e) {
@@ -637,40 +669,117 @@ __device__ __forceinline__ Drawn draw_part(const Row<DT>& row, const Settings& s
                         if (at < (uint32_t)kList) sh.list[at] = place_of(key_of(x[e]), (uint32_t)(first + e));
                     }
             }
+        },
+        [&](int32_t g) {
+            const uint64_t sum = last_lane(wave_upto(min_p ? kept : above));
+            if ((threadIdx.x & 63) == 0) segment_sum(g, sum);
+            d.above += above;
+            above = kept = 0;
         });
-        d.above += above;
-        kept = last_lane(wave_upto(min_p ? kept : above));
-        if (lane == 0) segment_sum(g, kept);
+    if (p.mode == kCut) {
+        d.all = whole_sum ? group.sum(d.all) : 0;
+        d.above = group.sum(d.above);
+    } else {
+        __syncthreads();
     }
-    d.all = group.sum(d.all);
-    d.above = group.sum(d.above);
     return d;
+}
+
+// v of lane ^ M
+template <int M>
+__device__ __forceinline__ uint32_t across(uint32_t v) {
+    if constexpr (M == 32) {
+        const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (threadIdx.x & 32) ? a[0] : a[1];
+    } else if constexpr (M == 16) {
+        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (threadIdx.x & 16) ? a[0] : a[1];
+    } else if constexpr (M == 8) {
+        return __builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false);
+    } else if constexpr (M == 4) {  // lane ^ 7, then ^ 3
+        return __builtin_amdgcn_update_dpp(0, __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false), 0x1b, 0xf, 0xf, false);
+    } else {
+        return __builtin_amdgcn_update_dpp(0, (int)v, M == 2 ? 0x4e : 0xb1, 0xf, 0xf, false);
+    }
+}
+// A step of a bitonic sort between lanes: the lower of the pair gets the smaller value where `up`.
+template <int M>
+__device__ __forceinline__ void sort_step(uint64_t& v, bool up) {
+    const uint64_t o = (uint64_t)across<M>((uint32_t)(v >> 32)) << 32 | across<M>((uint32_t)v);
+    const bool smaller = ((threadIdx.x & M) == 0) == up;
+    v = (o < v) == smaller ? o : v;
+}
+// Sorts list[0 .. n), n up to N * kThreads: value k of a thread is k * kThreads + its number.  Steps between lanes and between a thread's
+// own values are made in registers, those between waves through the list; what lies between n and the next power of two is overwritten.
+template <int N>
+__device__ __forceinline__ void sort_values(uint64_t* list, uint32_t n) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t size = 2;
+    while (size < n) size *= 2;
+    uint64_t v[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = k * kThreads + tid < n ? list[k * kThreads + tid] : ~0ull;
+    for (uint32_t run = 2; run <= size; run *= 2) {
+        auto up = [&](int k) { return ((k * kThreads + tid) & run) == 0; };
+#pragma unroll
+        for (int apart = N / 2; apart > 0; apart /= 2)
+            if (run >= 2u * apart * kThreads) {
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    if (!(k & apart)) {
+                        const uint64_t a = v[k], b = v[k + apart];
+                        const bool swap = (b < a) == up(k);
+                        v[k] = swap ? b : a;
+                        v[k + apart] = swap ? a : b;
+                    }
+            }
+#pragma nounroll
+        for (uint32_t step = run / 2 < kThreads / 2 ? run / 2 : kThreads / 2; step >= 64; step /= 2) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (tid < size) list[k * kThreads + tid] = v[k];
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (tid < size) {
+                    const uint64_t o = list[k * kThreads + (tid ^ step)];
+                    v[k] = (o < v[k]) == (((tid & step) == 0) == up(k)) ? o : v[k];
+                }
+        }
+        if ((tid & ~63u) >= size) continue;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (run >= 64) sort_step<32>(v[k], up(k));
+            if (run >= 32) sort_step<16>(v[k], up(k));
+            if (run >= 16) sort_step<8>(v[k], up(k));
+            if (run >= 8) sort_step<4>(v[k], up(k));
+            if (run >= 4) sort_step<2>(v[k], up(k));
+            sort_step<1>(v[k], up(k));
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        if (tid < size) list[k * kThreads + tid] = v[k];
+    __syncthreads();
+}
+__device__ __forceinline__ void sort_list(uint64_t* list, uint32_t n) {
+    static_assert(kList == 4 * kThreads, "");
+    if (n <= (uint32_t)kThreads) sort_values<1>(list, n);
+    else if (n <= 2u * kThreads) sort_values<2>(list, n);
+    else sort_values<4>(list, n);
 }
 
 // The token of a row whose parts are together: sh.list holds `listed` tokens, sh.kept the segments' sums.  False: the border is not in
 // its bins.
-template <int DT>
-__device__ bool draw_row(const SampleArgs& a, int64_t r, const Row<DT>& row, const Settings& s, const Weights& w, int bits, const Plan& p,
+template <typename R>
+__device__ __forceinline__ bool draw_row(const SampleArgs& a, int64_t r, const R& row, const Settings& s, const Weights& w, int bits, const Plan& p,
                          const Drawn& d, int32_t segments, uint32_t listed, Draw& sh, Group& group) {
     const int tid = threadIdx.x;
     uint64_t border = ~0ull;  // the last kept token in the sorted row
     if (p.mode == kCut) {
-        // the list in order: a bitonic sort
-        uint32_t size = 2;
-        while (size < listed) size *= 2;
-        for (uint32_t i = listed + tid; i < size; i += kThreads) sh.list[i] = ~0ull;
-        for (uint32_t run = 2; run <= size; run *= 2)
-            for (uint32_t step = run / 2; step > 0; step /= 2) {
-                __syncthreads();
-                for (uint32_t i = tid; i < size / 2; i += kThreads) {
-                    const uint32_t x = 2 * i - (i & (step - 1)), y = x + step;
-                    const uint64_t l = sh.list[x], h = sh.list[y];
-                    if ((l > h) == ((x & run) == 0)) {
-                        sh.list[x] = h;
-                        sh.list[y] = l;
-                    }
-                }
-            }
+        sort_list(sh.list, listed);
         if (tid == 0) {
             sh.found_k = sh.found_p = -1;
             sh.found_weight = d.all;
@@ -734,15 +843,15 @@ __device__ bool draw_row(const SampleArgs& a, int64_t r, const Row<DT>& row, con
     }
     __syncthreads();
     // and the token there
-    constexpr int kEach = kSegmentVectors * Row<DT>::kPer / kThreads;
-    const int32_t first = sh.segment * kSegmentVectors * Row<DT>::kPer + tid * kEach - row.offset;
+    constexpr int kEach = R::kSegment < kThreads ? 1 : R::kSegment / kThreads;
+    const int32_t first = tid * kEach < R::kSegment ? sh.segment * R::kSegment + tid * kEach - row.offset : row.n;
     float x[kEach];
     uint64_t weight[kEach];
     sum = 0;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
         const int32_t i = first + k;
-        x[k] = i >= 0 && i < row.n ? load_logit<DT>(row.start(), i) : -__builtin_inff();
+        x[k] = i >= 0 && i < row.n ? load_logit<R::kType>(row.start(), i) : -__builtin_inff();
         weight[k] = x[k] >= p.keep && place_of(key_of(x[k]), (uint32_t)i) <= border ? w.finite(x[k]) : 0;
         sum += weight[k];
     }
@@ -769,16 +878,16 @@ __device__ __forceinline__ bool cuts(const Settings& s, int64_t vocab) {
 // ---------------------------------------------------------------- kernels
 
 // A workgroup a row, nothing kept between its steps but in LDS.
-template <int DT>
+template <int DT, int STEPS>
 __global__ __launch_bounds__(kThreads, 4) void sample_rows(SampleArgs a, int bits, int32_t segments) {
     __shared__ Space space;
     __shared__ Group::Space shared;
     Group group = {shared};
     const int64_t r = blockIdx.x;
-    const Row<DT> row(a, r);
+    const Row<DT, STEPS> row(a, r);
     const Settings s = settings_of(a, r);
     const bool histogram = cuts(s, a.vocab) && segments > 0;
-    const Part part = look_at<DT>(row, s, histogram, 0, (row.count + kSegmentVectors - 1) / kSegmentVectors, space.look, group);
+    const Part part = look_at(row, s, histogram, 0, row.segments(), space.look, group);
     if (part.top == -__builtin_inff()) return write_plain(a, r, -1);
     if (s.greedy) return write_plain(a, r, (int32_t)part.first);
     Plan p = {kAlone, 0, 0, part.top, 0.0f, 0.0f, 0.0f};
@@ -796,8 +905,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_rows(SampleArgs a, int bit
     bool alone = p.mode == kAlone;
     if (!alone) {
         const Weights w = weights_of(s, p.top, bits);
-        const Drawn d = draw_part<DT>(row, s, w, p, 0, segments, space.draw, group, [&](int32_t g, uint64_t sum) { space.draw.kept[g] = sum; });
-        alone = !draw_row<DT>(a, r, row, s, w, bits, p, d, segments, space.draw.listed, space.draw, group);
+        const Drawn d = draw_part(row, s, w, p, 0, segments, space.draw, group, [&](int32_t g, uint64_t sum) { space.draw.kept[g] = sum; });
+        alone = !draw_row(a, r, row, s, w, bits, p, d, segments, space.draw.listed, space.draw, group);
     }
     if (alone) draw_alone<DT>(a, r, row.start(), s, p.top, bits, space.digits, group);
 }
@@ -827,7 +936,7 @@ __device__ __forceinline__ T get(const T* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-template <int DT>
+template <int DT, int STEPS>
 __global__ __launch_bounds__(kThreads) void sample_look(SplitArgs g) {
     __shared__ Look sh;
     __shared__ Group::Space shared;
@@ -835,11 +944,11 @@ __global__ __launch_bounds__(kThreads) void sample_look(SplitArgs g) {
     const SampleArgs& a = g.a;
     const int64_t r = blockIdx.x / (uint32_t)g.groups;
     const int which = (int)(blockIdx.x % (uint32_t)g.groups), tid = threadIdx.x;
-    const Row<DT> row(a, r);
+    const Row<DT, STEPS> row(a, r);
     const Settings s = settings_of(a, r);
     const bool histogram = cuts(s, a.vocab);
     const int32_t seg0 = which * g.per_group, seg1 = seg0 + g.per_group < g.segments ? seg0 + g.per_group : g.segments;
-    const Part part = look_at<DT>(row, s, histogram, seg0, seg1, sh, group);
+    const Part part = look_at(row, s, histogram, seg0, seg1, sh, group);
     Part* const parts = g.parts + r * g.groups;
     uint64_t* const bins = g.bins + r * g.groups * kBins;
     if (tid == 0) {
@@ -864,7 +973,7 @@ __global__ __launch_bounds__(kThreads) void sample_look(SplitArgs g) {
     } else if (!histogram) {
         p = plan_of(s, top, g.bits);
     } else {
-        const float per_bin = (float)kPerUnit / s.temperature;
+        const float per_bin = bins_per_logit(s);
         // how far a part's histogram lies below the row's (one without a logit: past it)
         if (tid < g.groups) {
             const uint32_t lower = (uint32_t)bin_at(top, per_bin) - (uint32_t)bin_at(own, per_bin);
@@ -889,7 +998,7 @@ __global__ __launch_bounds__(kThreads) void sample_look(SplitArgs g) {
     }
 }
 
-template <int DT>
+template <int DT, int STEPS>
 __global__ __launch_bounds__(kThreads, 4) void sample_draw(SplitArgs g) {
     __shared__ Space space;
     __shared__ Group::Space shared;
@@ -900,7 +1009,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SplitArgs g) {
     const int which = (int)(blockIdx.x % (uint32_t)g.groups), tid = threadIdx.x;
     const Plan p = g.plans[r];
     if (p.mode == kDone || (p.mode == kAlone && which > 0)) return;
-    const Row<DT> row(a, r);
+    const Row<DT, STEPS> row(a, r);
     const Settings s = settings_of(a, r);
     bool alone = p.mode == kAlone;
     if (!alone) {
@@ -909,7 +1018,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SplitArgs g) {
     uint64_t* const kept = g.kept + r * g.segments;
     uint64_t* const list = g.list + r * kList;
     Drawn* const sums = g.sums + r * g.groups;
-    Drawn d = draw_part<DT>(row, s, w, p, seg0, seg1, sh, group, [&](int32_t at, uint64_t sum) { put(kept + at, sum); });
+    Drawn d = draw_part(row, s, w, p, seg0, seg1, sh, group, [&](int32_t at, uint64_t sum) { put(kept + at, sum); });
     const uint32_t own = sh.listed < (uint32_t)kList ? sh.listed : kList;
     if (tid == 0) {
         put(&sums[which].all, d.all);
@@ -927,7 +1036,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SplitArgs g) {
     for (int32_t i = tid; i < g.segments; i += kThreads) sh.kept[i] = get(kept + i);
     d.all = group.sum(tid < g.groups ? get(&sums[tid].all) : 0);
     d.above = group.sum(tid < g.groups ? get(&sums[tid].above) : 0);
-    alone = !draw_row<DT>(a, r, row, s, w, g.bits, p, d, g.segments, listed, sh, group);
+    alone = !draw_row(a, r, row, s, w, g.bits, p, d, g.segments, listed, sh, group);
     }
     if (alone) draw_alone<DT>(a, r, row.start(), s, p.top, g.bits, space.digits, group);
 }
@@ -941,25 +1050,30 @@ int weight_bits(int64_t vocab) {
     return 62 - bits < 50 ? 62 - bits : 50;
 }
 
-// Workgroups that a call should have: rows are cut until there are so many.
-constexpr int64_t kWanted = 512;
+// A row is split over workgroups where that makes three parts at least of each and the parts fill the card once: two launches and
+// their joins cost what a workgroup needs for some 30000 tokens.
+constexpr int64_t kWanted = 256, kLeastGroups = 3;
+
+// Rows up to so many tokens have short segments: their few vectors spread over more waves.
+constexpr int64_t kShortRow = 65536;
 
 struct Split {
+    bool small;
     int32_t segments, per_group;
     int64_t groups;
     int64_t arrivals, plans, listed, parts, bins, sums, kept, list, bytes;  // offsets in the workspace
 };
 Split split(int64_t rows, int64_t vocab, int dtype) {
     Split p = {};
-    const int64_t per = dtype == QK_F32 ? 4 : 8;
+    p.small = vocab <= kShortRow;
+    p.groups = 1;
+    if (vocab > kMostTokens - 8) return p;
+    const int64_t per = dtype == QK_F32 ? 4 : 8, segment = 64 * (p.small ? 1 : kBatch);
     const int64_t most = (vocab + per - 1 + per - 1) / per;  // vectors of a row that begins with the last element of one
-    if (vocab > kMostTokens - 8) {
-        p.groups = 1;
-        return p;
-    }
-    p.segments = (int32_t)((most + kSegmentVectors - 1) / kSegmentVectors);
+    p.segments = (int32_t)((most + segment - 1) / segment);
     const int64_t steps = (p.segments + kWaves - 1) / kWaves;  // of a workgroup that has all
-    int64_t groups = (kWanted + rows - 1) / rows;
+    int64_t groups = kWanted / rows;
+    if (groups < kLeastGroups) return p;
     groups = groups < steps ? groups : steps;
     p.per_group = (int32_t)((steps + groups - 1) / groups) * kWaves;
     p.groups = (p.segments + p.per_group - 1) / p.per_group;
@@ -980,12 +1094,11 @@ Split split(int64_t rows, int64_t vocab, int dtype) {
     return p;
 }
 
-template <int DT>
-hipError_t launch(const SampleArgs& a, void* workspace, hipStream_t stream) {
-    const Split p = split(a.rows, a.vocab, a.dtype);
+template <int DT, int STEPS>
+hipError_t launch_steps(const SampleArgs& a, const Split& p, void* workspace, hipStream_t stream) {
     const int bits = weight_bits(a.vocab);
     if (p.groups == 1) {
-        sample_rows<DT><<<dim3((unsigned)a.rows), kThreads, 0, stream>>>(a, bits, p.segments);
+        sample_rows<DT, STEPS><<<dim3((unsigned)a.rows), kThreads, 0, stream>>>(a, bits, p.segments);
         return hipGetLastError();
     }
     char* const ws = (char*)workspace;
@@ -1006,11 +1119,16 @@ hipError_t launch(const SampleArgs& a, void* workspace, hipStream_t stream) {
     g.kept = (uint64_t*)(ws + p.kept);
     g.list = (uint64_t*)(ws + p.list);
     const dim3 grid((unsigned)(a.rows * p.groups));
-    sample_look<DT><<<grid, kThreads, 0, stream>>>(g);
+    sample_look<DT, STEPS><<<grid, kThreads, 0, stream>>>(g);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    sample_draw<DT><<<grid, kThreads, 0, stream>>>(g);
+    sample_draw<DT, STEPS><<<grid, kThreads, 0, stream>>>(g);
     return hipGetLastError();
+}
+template <int DT>
+hipError_t launch(const SampleArgs& a, void* workspace, hipStream_t stream) {
+    const Split p = split(a.rows, a.vocab, a.dtype);
+    return p.small ? launch_steps<DT, 1>(a, p, workspace, stream) : launch_steps<DT, kBatch>(a, p, workspace, stream);
 }
 
 }  // namespace
