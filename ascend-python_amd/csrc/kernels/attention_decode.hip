@@ -55,16 +55,6 @@ struct Line {
     int64_t begin, end;
     int32_t workers;
 };
-// n / d for n >= 0, d > 0: by 32 bits where they fit, as they all but always do
-__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
-    return (uint64_t)(n | d) >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
-}
-__device__ __forceinline__ int64_t line_begin(int64_t total, int64_t workers, int64_t i) { return quotient(total * i, workers); }
-// The worker whose part holds unit u
-__device__ __forceinline__ int64_t worker_of(int64_t total, int64_t workers, int64_t u) {
-    return quotient((u + 1) * workers + total - 1, total) - 1;
-}
-
 __device__ __forceinline__ int32_t length_of(const AttnArgs& a, int64_t b) {
     const int64_t most = a.kv.table_width * a.kv.c.page_size, n = a.kv.lens[b];
     return (int32_t)(n < 0 ? 0 : n > most ? most : n);

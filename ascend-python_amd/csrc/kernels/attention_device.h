@@ -100,6 +100,56 @@ __device__ __forceinline__ int32_t wave_scan(int32_t v) {
     return v;
 }
 
+// Work along a line of `total` units, of which each of `workers` takes an equal part.
+// n / d for n >= 0, d > 0: by 32 bits where they fit, as they all but always do
+__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
+    return (uint64_t)(n | d) >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
+}
+__device__ __forceinline__ int64_t line_begin(int64_t total, int64_t workers, int64_t i) { return quotient(total * i, workers); }
+// The worker whose part holds unit u
+__device__ __forceinline__ int64_t worker_of(int64_t total, int64_t workers, int64_t u) {
+    return quotient((u + 1) * workers + total - 1, total) - 1;
+}
+
+// Rows of tokens and keys of sequence b (b == batch: the rows past the last sequence, which see nothing)
+struct Sequence {
+    int32_t first, tokens;
+};
+__device__ __forceinline__ Sequence sequence_of(const AttnArgs& a, int64_t b) {
+    const int32_t T = (int32_t)a.tokens;
+    int32_t first = b == 0 ? 0 : a.cu_q[b], end = b == a.batch ? T : a.cu_q[b + 1];
+    first = first < 0 ? 0 : first > T ? T : first;
+    end = end > T ? T : end;
+    return {first, end > first ? end - first : 0};
+}
+
+template <int DT>
+__device__ __forceinline__ constexpr uint32_t exponent_of() {
+    return DT == QK_BF16 ? 0x7f80u : 0x7c00u;
+}
+template <int DT>
+__device__ __forceinline__ bool not_finite(u32x4 w) {
+    constexpr uint32_t E = exponent_of<DT>(), H = E << 16;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= (w[i] & E) == E || (w[i] & H) == H;
+    return any;
+}
+// The finite values, and zero for the others.
+template <int DT>
+__device__ __forceinline__ u32x4 finite_only(u32x4 w) {
+    constexpr uint32_t E = exponent_of<DT>(), H = E << 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] &= ((w[i] & E) == E ? 0u : 0xffffu) | ((w[i] & H) == H ? 0u : 0xffff0000u);
+    return w;
+}
+
+// Tokens of sequence b in the cache.
+__device__ __forceinline__ int32_t cached_tokens(const AttnArgs& a, int64_t b) {
+    const int64_t most = a.kv.table_width * a.kv.c.page_size, n = a.kv.lens[b];
+    return (int32_t)(n < 0 ? 0 : n > most ? most : n);
+}
+
 // The keys that a position sees, without a gap: the first `sinks` of them, then those from `low` on.
 struct Seen {
     int32_t count, sinks, gap;

@@ -43,8 +43,10 @@ constexpr int kSplitTiles = 8;
 // Workgroups that the card holds, two per CU; cutting up to 768 or 1024 takes longer where tiles are nearly enough (1500
 // tokens 41.5 -> 46.9 us, chunks with a window 64 -> 69).
 constexpr int64_t kResident = 512;
-// Trees: a part's steps at least.
+// Trees: a part's steps at least; parts that are joined by one workgroup, and in groups of how many where there are more; and at
+// most (128 parts are 32 groups of 4; 512, all that there are, 16 of 32).
 constexpr int kTreeSteps = 4;
+constexpr int kJoinAtOnce = 8, kJoinGroup = 4, kJoined = 32;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <int DT>
@@ -82,44 +84,12 @@ struct PromptArgs {
     int splits;       // at most: parts that a tile's keys are cut into (trees: parts of all tiles where any is cut)
     uint64_t tag;
     uint64_t* arrivals;   // a counter for every tile and key-value head
-    float* parts;         // [tile and head][splits] (trees: [part and head]) [kRows * (DP + 2)], in the order of the registers
+    uint64_t* group_arrivals;  // trees: one for every part and key-value head
+    float* parts;         // [tile and head][splits] (trees: [part and head]) [ROWS * (DP + 2)], in the order of the registers
     int64_t part_bytes;   // of one of them
     TreeMask mask;
     int64_t most_tiles;   // trees: of a key-value head
 };
-
-// Rows of tokens and keys of sequence b (b == batch: the rows past the last sequence, which see nothing)
-struct Sequence {
-    int32_t first, tokens;
-};
-__device__ __forceinline__ Sequence sequence_of(const AttnArgs& a, int64_t b) {
-    const int32_t T = (int32_t)a.tokens;
-    int32_t first = b == 0 ? 0 : a.cu_q[b], end = b == a.batch ? T : a.cu_q[b + 1];
-    first = first < 0 ? 0 : first > T ? T : first;
-    end = end > T ? T : end;
-    return {first, end > first ? end - first : 0};
-}
-
-template <int DT>
-__device__ __forceinline__ constexpr uint32_t exponent_of() {
-    return DT == QK_BF16 ? 0x7f80u : 0x7c00u;
-}
-template <int DT>
-__device__ __forceinline__ bool not_finite(u32x4 w) {
-    constexpr uint32_t E = exponent_of<DT>(), H = E << 16;
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) any |= (w[i] & E) == E || (w[i] & H) == H;
-    return any;
-}
-// The finite values, and zero for the others.
-template <int DT>
-__device__ __forceinline__ u32x4 finite_only(u32x4 w) {
-    constexpr uint32_t E = exponent_of<DT>(), H = E << 16;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] &= ((w[i] & E) == E ? 0u : 0xffffu) | ((w[i] & H) == H ? 0u : 0xffff0000u);
-    return w;
-}
 
 // Largest value, and sum, over lanes l and l ^ 32.
 __device__ __forceinline__ float pair_max(float v) {
@@ -131,19 +101,12 @@ __device__ __forceinline__ float pair_sum(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-__device__ __forceinline__ float largest(const f32x16 (&x)[2]) {
+template <int N>
+__device__ __forceinline__ float largest(const f32x16 (&x)[N]) {
     float top = x[0][0];
 #pragma unroll
-    for (int e = 1; e < 16; ++e) top = __builtin_elementwise_maximum(top, x[0][e]);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) top = __builtin_elementwise_maximum(top, x[1][e]);
+    for (int e = 1; e < 16 * N; ++e) top = __builtin_elementwise_maximum(top, x[e >> 4][e & 15]);
     return top;
-}
-
-// Tokens of sequence b in the cache.
-__device__ __forceinline__ int32_t cached_tokens(const AttnArgs& a, int64_t b) {
-    const int64_t most = a.kv.table_width * a.kv.c.page_size, n = a.kv.lens[b];
-    return (int32_t)(n < 0 ? 0 : n > most ? most : n);
 }
 
 // Trees: row tiles of a sequence, and steps over the keys that any of its rows sees (b == a.batch: the rows past the last
@@ -151,9 +114,10 @@ __device__ __forceinline__ int32_t cached_tokens(const AttnArgs& a, int64_t b) {
 struct TreeSize {
     int32_t tiles, steps;
 };
+template <int ROWS>
 __device__ __forceinline__ TreeSize tree_size(const AttnArgs& a, int32_t G, int64_t b) {
     const int32_t tokens = sequence_of(a, b).tokens;
-    TreeSize s = {(int32_t)(((int64_t)tokens * G + kRows - 1) / kRows), 0};
+    TreeSize s = {(int32_t)(((int64_t)tokens * G + ROWS - 1) / ROWS), 0};
     if (b < a.batch) {
         int32_t keys = cached_tokens(a, b);
         const int32_t past = keys - tokens;
@@ -176,22 +140,24 @@ struct TreeWork {
 
 // The lengths are on the device only, so each wave finds the share at `rank` by itself, a lane per sequence.  A part has at most `unit` steps,
 // the fewest (but kTreeSteps) at which all parts fit into `room`; where the tiles alone fill it, none is cut.
+template <int ROWS>
 __device__ __forceinline__ bool tree_work(const AttnArgs& a, int32_t G, int32_t room, int64_t rank, TreeWork& w) {
     const int lane = threadIdx.x & 63;
     const int64_t n = a.batch + 1;
     const bool small = n <= 64;
-    const TreeSize none = {0, 0}, own = small && lane < n ? tree_size(a, G, lane) : none;
+    const TreeSize none = {0, 0}, own = small && lane < n ? tree_size<ROWS>(a, G, lane) : none;
     // a sum over the sequences that fits 31 bits
     auto total = [&](auto of) INLINE {
         int32_t sum = small ? of(own) : 0;
         if (!small)
-            for (int64_t b = lane; b < n; b += 64) sum += of(tree_size(a, G, b));
+            for (int64_t b = lane; b < n; b += 64) sum += of(tree_size<ROWS>(a, G, b));
         return __builtin_amdgcn_readlane(wave_scan(sum), 63);
     };
     // (about: a part more or less does not matter, only that every workgroup finds the same)
     auto parts_of = [](TreeSize s, float unit) INLINE {
-        const float p = __builtin_ceilf((float)s.steps * (1.0f / unit));
-        return p < 1.0f ? 1 : p > 1024.0f ? 1024 : (int32_t)p;
+        const float p = __builtin_ceilf((float)s.steps * __builtin_amdgcn_rcpf(unit));
+        const int32_t most = (s.steps + kTreeSteps - 1) / kTreeSteps;
+        return p < 1.0f ? 1 : p < (float)most ? (int32_t)p : most < 1 ? 1 : most < 1024 ? most : 1024;
     };
     const int32_t tiles = total([](TreeSize s) INLINE { return s.tiles; });
     if (rank >= (tiles < room ? room : tiles)) return false;
@@ -200,7 +166,7 @@ __device__ __forceinline__ bool tree_work(const AttnArgs& a, int32_t G, int32_t 
         float work = (float)own.tiles * (float)own.steps;
         if (!small)
             for (int64_t b = lane; b < n; b += 64) {
-                const TreeSize s = tree_size(a, G, b);
+                const TreeSize s = tree_size<ROWS>(a, G, b);
                 work += (float)s.tiles * (float)s.steps;
             }
         work = wave_sum(work);
@@ -217,7 +183,7 @@ __device__ __forceinline__ bool tree_work(const AttnArgs& a, int32_t G, int32_t 
             float low = unit;
             unit = fmaxf(2.0f * (float)kTreeSteps, work / (float)(room - tiles) + 1.0f);
             while (unit < 0x1p30f && !fits(unit)) unit *= 2.0f;
-            for (int i = 0; i < 6; ++i) {
+            for (int i = 0; i < 3; ++i) {
                 const float mid = 0.5f * (low + unit);
                 if (fits(mid)) unit = mid;
                 else low = mid;
@@ -226,7 +192,7 @@ __device__ __forceinline__ bool tree_work(const AttnArgs& a, int32_t G, int32_t 
     }
     int64_t before = 0, index = 0;
     for (int64_t b0 = 0; b0 < n; b0 += 64) {
-        const TreeSize s = small ? own : b0 + lane < n ? tree_size(a, G, b0 + lane) : none;
+        const TreeSize s = small ? own : b0 + lane < n ? tree_size<ROWS>(a, G, b0 + lane) : none;
         const int32_t parts = parts_of(s, unit), mine = s.tiles * parts;
         const int32_t upto = wave_scan(mine), tiles_upto = wave_scan(s.tiles);
         if (rank < before + __builtin_amdgcn_readlane(upto, 63)) {
@@ -248,9 +214,13 @@ __device__ __forceinline__ bool tree_work(const AttnArgs& a, int32_t G, int32_t 
     return false;
 }
 
-// DP: head_dim padded to 32s; WHOLE: head_dim == DP; Q8: int8 cache; TREE: rows of trees, on keys in pages
-template <int DP, int DT, bool Q8, bool WHOLE, bool TREE>
+// DP: head_dim padded to 32s; WHOLE: head_dim == DP; Q8: int8 cache; TREE: rows of trees, on keys in pages; HALF (trees): tiles of 64
+// rows, of whose keys two of the waves take one half and two the other
+template <int DP, int DT, bool Q8, bool WHOLE, bool TREE, bool HALF>
 __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(PromptArgs g) {
+    static_assert(TREE || !HALF, "");
+    constexpr int ROWS = HALF ? kRows / 2 : kRows;
+    constexpr int KN = HALF ? 1 : 2;             // 32-key blocks of a tile that a wave takes
     constexpr int KS = DP / 16;                  // steps of the first product
     constexpr int NB = DP / 32;                  // 32-row blocks of V^T
     constexpr int LS = DP <= 64 ? 128 : DP <= 128 ? 256 : 512;  // bytes of a row in LDS
@@ -273,19 +243,20 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     const qk_kv_cache& c = a.kv.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, kg = lane >> 5;
+    const int part_of_rows = HALF ? wave & 1 : wave, half = HALF ? wave >> 1 : 0;  // which 32 rows, and which keys of a tile
     const int D = (int)c.head_dim, G = (int)(a.q_heads / c.kv_heads);
     const int kvh = (int)(blockIdx.x % (uint32_t)c.kv_heads);
 
     // ---- which tile: those of all sequences in a line, the last first (the longest of a prompt come first)
     TreeWork work = {};
     if constexpr (TREE) {
-        if (!tree_work(a, G, g.splits, blockIdx.x / (uint32_t)c.kv_heads, work) || work.index >= g.most_tiles) return;
+        if (!tree_work<ROWS>(a, G, g.splits, blockIdx.x / (uint32_t)c.kv_heads, work) || work.index >= g.most_tiles) return;
         if (tid < 3) bad[tid] = 0;
     } else {
         const int64_t per = (a.batch + 1 + kThreads - 1) / kThreads;
         const int64_t b0 = tid * per, b1 = b0 + per < a.batch + 1 ? b0 + per : a.batch + 1;
         int64_t mine = 0;
-        for (int64_t b = b0; b < b1; ++b) mine += ((int64_t)sequence_of(a, b).tokens * G + kRows - 1) / kRows;
+        for (int64_t b = b0; b < b1; ++b) mine += ((int64_t)sequence_of(a, b).tokens * G + ROWS - 1) / ROWS;
         int64_t* const sums = (int64_t*)&info[0][0][0];
         int64_t in = mine;
         for (int d = 1; d < 64; d <<= 1) {
@@ -300,7 +271,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         if (rank < 0) return;
         int64_t at = in - mine;
         for (int64_t b = b0; b < b1; ++b) {
-            const int64_t n = ((int64_t)sequence_of(a, b).tokens * G + kRows - 1) / kRows;
+            const int64_t n = ((int64_t)sequence_of(a, b).tokens * G + ROWS - 1) / ROWS;
             if (at <= rank && rank < at + n) {
                 found[0] = b;
                 found[1] = rank - at;
@@ -311,9 +282,9 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         __syncthreads();
     }
     const int32_t b = TREE ? work.b : __builtin_amdgcn_readfirstlane((int32_t)found[0]);
-    const int32_t row0 = (TREE ? work.tile : __builtin_amdgcn_readfirstlane((int32_t)found[1])) * kRows;
+    const int32_t row0 = (TREE ? work.tile : __builtin_amdgcn_readfirstlane((int32_t)found[1])) * ROWS;
     const Sequence seq = sequence_of(a, b);
-    const int32_t rows = (int32_t)((int64_t)seq.tokens * G - row0 < kRows ? (int64_t)seq.tokens * G - row0 : kRows);
+    const int32_t rows = (int32_t)((int64_t)seq.tokens * G - row0 < ROWS ? (int64_t)seq.tokens * G - row0 : ROWS);
 
     // keys of the sequence, and the row of the first where they are contiguous
     int32_t keys = 0, key0 = 0;
@@ -334,7 +305,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     const int32_t p_last = TREE ? keys - 1 : past + div31(row0 + rows - 1, g.group_div);
 
     // this lane's row (past the last: as the last)
-    const int32_t mine = row0 + (wave * 32 + col < rows ? wave * 32 + col : rows - 1);
+    const int32_t mine = row0 + (part_of_rows * 32 + col < rows ? part_of_rows * 32 + col : rows - 1);
     const int32_t token = div31(mine, g.group_div);
     const int64_t t = seq.first + token;
     const int h = kvh * G + (mine - token * G);
@@ -508,7 +479,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         }
     };
 
-    const bool no_rows = wave * 32 >= rows;  // for this wave
+    const bool no_rows = part_of_rows * 32 >= rows;  // for this wave
     if (tile0 < tiles) {
         int32_t page = page_of(tile0);
         put_info(tile0, page);
@@ -527,20 +498,21 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         }
         __syncthreads();
 
-        const int k_at = col * LS + ((kg ^ k_turn(col)) << 4);
+        const int k_at = (half * 32 + col) * LS + ((kg ^ k_turn(col)) << 4);
         const int v_row = 4 * kg + (lane >> 2 & 3);
-        const int v_at = v_row * LS + (((lane >> 4 & 1) << 1 | (lane >> 1 & 1)) ^ v_turn(v_row)) * 16 + 8 * (lane & 1);
+        const int v_at = (half * 32 + v_row) * LS + (((lane >> 4 & 1) << 1 | (lane >> 1 & 1)) ^ v_turn(v_row)) * 16 + 8 * (lane & 1);
+        const int s_at = half * 32 + 4 * kg;
         // scores of a tile: lane (row, kg) holds keys 32 n + 8 (e / 4) + 4 kg + e % 4
-        auto scores = [&](int tile, f32x16 (&x)[2]) INLINE {
+        auto scores = [&](int tile, f32x16 (&x)[KN]) INLINE {
             const char* const kb = lds + 2 * (tile & 1) * TILE;
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < KN; ++n)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[n][e] = 0.0f;
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
-                for (int n = 0; n < 2; ++n) x[n] = mma32<DT>(*(const u32x4*)(kb + (k_at ^ s << 5) + 32 * n * LS), q[s], x[n]);
+                for (int n = 0; n < KN; ++n) x[n] = mma32<DT>(*(const u32x4*)(kb + (k_at ^ s << 5) + 32 * n * LS), q[s], x[n]);
         };
 
         uint64_t mine = ~0ull;  // the tile's keys that this lane's row sees, from the lane's first on: bit 32 n + 8 (e / 4) + e % 4
@@ -566,16 +538,16 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         };
         // int8: scores times the keys' scales, in units of log2; the largest of them, each with its value's scale: what the weight that
         // goes into the product is held against.  Keys that are hidden are not looked at.
-        auto scale_scores = [&](int tile, f32x16 (&x)[2], auto hide) INLINE {
+        auto scale_scores = [&](int tile, f32x16 (&x)[KN], auto hide) INLINE {
             float top = -__builtin_inff();
             const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < KN; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     __builtin_amdgcn_sched_barrier(0);  // few of them in registers at a time
-                    const f32x4 k4 = *(const f32x4*)&scales[tile & 7][0][32 * n + 8 * i + 4 * kg];
-                    const f32x4 l4 = *(const f32x4*)&scales[tile & 7][2][32 * n + 8 * i + 4 * kg];
+                    const f32x4 k4 = *(const f32x4*)&scales[tile & 7][0][32 * n + 8 * i + s_at];
+                    const f32x4 l4 = *(const f32x4*)&scales[tile & 7][2][32 * n + 8 * i + s_at];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float v = x[n][4 * i + r] * k4[r];
@@ -592,15 +564,15 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             return top;
         };
         // int8: the weights' sum, and the weights with the values' scales (0 for what is hidden, whatever its scale)
-        auto scale_weights = [&](int tile, f32x16 (&x)[2], auto hide) INLINE {
+        auto scale_weights = [&](int tile, f32x16 (&x)[KN], auto hide) INLINE {
             const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
             float part[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < KN; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     __builtin_amdgcn_sched_barrier(0);
-                    const f32x4 v4 = *(const f32x4*)&scales[tile & 7][1][32 * n + 8 * i + 4 * kg];
+                    const f32x4 v4 = *(const f32x4*)&scales[tile & 7][1][32 * n + 8 * i + s_at];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         part[r & 1] += x[n][4 * i + r];
@@ -627,7 +599,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         };
 
         // Looks at the tile whose scores x are there, `top` a lane's largest: hides what is not seen, moves the maximum.
-        auto prepare = [&](int tile, uint64_t which, f32x16 (&x)[2], float top) INLINE {
+        auto prepare = [&](int tile, uint64_t which, f32x16 (&x)[KN], float top) INLINE {
             look(tile, which);
             if (no_rows) return;
             mine = ~0ull;
@@ -645,6 +617,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                         seen |= ok & (turn ? mask_word(k) >> turn | mask_word(k + 1) << (64 - turn) : mask_word(k));
                     }
                 }
+                if constexpr (HALF) seen = half ? seen >> 32 : seen & 0xffffffffu;
                 any |= seen != 0;
                 mine = seen >> here(4 * kg);
                 if constexpr (Q8) {
@@ -652,7 +625,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 } else {
                     const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < KN; ++n)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) x[n][e] = (n ? hi : lo) & 1u << (8 * (e >> 2) + (e & 3)) ? x[n][e] : -__builtin_inff();
                     top = largest(x);
@@ -665,7 +638,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         };
 
         // One step: the tile's weights from its scores x, while the next tile's scores are made (into y), then its values.
-        auto step = [&](int it, f32x16 (&x)[2], f32x16 (&y)[2]) INLINE {
+        auto step = [&](int it, f32x16 (&x)[KN], f32x16 (&y)[KN]) INLINE {
             begin(it);
             if (!Q8 && __builtin_expect(edge, 0)) {
                 char* const vb = lds + (2 * (it & 1) + 1) * TILE;
@@ -689,7 +662,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 return;
             }
             const uint32_t k_from = lds0 + 2 * (it + 1 & 1) * TILE + here(k_at);
-            auto k_operand = [&](int i) INLINE { return lds_load(k_from ^ (i >> 1) << 5, 32 * (i & 1) * LS); };
+            auto k_operand = [&](int i) INLINE { return lds_load(k_from ^ i / KN << 5, 32 * (i % KN) * LS); };
             constexpr int AHEAD1 = Q8 ? 4 : 6;
             u32x4 k_ring[AHEAD1];
 #pragma unroll
@@ -717,14 +690,14 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             u32x4 v_ring[AHEAD2];
             // the next tile's scores, with this one's weights between the products
             {
-                constexpr int N = 2 * KS, FIRST = 6;
+                constexpr int N = KN * KS, FIRST = 6;
                 auto weight = [&](int k) INLINE {
                     float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 4][k & 15], factor, -m));
                     asm volatile("" : "+v"(w));  // made here, not where it is used
                     x[k >> 4][k & 15] = w;
                 };
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < KN; ++n)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) y[n][e] = 0.0f;
                 __builtin_amdgcn_sched_barrier(0);
@@ -733,7 +706,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     __builtin_amdgcn_sched_barrier(0);
-                    y[i & 1] = mma32<DT>(k_ring[i % AHEAD1], q[i >> 1], y[i & 1]);
+                    y[i % KN] = mma32<DT>(k_ring[i % AHEAD1], q[i / KN], y[i % KN]);
                     if (i + AHEAD1 < N) k_ring[i % AHEAD1] = k_operand(i + AHEAD1);
                     if constexpr (!Q8) {
 #pragma unroll
@@ -742,7 +715,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                     }
                     if (i >= N - AHEAD2) v_ring[i - N + AHEAD2] = v_operand(i - N + AHEAD2);
 #pragma unroll
-                    for (int k = FIRST + i * (32 - FIRST) / N; k < FIRST + (i + 1) * (32 - FIRST) / N; ++k) weight(k);
+                    for (int k = FIRST + i * (16 * KN - FIRST) / N; k < FIRST + (i + 1) * (16 * KN - FIRST) / N; ++k) weight(k);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -751,17 +724,17 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 else scale_weights(it, x, std::false_type());
             } else if (__builtin_expect(edge, 0)) {
 #pragma nounroll
-                for (uint64_t left = uniform64(bad[it % 3]); left; left &= left - 1) {
+                for (uint64_t left = uniform64(HALF ? (uint32_t)(bad[it % 3] >> 32 * half) : bad[it % 3]); left; left &= left - 1) {
                     const int key = __builtin_ctzll(left), own = key - here(4 * kg);
                     // this row's weight of the key, from whichever of the two lanes holds it, and whether it is seen
                     float w = 0.0f;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < KN; ++n)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) w = own == 32 * n + 8 * (e >> 2) + (e & 3) ? x[n][e] : w;
                     w = load_half_bits(pack2<DT>(pair_sum(w), 0.0f) & 0xffffu, DT);  // as the products round it
                     const bool sees = pair_max(own >= 0 && !(own & 4) && (mine >> (own & 63) & 1) ? 1.0f : 0.0f) != 0.0f;
-                    const Global row = (Global)(uintptr_t)info[it & 7][key][1];
+                    const Global row = (Global)(uintptr_t)info[it & 7][key + 32 * half][1];
 #pragma unroll
                     for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -779,7 +752,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             // acc += V^T P^T; between the products the weights' sum, their rounding to 16 bits, and the largest of the next scores
             float top = y[0][0];
             {
-                constexpr int N = 4 * NB;
+                constexpr int N = 2 * KN * NB;
                 auto weights = [&](int s, int i) INLINE {
                     return pack2<PV>(x[s >> 1][8 * (s & 1) + 2 * i], x[s >> 1][8 * (s & 1) + 2 * i + 1]);
                 };
@@ -793,13 +766,13 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                     const int s = i / NB;
                     acc[i % NB] = mma32<PV>(v_ring[i % AHEAD2], pw[s & 1], acc[i % NB]);
                     if (i + AHEAD2 < N) v_ring[i % AHEAD2] = v_operand(i + AHEAD2);
-                    if (s < 3) {
+                    if (s < 2 * KN - 1) {
 #pragma unroll
                         for (int k = i % NB * 4 / NB; k < (i % NB + 1) * 4 / NB; ++k) pw[s + 1 & 1][k] = weights(s + 1, k);
                     }
                     if constexpr (!Q8) {
 #pragma unroll
-                        for (int k = i * 32 / N; k < (i + 1) * 32 / N; ++k) {
+                        for (int k = i * 16 * KN / N; k < (i + 1) * 16 * KN / N; ++k) {
                             part[k & 3] += x[k >> 4][k & 15];
                             top = __builtin_elementwise_maximum(top, y[k >> 4][k & 15]);
                         }
@@ -812,7 +785,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             prepare(it + 1, ok_next, y, top);
         };
 
-        f32x16 xa[2], xb[2];
+        f32x16 xa[KN], xb[KN];
         if (!no_rows) scores(tile0, xa);
         prepare(tile0, info_ok[tile0 & 7], xa, largest(xa));
         for (int it = tile0; it < tiles; it += 2) {
@@ -822,10 +795,41 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     }
 
     l = pair_sum(l);
+    if constexpr (HALF) {
+        // the two halves of the keys: the second waves' sums go to the first
+        __syncthreads();  // the last values have been read
+        float* const to = (float*)lds + part_of_rows * (NB * 16 + 2) * 64 + lane;
+        if (here(half)) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) to[(i * 16 + e) * 64] = acc[i][e];
+            to[NB * 16 * 64] = any ? m : -__builtin_inff();
+            to[(NB * 16 + 1) * 64] = l;
+        }
+        __syncthreads();
+        if (!here(half)) {
+            const float m1 = to[NB * 16 * 64], top = fmaxf(any ? m : -__builtin_inff(), m1);
+            const bool other = m1 != -__builtin_inff();
+            const float f0 = any ? __builtin_amdgcn_exp2f(m - top) : 0.0f, f1 = other ? __builtin_amdgcn_exp2f(m1 - top) : 0.0f;
+            l = l * f0 + to[(NB * 16 + 1) * 64] * f1;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                __builtin_amdgcn_sched_barrier(0);  // few of them in registers at a time
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][e] = acc[i][e] * f0 + to[(i * 16 + e) * 64] * f1;
+            }
+            any |= other;
+            m = any ? top : kLowest;
+        }
+    }
+    // The second waves write nothing: their rows lie past the last, and their parts past the buffer's end.  (A branch on `half` would make
+    // the compiler write all of the above out for each.)
+    const int away = HALF ? here(half) << 29 : 0;
     if (splits > 1) {
         const int64_t place = (TREE ? work.index : (int64_t)(blockIdx.x / (uint32_t)(c.kv_heads * g.splits))) * c.kv_heads + kvh;
         // in the order of the registers: whole lines, and the joining lane finds its own rows
-        constexpr uint32_t SUMS = 4 * NB * 4 * 1024;
+        constexpr uint32_t SUMS = ROWS / 32 * NB * 4 * 1024;
         auto part = [&](int s) INLINE {
             const int64_t at = TREE ? (work.first + (int64_t)s * work.tiles) * c.kv_heads + kvh : place * g.splits + s;
             return make_rsrc((const char*)g.parts + at * g.part_bytes, (uint32_t)g.part_bytes);
@@ -838,10 +842,97 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
                 for (int e = 0; e < 4; ++e)
                     __builtin_amdgcn_raw_buffer_store_b128(
                         __builtin_bit_cast(u32x4, (f32x4){acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]}), own,
-                        lane * 16, ((wave * NB + i) * 4 + e) * 1024, kCoherent);
+                        lane * 16 + away, ((part_of_rows * NB + i) * 4 + e) * 1024, kCoherent);
             if (kg == 0)
                 __builtin_amdgcn_raw_buffer_store_b64((u32x2){__float_as_uint(any ? m : -__builtin_inff()), __float_as_uint(l)}, own,
-                                                      SUMS + (wave * 32 + col) * 8, 0, kCoherent);
+                                                      SUMS + (part_of_rows * 32 + col) * 8 + away, 0, kCoherent);
+        }
+        if constexpr (TREE) {
+            // The parts of a tile, in pieces of 32 rows and 32 elements (a lane's 16 of its row) that the four waves take in turn, however
+            // few rows there are: `count` of them, every `step`-th from `from` on.  emit(row, element, values, max, sum).
+            const int pieces = (rows + 31) / 32 * NB;
+            auto join = [&](int from, int count, int step, auto emit) INLINE {
+                float* const pm = (float*)lds;  // [count][ROWS] maxima, then as many sums
+                float* const pl = pm + kJoined * ROWS;
+                __syncthreads();
+                for (int k = wave; k < count; k += 4)
+                    for (int r = lane; r < rows; r += 64) {
+                        const u32x2 ml = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(part(from + k * step), SUMS + r * 8, 0, kCoherent));
+                        pm[k * ROWS + r] = __uint_as_float(ml[0]);
+                        pl[k * ROWS + r] = __uint_as_float(ml[1]);
+                    }
+                __syncthreads();
+                for (int piece = wave; piece < pieces; piece += 4) {
+                    const int r = piece / NB * 32 + col < rows ? piece / NB * 32 + col : rows - 1;
+                    float top = -__builtin_inff(), sum = 0.0f;
+                    for (int k = 0; k < count; ++k) top = fmaxf(top, pm[k * ROWS + r]);
+                    f32x4 to[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) to[e] = (f32x4){0, 0, 0, 0};
+                    constexpr int kDeep = 6;
+#pragma nounroll
+                    for (int k0 = 0; k0 < count; k0 += kDeep) {
+                        f32x4 v[kDeep][4];
+#pragma unroll
+                        for (int k = 0; k < kDeep; ++k)
+                            if (k0 + k < count) {
+                                const __amdgpu_buffer_rsrc_t rs = part(from + (k0 + k) * step);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    v[k][e] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, lane * 16, (piece * 4 + e) * 1024, kCoherent));
+                            }
+#pragma unroll
+                        for (int k = 0; k < kDeep; ++k)
+                            if (k0 + k < count) {
+                                const float m1 = pm[(k0 + k) * ROWS + r];
+                                const bool none = m1 == -__builtin_inff();
+                                const float f = none ? 0.0f : __builtin_amdgcn_exp2f(m1 - top);
+                                sum += none ? 0.0f : pl[(k0 + k) * ROWS + r] * f;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                                    for (int d = 0; d < 4; ++d) to[e][d] += none ? 0.0f : v[k][e][d] * f;
+                            }
+                    }
+                    emit(piece, to, top, sum);
+                }
+            };
+            auto out = [&](int piece, f32x4 (&v)[4], float top, float sum) INLINE {
+                const int r = piece / NB * 32 + col;
+                if (r >= rows) return;
+                const bool none = top == -__builtin_inff();
+                const float inv = 1.0f / sum;
+                const int32_t tok = div31(row0 + r, g.group_div);
+                const int64_t o = (seq.first + (int64_t)tok) * a.q_heads + kvh * G + (row0 + r - tok * G);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = piece % NB * 32 + 8 * e + 4 * kg;
+                    if (!WHOLE && d >= D) continue;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[e][k] = none ? 0.0f : v[e][k] * inv;
+                    *(u32x2*)((uint16_t*)a.out + o * D + d) = (u32x2){pack2<DT>(v[e][0], v[e][1]), pack2<DT>(v[e][2], v[e][3])};
+                }
+                if (piece % NB == 0 && kg == 0 && a.lse) a.lse[o] = none ? top : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+            };
+            if (splits <= kJoinAtOnce) {
+                if (splitk_last(g.arrivals + place, (uint32_t)splits, g.tag)) join(0, splits, 1, out);
+                return;
+            }
+            // in two steps: the last of a group of parts leaves their join in the group's first, the last group joins those
+            const int step = splits <= kJoinGroup * kJoined ? kJoinGroup : kJoined, first = split / step * step;
+            const int members = splits - first < step ? splits - first : step, groups = (splits + step - 1) / step;
+            if (!splitk_last(g.group_arrivals + (work.first + (int64_t)first * work.tiles) * c.kv_heads + kvh, (uint32_t)members, g.tag)) return;
+            const __amdgpu_buffer_rsrc_t of_group = part(first);
+            join(first, members, 1, [&](int piece, f32x4 (&v)[4], float top, float sum) INLINE {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[e]), of_group, lane * 16, (piece * 4 + e) * 1024, kCoherent);
+                if (piece % NB == 0 && kg == 0)
+                    __builtin_amdgcn_raw_buffer_store_b64((u32x2){__float_as_uint(top), __float_as_uint(sum)}, of_group,
+                                                          SUMS + (piece / NB * 32 + col) * 8, 0, kCoherent);
+            });
+            if (splitk_last(g.arrivals + place, (uint32_t)groups, g.tag)) join(0, groups, step, out);
+            return;
         }
         if (!splitk_last(g.arrivals + place, (uint32_t)splits, g.tag)) return;
         m = -__builtin_inff();
@@ -894,7 +985,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
         }
         any = m != -__builtin_inff();
     }
-    if (wave * 32 + col >= rows) return;
+    if (part_of_rows * 32 + col + away >= rows) return;
     const float inv = 1.0f / l;
     const int64_t o = t * a.q_heads + h;
 #pragma unroll
@@ -911,37 +1002,37 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
     if (kg == 0 && a.lse) a.lse[o] = any ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -__builtin_inff();
 }
 
-template <int DP, int DT, bool Q8, bool TREE>
+template <int DP, int DT, bool Q8, bool TREE, bool HALF>
 void launch_width(const PromptArgs& g, int64_t grid, hipStream_t stream) {
-    if (g.a.kv.c.head_dim == DP) attention_prompt<DP, DT, Q8, true, TREE><<<dim3((unsigned)grid), kThreads, 0, stream>>>(g);
-    else attention_prompt<DP, DT, Q8, false, TREE><<<dim3((unsigned)grid), kThreads, 0, stream>>>(g);
+    if (g.a.kv.c.head_dim == DP) attention_prompt<DP, DT, Q8, true, TREE, HALF><<<dim3((unsigned)grid), kThreads, 0, stream>>>(g);
+    else attention_prompt<DP, DT, Q8, false, TREE, HALF><<<dim3((unsigned)grid), kThreads, 0, stream>>>(g);
 }
 // The head_dim that a kernel is built for
 int64_t padded_width(const qk_kv_cache& c) {
     const int64_t D = c.head_dim;
     return D <= 64 ? 64 : D <= 96 && c.dtype != QK_I8 ? 96 : D <= 128 ? 128 : D <= 192 ? 192 : 256;
 }
-template <int DT, bool Q8, bool TREE>
+template <int DT, bool Q8, bool TREE, bool HALF>
 void launch_type(const PromptArgs& g, int64_t grid, hipStream_t stream) {
     switch (padded_width(g.a.kv.c)) {
-    case 64: return launch_width<64, DT, Q8, TREE>(g, grid, stream);
+    case 64: return launch_width<64, DT, Q8, TREE, HALF>(g, grid, stream);
     case 96:
-        if constexpr (!Q8) return launch_width<96, DT, false, TREE>(g, grid, stream);
+        if constexpr (!Q8) return launch_width<96, DT, false, TREE, HALF>(g, grid, stream);
         return;
-    case 128: return launch_width<128, DT, Q8, TREE>(g, grid, stream);
-    case 192: return launch_width<192, DT, Q8, TREE>(g, grid, stream);
-    default: return launch_width<256, DT, Q8, TREE>(g, grid, stream);
+    case 128: return launch_width<128, DT, Q8, TREE, HALF>(g, grid, stream);
+    case 192: return launch_width<192, DT, Q8, TREE, HALF>(g, grid, stream);
+    default: return launch_width<256, DT, Q8, TREE, HALF>(g, grid, stream);
     }
 }
-template <bool TREE>
+template <bool TREE, bool HALF = false>
 void launch_form(const PromptArgs& g, int64_t grid, hipStream_t stream) {
     const bool q8 = g.a.kv.c.dtype == QK_I8;
     if (g.a.dtype == QK_BF16) {
-        if (q8) launch_type<QK_BF16, true, TREE>(g, grid, stream);
-        else launch_type<QK_BF16, false, TREE>(g, grid, stream);
+        if (q8) launch_type<QK_BF16, true, TREE, HALF>(g, grid, stream);
+        else launch_type<QK_BF16, false, TREE, HALF>(g, grid, stream);
     } else {
-        if (q8) launch_type<QK_F16, true, TREE>(g, grid, stream);
-        else launch_type<QK_F16, false, TREE>(g, grid, stream);
+        if (q8) launch_type<QK_F16, true, TREE, HALF>(g, grid, stream);
+        else launch_type<QK_F16, false, TREE, HALF>(g, grid, stream);
     }
 }
 

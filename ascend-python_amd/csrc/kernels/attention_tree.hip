@@ -9,18 +9,28 @@
 #include "attention_prompt.h"
 
 namespace qk {
+
+void launch_attention_few_rows(const void* args, int64_t grid, hipStream_t stream);
+
 namespace {
+
+// Rows of a tree and key-value head, on average, up to which tiles are of 64 rows.
+constexpr int64_t kFewRows = 64;
 
 struct Plan {
     int64_t grid, arrivals_bytes, part_bytes, parts, tiles;
     int room;
+    bool half;
 };
 
 Plan plan(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache& c, int64_t table_width) {
     Plan p = {};
     const int64_t some = batch < tokens ? batch : tokens;
     // at most, of a key-value head: row tiles, and parts of a tile
-    const int64_t tiles = p.tiles = tokens * (q_heads / c.kv_heads) / kRows + some + 1;
+    const int64_t group = q_heads / c.kv_heads;
+    p.half = tokens * group <= kFewRows * batch;
+    const int64_t rows = p.half ? kRows / 2 : kRows;
+    const int64_t tiles = p.tiles = tokens * group / rows + some + 1;
     const int64_t parts = table_width * c.page_size / kKeys / kTreeSteps + 1;
     // cut tiles fill the card's places once; heads wider than 128 leave one workgroup per CU
     const int64_t room = (c.head_dim <= 128 ? kResident : kResident / 2) / c.kv_heads;
@@ -31,8 +41,8 @@ Plan plan(int64_t tokens, int64_t batch, int64_t q_heads, const qk_kv_cache& c, 
     p.grid = ranks * c.kv_heads;
     if (p.room > 1 && parts > 1) {
         p.parts = (ranks < p.room ? ranks : p.room) * c.kv_heads;
-        p.arrivals_bytes = (tiles * c.kv_heads * 8 + 255) / 256 * 256;
-        p.part_bytes = kRows * (padded_width(c) + 2) * 4;
+        p.arrivals_bytes = ((tiles * c.kv_heads + p.parts) * 8 + 255) / 256 * 256;
+        p.part_bytes = rows * (padded_width(c) + 2) * 4;
     }
     return p;
 }
@@ -56,10 +66,12 @@ hipError_t launch_attention_tree(const AttnArgs& a, const TreeMask& mask, void* 
     if (p.parts > 0) {
         g.tag = next_split_tag();
         g.arrivals = (uint64_t*)workspace;
+        g.group_arrivals = g.arrivals + p.tiles * a.kv.c.kv_heads;
         g.parts = (float*)((char*)workspace + p.arrivals_bytes);
         g.part_bytes = p.part_bytes;
     }
-    launch_form<true>(g, p.grid, stream);
+    if (p.half) launch_attention_few_rows(&g, p.grid, stream);
+    else launch_form<true>(g, p.grid, stream);
     return hipGetLastError();
 }
 
