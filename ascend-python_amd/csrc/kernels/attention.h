@@ -109,7 +109,8 @@ hipError_t launch_kv_compact(const qk_pages* pages, int64_t tensors, const PoolA
                              int32_t* new_count, int32_t* moved, void* ws, hipStream_t stream);
 hipError_t launch_kv_accept(const qk_rows* rows, int64_t tensors, const PoolArgs& p, const int32_t* seqs, const int32_t* cu,
                             int64_t n, int64_t total, const int32_t* tokens, const int32_t* parents, const int32_t* sampled,
-                            int32_t* path, int32_t* accepted, int32_t* next, hipStream_t stream);
+                            int32_t* path, int32_t* accepted, int32_t* next, void* ws, hipStream_t stream);
+size_t kv_accept_workspace(int64_t n);
 size_t kv_fork_workspace(int64_t n);
 size_t kv_extend_workspace(int64_t n, int64_t num_pages);
 size_t kv_compact_workspace(int64_t num_pages);

@@ -99,8 +99,21 @@ __device__ __forceinline__ void move_rows(const qk_rows& t, int64_t page_size, i
     else move_units<uint8_t>(t, page_size, u, step, j0, n, slots);
 }
 
-// blockIdx.x: the sequence (n: the rows of none); blockIdx.y: the tensor (0, in the first launch: also writes the way).
-__global__ __launch_bounds__(kThreads) void accept_rows(RowList list, int tensors, AcceptArgs a, bool write) {
+// The sequence's length, and the pages that it no longer needs.
+__device__ __forceinline__ void finish(const AcceptArgs& a, const Tree& t, int32_t kept) {
+    const int64_t S = a.p.page_size, len = (int64_t)t.past + kept, old = (int64_t)t.past + t.size;
+    for (int64_t j = (len + S - 1) / S + threadIdx.x; j < (old + S - 1) / S; j += blockDim.x) {
+        const int32_t page = atomicExch(a.p.table + t.seq * a.p.table_stride + j, -1);
+        if (page >= 0 && page < a.p.num_pages && atomicSub(a.p.count + page, 1) <= 0) atomicAdd(a.p.count + page, 1);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) a.p.lens[t.seq] = (int32_t)len;
+}
+
+// blockIdx.x: the sequence (n: the rows of none); blockIdx.y: the tensor (0, in the first launch: also writes the way).  arrivals: of the
+// sequences' workgroups that have read its length and its table, the last of which may then change them (nullptr: a launch of
+// its own does).
+__global__ __launch_bounds__(kThreads) void accept_rows(RowList list, int tensors, AcceptArgs a, bool write, uint64_t* arrivals, uint64_t tag) {
     __shared__ int32_t child[kTree], way[kTree];
     __shared__ int64_t from[kTree], to[kTree];
     __shared__ int32_t found[2];
@@ -146,12 +159,16 @@ __global__ __launch_bounds__(kThreads) void accept_rows(RowList list, int tensor
                 a.next[blockIdx.x] = sampled[found[1]];
             }
         }
-        if ((int)blockIdx.y >= tensors) return;
+        if (tensors == 0) {
+            if (arrivals) finish(a, t, n);
+            return;
+        }
         for (int32_t j = threadIdx.x; j < n; j += kThreads) {
             from[j] = way[j] == j ? -1 : slot_of(a.p, t.seq, (int64_t)t.past + way[j]);
             to[j] = way[j] == j ? -1 : slot_of(a.p, t.seq, (int64_t)t.past + j);
         }
         __syncthreads();
+        if (arrivals && splitk_last(arrivals + blockIdx.x, gridDim.y, tag)) finish(a, t, n);
         // the first rows of the way lie where they belong
         int32_t j0 = 0;
         while (j0 < n && way[j0] == j0) ++j0;
@@ -194,38 +211,37 @@ __global__ __launch_bounds__(kThreads) void accept_rows(RowList list, int tensor
             a.next[blockIdx.x] = sampled[last];
         }
     }
+    if (arrivals && splitk_last(arrivals + blockIdx.x, gridDim.y, tag)) finish(a, t, n);
 }
 
-// The sequences' lengths, and the pages that they no longer need.
 __global__ __launch_bounds__(64) void accept_finish(AcceptArgs a) {
     const Tree t = tree_of(a, blockIdx.x);
-    if (t.size == 0) return;
-    const int64_t S = a.p.page_size, len = (int64_t)t.past + a.accepted[blockIdx.x], old = (int64_t)t.past + t.size;
-    for (int64_t j = (len + S - 1) / S + threadIdx.x; j < (old + S - 1) / S; j += 64) {
-        const int32_t page = atomicExch(a.p.table + t.seq * a.p.table_stride + j, -1);
-        if (page >= 0 && page < a.p.num_pages && atomicSub(a.p.count + page, 1) <= 0) atomicAdd(a.p.count + page, 1);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) a.p.lens[t.seq] = (int32_t)len;
+    if (t.size > 0) finish(a, t, a.accepted[blockIdx.x]);
 }
 
 }  // namespace
 
+size_t kv_accept_workspace(int64_t n) { return (size_t)n * 8; }
+
 hipError_t launch_kv_accept(const qk_rows* rows, int64_t tensors, const PoolArgs& p, const int32_t* seqs, const int32_t* cu,
                             int64_t n, int64_t total, const int32_t* tokens, const int32_t* parents, const int32_t* sampled,
-                            int32_t* path, int32_t* accepted, int32_t* next, hipStream_t stream) {
+                            int32_t* path, int32_t* accepted, int32_t* next, void* ws, hipStream_t stream) {
     const AcceptArgs a = {p, seqs, cu, n, total, tokens, parents, sampled, path, accepted, next};
+    // one launch ends the sequences too; more of them read what that changes
+    const bool one = tensors <= kTensors;
+    const uint64_t tag = next_split_tag();
     int64_t i = 0;
     do {
         RowList list = {};
         const int k = (int)(tensors - i < kTensors ? tensors - i : kTensors);
         for (int j = 0; j < k; ++j) list.t[j] = rows[i + j];
-        accept_rows<<<dim3((unsigned)(n + 1), (unsigned)(k < 1 ? 1 : k)), kThreads, 0, stream>>>(list, k, a, i == 0);
+        accept_rows<<<dim3((unsigned)(n + 1), (unsigned)(k < 1 ? 1 : k)), kThreads, 0, stream>>>(list, k, a, i == 0,
+                                                                                                      one ? (uint64_t*)ws : nullptr, tag);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         i += kTensors;
     } while (i < tensors);
-    if (n > 0) accept_finish<<<dim3((unsigned)n), 64, 0, stream>>>(a);
+    if (n > 0 && !one) accept_finish<<<dim3((unsigned)n), 64, 0, stream>>>(a);
     return hipGetLastError();
 }
 

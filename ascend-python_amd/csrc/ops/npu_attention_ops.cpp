@@ -711,7 +711,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> npu_kv_extend_meta(const at::Tens
 std::vector<qk_rows> row_list(const char* op, at::TensorList caches, int64_t num_pages, int64_t page_size, const at::Tensor& like) {
     std::vector<qk_rows> list;
     list.reserve(caches.size());
+    const at::Tensor* last = nullptr;
     for (const at::Tensor& t : caches) {
+        // layers are alike: what the one before passed need not be looked at again
+        if (last && t.element_size() == last->element_size() && t.strides() == last->strides() && t.sizes() == last->sizes() &&
+            t.device() == last->device()) {
+            list.push_back(list.back());
+            list.back().base = t.is_meta() ? nullptr : t.data_ptr();
+            continue;
+        }
         TORCH_CHECK(t.dim() >= 2 && t.dim() <= 64 && t.size(0) == num_pages && t.size(1) == page_size, op,
                     ": every cache tensor must be [", num_pages, ", ", page_size, ", ...], got ", t.sizes());
         check_device(op, "a cache tensor", t, like);
@@ -738,6 +746,7 @@ std::vector<qk_rows> row_list(const char* op, at::TensorList caches, int64_t num
         }
         TORCH_CHECK((num_pages == 1 || t.stride(0) > 0) && (page_size == 1 || t.stride(1) > 0), op, ": tokens of a cache tensor overlap");
         list.push_back(r);
+        last = &t;
     }
     return list;
 }
@@ -774,10 +783,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> npu_kv_accept(at::TensorList cach
     const auto seqs = seqs_in.contiguous(), cu = cu_in.contiguous(), tokens = tokens_in.contiguous(), parents = parents_in.contiguous(),
                sampled = sampled_in.contiguous();
     auto [path, accepted, next] = accept_outputs(tokens, seqs);
+    size_t ws_bytes = 0;
+    check_rc(qk_kv_accept_workspace_size(seqs.numel(), &ws_bytes), op);
+    const auto ws = workspace_for(table, ws_bytes);
     check_rc(qk_kv_accept(list.data(), (int64_t)list.size(), count.size(0), page_size, written(table), table.size(0), table.size(1),
                           stride_of(table, 0), written(lens), written(count), index_data(seqs), index_data(cu), seqs.numel(),
                           tokens.numel(), index_data(tokens), index_data(parents), index_data(sampled), written(path),
-                          written(accepted), written(next), current_stream(table)),
+                          written(accepted), written(next), ws.data_ptr(), ws_bytes, current_stream(table)),
              op);
     return {path, accepted, next};
 }

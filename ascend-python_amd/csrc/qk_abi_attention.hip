@@ -464,11 +464,19 @@ int qk_kv_extend(int64_t num_pages, int64_t page_size, int32_t* block_table, int
     return launched(qk::launch_kv_extend(p, seqs, cu_tokens, n, total, slots, positions, missing, workspace, (hipStream_t)stream), op);
 }
 
+int qk_kv_accept_workspace_size(int64_t n, size_t* bytes) {
+    qk::abi_begin();
+    if (!bytes) return fail(QK_ERR_ARG, "npu_kv_accept: null pointer");
+    if (int rc = check_seqs("npu_kv_accept", n)) return rc;
+    *bytes = qk::kv_accept_workspace(n);
+    return QK_OK;
+}
+
 int qk_kv_accept(const qk_rows* rows, int64_t tensors, int64_t num_pages, int64_t page_size, int32_t* block_table,
                  int64_t max_seqs, int64_t table_width, int64_t table_stride, int32_t* context_lens, int32_t* ref_count,
                  const int32_t* seqs, const int32_t* cu_tokens, int64_t n, int64_t total, const int32_t* tokens,
                  const int32_t* parents, const int32_t* sampled, int32_t* path, int32_t* accepted, int32_t* next,
-                 qk_stream_t stream) {
+                 void* workspace, size_t workspace_bytes, qk_stream_t stream) {
     qk::abi_begin();
     const char* op = "npu_kv_accept";
     if (int rc = check_pool(op, num_pages, page_size, block_table, max_seqs, table_width, table_stride, context_lens, ref_count)) return rc;
@@ -487,9 +495,10 @@ int qk_kv_accept(const qk_rows* rows, int64_t tensors, int64_t num_pages, int64_
     if ((n > 0 && (!seqs || !cu_tokens || !accepted || !next)) || (total > 0 && (!tokens || !parents || !sampled || !path)))
         return fail(QK_ERR_ARG, "%s: null pointer", op);
     if (n == 0 && total == 0) return QK_OK;
+    if (int rc = check_workspace(op, qk::kv_accept_workspace(n), workspace, workspace_bytes)) return rc;
     const qk::PoolArgs p = {num_pages, page_size, block_table, max_seqs, table_width, table_stride, context_lens, ref_count};
     return launched(qk::launch_kv_accept(rows, tensors, p, seqs, cu_tokens, n, total, tokens, parents, sampled, path, accepted, next,
-                                         (hipStream_t)stream),
+                                         workspace, (hipStream_t)stream),
                     op);
 }
 

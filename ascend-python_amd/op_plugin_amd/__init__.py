@@ -118,7 +118,8 @@ ABI_SYMBOLS = (
     "qk_prompt_attention_workspace_size", "qk_prompt_attention", "qk_tree_attention_workspace_size", "qk_tree_attention",
     "qk_mrope", "qk_kv_copy_pages",
     "qk_kv_fork_workspace_size", "qk_kv_fork", "qk_kv_free", "qk_kv_extend_workspace_size", "qk_kv_extend",
-    "qk_kv_compact_workspace_size", "qk_kv_compact", "qk_kv_accept", "qk_sample_workspace_size", "qk_sample",
+    "qk_kv_compact_workspace_size", "qk_kv_compact", "qk_kv_accept_workspace_size",
+    "qk_kv_accept", "qk_sample_workspace_size", "qk_sample",
 )
 
 
@@ -197,7 +198,8 @@ def abi() -> ctypes.CDLL:
         L.qk_kv_compact_workspace_size.argtypes = [I64, Z]
         L.qk_kv_compact.argtypes = [G, I64, I64, P, I64, I64, I64, P, P, P, P, P, SZ, P]
         L.qk_kv_accept.argtypes = [ctypes.POINTER(Rows), I64, I64, I64, P, I64, I64, I64, P, P, P, P, I64, I64, P, P, P, P, P, P,
-                                   P]
+                                   P, SZ, P]
+        L.qk_kv_accept_workspace_size.argtypes = [I64, Z]
         L.qk_sample_workspace_size.argtypes = [I64, I64, I, Z]
         L.qk_sample.argtypes = [P, I, I64, I64, I64, P, P, P, P, P, P, P, P, SZ, P]
         for name in ABI_SYMBOLS:

@@ -583,17 +583,18 @@ int qk_kv_compact(const qk_pages* pages, int64_t tensors, int64_t num_pages, con
  * must not be shared.  A sequence number outside [0, max_seqs), an empty tree, and one larger than the sequence are passed over:
  * accepted 0, next and path -1.  path [total], accepted and next [n].
  * A cache tensor is described by qk_rows: the row of the token at place s of page p is `pieces` pieces of piece_bytes bytes,
- * piece_stride apart, from base + p * page_stride + s * token_stride on (all in bytes).  No workspace. */
+ * piece_stride apart, from base + p * page_stride + s * token_stride on (all in bytes).  Workspace: see the query. */
 typedef struct qk_rows {
     void* base;
     int64_t page_stride, token_stride, piece_stride;
     int64_t pieces, piece_bytes;
 } qk_rows;
+int qk_kv_accept_workspace_size(int64_t n, size_t* bytes);
 int qk_kv_accept(const qk_rows* rows, int64_t tensors, int64_t num_pages, int64_t page_size, int32_t* block_table,
                  int64_t max_seqs, int64_t table_width, int64_t table_stride, int32_t* context_lens, int32_t* ref_count,
                  const int32_t* seqs, const int32_t* cu_tokens, int64_t n, int64_t total, const int32_t* tokens,
                  const int32_t* parents, const int32_t* sampled, int32_t* path, int32_t* accepted, int32_t* next,
-                 qk_stream_t stream);
+                 void* workspace, size_t workspace_bytes, qk_stream_t stream);
 
 /* ------------------------------------------------------------------ a token per row of logits
  *
