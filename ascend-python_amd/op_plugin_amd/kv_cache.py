@@ -2,14 +2,14 @@
 
 The state is three int32 tensors on the device, the page table, the sequences' lengths and a count per page, which the
 npu_kv_* ops change in place, so a serving loop never waits for the host: ``extend`` gives the slots that
-npu_mrope_scatter_kv writes and the positions it turns by, and the table and lengths go straight to npu_paged_attention and
-npu_prompt_attention.
+npu_mrope_scatter_kv writes and the positions it turns by, and the table and lengths go straight to npu_paged_attention,
+npu_prompt_attention and npu_tree_attention.
 """
 from __future__ import annotations
 
 import torch
 
-from . import (npu_kv_compact, npu_kv_copy_pages, npu_kv_extend, npu_kv_fork, npu_kv_free)
+from . import (npu_kv_accept, npu_kv_compact, npu_kv_copy_pages, npu_kv_extend, npu_kv_fork, npu_kv_free)
 
 
 class PagedKVCache:
@@ -48,6 +48,15 @@ class PagedKVCache:
         """children[i] becomes a copy of parents[i]: whole pages are shared, a started last page is copied."""
         return npu_kv_fork(self._pools(), self.block_table, self.context_lens, self.ref_count, parents, children,
                            self.page_size)
+
+    def accept(self, seqs: torch.Tensor, cu_tokens: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor,
+               sampled: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """The end of a step with drafts, whose trees (tree.py) were the last that ``extend`` made room for: of the tree of
+        seqs[i], rows cu_tokens[i] .. cu_tokens[i + 1], the way from row 0 along the tokens that were drawn (sampled[r] at
+        row r) stays, in every layer, and the rest is given back.  (path, accepted, next): which rows stay (-1 behind),
+        how many of each sequence, and the token that its next tree begins with."""
+        return npu_kv_accept(self._pools(), self.block_table, self.context_lens, self.ref_count, seqs, cu_tokens, tokens, parents,
+                             sampled, self.page_size)
 
     def free(self, seqs: torch.Tensor) -> None:
         npu_kv_free(self.block_table, self.context_lens, self.ref_count, seqs, self.page_size)
