@@ -6,7 +6,6 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
-#include <limits>
 #include <optional>
 #include <tuple>
 
@@ -33,7 +32,7 @@ void sample_check(const at::Tensor& x, const at::Tensor& uniform, const OptTenso
                 ": logits must be float16, bfloat16 or float32, got ", x.scalar_type());
     TORCH_CHECK(x.dim() == 2, kOp, ": logits must be [rows, vocabulary], got ", x.sizes());
     TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= QK_MAX_VOCAB, kOp, ": a vocabulary of 1 to ", QK_MAX_VOCAB, " tokens, got ", x.size(1));
-    TORCH_CHECK(x.size(0) <= std::numeric_limits<int32_t>::max(), kOp, ": invalid number of rows ", x.size(0));
+    TORCH_CHECK(x.size(0) <= QK_MAX_SAMPLE_ROWS, kOp, ": invalid number of rows ", x.size(0), ", at most ", QK_MAX_SAMPLE_ROWS);
     check_setting("uniform", uniform, at::kFloat, x);
     if (temperature.has_value()) check_setting("temperature", *temperature, at::kFloat, x);
     if (top_k.has_value()) check_setting("top_k", *top_k, at::kInt, x);

@@ -22,7 +22,9 @@ int fail(int code, const char* fmt, ...) {
 int check_sizes(int64_t rows, int64_t vocab, int dtype) {
     if (dtype != QK_F16 && dtype != QK_BF16 && dtype != QK_F32)
         return fail(QK_ERR_ARG, "%s: logits must be float16, bfloat16 or float32 (got dtype %d)", kOp, dtype);
-    if (rows < 0 || rows > ((int64_t)1 << 31) - 1) return fail(QK_ERR_ARG, "%s: invalid number of rows %lld", kOp, (long long)rows);
+    // a launch holds less than 2^32 threads
+    if (rows < 0 || rows > QK_MAX_SAMPLE_ROWS)
+        return fail(QK_ERR_ARG, "%s: invalid number of rows %lld (at most %d)", kOp, (long long)rows, QK_MAX_SAMPLE_ROWS);
     if (vocab < 1 || vocab > QK_MAX_VOCAB)
         return fail(QK_ERR_UNSUPPORTED, "%s: a vocabulary of 1 to %d tokens (got %lld)", kOp, QK_MAX_VOCAB, (long long)vocab);
     return QK_OK;

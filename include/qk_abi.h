@@ -583,7 +583,7 @@ int qk_kv_compact(const qk_pages* pages, int64_t tensors, int64_t num_pages, con
  * must not be shared.  A sequence number outside [0, max_seqs), an empty tree, and one larger than the sequence are passed over:
  * accepted 0, next and path -1.  path [total], accepted and next [n].
  * A cache tensor is described by qk_rows: the row of the token at place s of page p is `pieces` pieces of piece_bytes bytes,
- * piece_stride apart, from base + p * page_stride + s * token_stride on (all in bytes).  Workspace: see the query. */
+ * piece_stride apart, from base + p * page_stride + s * token_stride on (all in bytes); no two tensors share bytes.  Workspace: see the query. */
 typedef struct qk_rows {
     void* base;
     int64_t page_stride, token_stride, piece_stride;
@@ -600,7 +600,7 @@ int qk_kv_accept(const qk_rows* rows, int64_t tensors, int64_t num_pages, int64_
  *
  * npu_sample -- temperature, top-k, top-p and min-p, and a draw from a given uniform number (the reference leaves sampling
  * to the framework's own sort, cumsum and multinomial).  logits: [rows][vocab] QK_F16, QK_BF16 or QK_F32, rows row_stride
- * elements apart, vocab 1 .. QK_MAX_VOCAB.  The others are [rows] on the device; all but uniform may be NULL.
+ * elements apart, vocab 1 .. QK_MAX_VOCAB, rows up to QK_MAX_SAMPLE_ROWS.  The others are [rows] on the device; all but uniform may be NULL.
  *   w_i = exp((x_i - max x) / temperature[r])       (NULL: 1)
  * The row's tokens in order of x, falling, ties by index.  top_k[r] > 0 keeps the first so many.  top_p[r] < 1 keeps of
  * those the ones before which less than top_p of their sum of w lies.  min_p[r] > 0 keeps those with w_i >= min_p (above 1:
@@ -611,6 +611,7 @@ int qk_kv_accept(const qk_rows* rows, int64_t tensors, int64_t num_pages, int64_
  * ceil(log2 vocab), at most 50, and sums of them exact: the result does not depend on how the work is split.
  */
 #define QK_MAX_VOCAB (1 << 24)
+#define QK_MAX_SAMPLE_ROWS ((1 << 22) - 1)
 int qk_sample_workspace_size(int64_t rows, int64_t vocab, int dtype, size_t* bytes);
 int qk_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride, const float* uniform,
               const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens,

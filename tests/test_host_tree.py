@@ -102,6 +102,7 @@ def test_sample_refusals():
     _refuses(lambda: call(logits=_m((7,))), "rows, vocabulary")
     _refuses(lambda: call(logits=_m((7, 0))), "vocabulary of 1 to")
     _refuses(lambda: call(logits=_m((7, (1 << 24) + 1))), "vocabulary of 1 to")
+    _refuses(lambda: call(logits=_m((1 << 22, 2)), uniform=_m((1 << 22,), F32)), "number of rows")
     _refuses(lambda: call(uniform=_m((6,), F32)), "uniform must be")
     _refuses(lambda: call(uniform=_m((7,), BF16)), "uniform must be")
     _refuses(lambda: call(uniform=torch.zeros(7)), "uniform must be on")
@@ -152,6 +153,7 @@ def test_abi_refusals():
     assert L.qk_sample_workspace_size(3, 0, q.QK_F32, ctypes.byref(size)) == q.QK_ERR_UNSUPPORTED
     assert L.qk_sample_workspace_size(3, 100, q.QK_I8, ctypes.byref(size)) == q.QK_ERR_ARG and "float16" in q.last_error()
     assert L.qk_sample_workspace_size(-1, 100, q.QK_F32, ctypes.byref(size)) == q.QK_ERR_ARG
+    assert L.qk_sample_workspace_size(1 << 22, 100, q.QK_F32, ctypes.byref(size)) == q.QK_ERR_ARG and "at most" in q.last_error()
     assert L.qk_sample_workspace_size(3, 100, q.QK_F32, None) == q.QK_ERR_ARG
     assert L.qk_sample_workspace_size(0, 100, q.QK_F32, ctypes.byref(size)) == q.QK_OK and size.value == 0
     assert L.qk_sample_workspace_size(4, 200000, q.QK_BF16, ctypes.byref(size)) == q.QK_OK and size.value > 0
