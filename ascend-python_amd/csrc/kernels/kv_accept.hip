@@ -13,7 +13,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kTree = 1024;   // rows of a tree whose way is found in LDS; in larger ones a search in memory finds each step's child
-constexpr int kTensors = 64;  // tensors per launch: 3072 bytes of arguments
+constexpr int kTensors = 64;  // tensors per launch: 48 bytes of arguments each, of the 4 KB that a launch has
 constexpr int kAhead = 8;     // rows of a column in flight
 
 struct RowList {

@@ -10,6 +10,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
 #include <limits>
 #include <optional>
@@ -707,7 +708,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> npu_kv_extend_meta(const at::Tens
     return {at::empty({total}, table.options()), at::empty({total}, table.options()), at::empty({1}, table.options())};
 }
 
-// A token's row in each cache tensor: its dimensions behind pages and tokens, as pieces of whole bytes that lie one apart.
+// A token's row in each cache tensor: its dimensions behind pages and tokens, as pieces of whole bytes that lie one apart.  A tensor
+// that is there twice (layers that share a cache) is listed once: its rows move once.
 std::vector<qk_rows> row_list(const char* op, at::TensorList caches, int64_t num_pages, int64_t page_size, const at::Tensor& like) {
     std::vector<qk_rows> list;
     list.reserve(caches.size());
@@ -748,7 +750,19 @@ std::vector<qk_rows> row_list(const char* op, at::TensorList caches, int64_t num
         list.push_back(r);
         last = &t;
     }
-    return list;
+    const auto first = [](const qk_rows& a, const qk_rows& b) { return a.base < b.base; };
+    const auto same = [](const qk_rows& a, const qk_rows& b) { return a.base && a.base == b.base; };
+    std::vector<qk_rows> by_base = list;
+    std::sort(by_base.begin(), by_base.end(), first);
+    if (std::adjacent_find(by_base.begin(), by_base.end(), same) == by_base.end()) return list;
+    for (size_t i = 1; i < by_base.size(); ++i) {
+        const qk_rows &a = by_base[i - 1], &b = by_base[i];
+        TORCH_CHECK(!same(a, b) || (a.page_stride == b.page_stride && a.token_stride == b.token_stride && a.pieces == b.pieces &&
+                                    a.piece_bytes == b.piece_bytes && (a.pieces == 1 || a.piece_stride == b.piece_stride)),
+                    op, ": cache tensors of different layouts begin at one place");
+    }
+    by_base.erase(std::unique(by_base.begin(), by_base.end(), same), by_base.end());
+    return by_base;
 }
 
 void accept_check(const char* op, const at::Tensor& table, const at::Tensor& lens, const at::Tensor& count, const at::Tensor& seqs,

@@ -54,7 +54,8 @@ class PagedKVCache:
         """The end of a step with drafts, whose trees (tree.py) were the last that ``extend`` made room for: of the tree of
         seqs[i], rows cu_tokens[i] .. cu_tokens[i + 1], the way from row 0 along the tokens that were drawn (sampled[r] at
         row r) stays, in every layer, and the rest is given back.  (path, accepted, next): which rows stay (-1 behind),
-        how many of each sequence, and the token that its next tree begins with."""
+        how many of each sequence, and the token that its next tree begins with.  Where ``extend`` found no room there are no
+        trees: a step that does not wait for ``missing`` passes all sequences over then, as tree.py shows."""
         return npu_kv_accept(self._pools(), self.block_table, self.context_lens, self.ref_count, seqs, cu_tokens, tokens, parents,
                              sampled, self.page_size)
 

@@ -3,7 +3,8 @@
 A sequence's tree is its rows cu_tokens[i] .. cu_tokens[i + 1]: row 0 is the token drawn last, every other one a draft that follows
 row parents[r] of its tree, a lower one.  One step, on the device throughout:
 
-    slots, positions, _ = cache.extend(seqs, cu_tokens, total)
+    slots, positions, missing = cache.extend(seqs, cu_tokens, total)
+    seqs = torch.where(missing == 0, seqs, -1)                     # no room: nothing was added, every sequence is passed over
     mask, depth = tree_mask(parents, cu_tokens, words)             # once for all steps whose trees are alike
     positions = tree_positions(positions, cu_tokens, depth)
     x = quant_attention(..., slots, positions, ..., tree_mask=mask)  # in every layer

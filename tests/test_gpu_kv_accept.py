@@ -207,6 +207,29 @@ def test_strided_tensors(ops, form):
     assert torch.equal(dev.cpu(), whole) and torch.equal(td.cpu(), table) and torch.equal(ld.cpu(), lens)
 
 
+@pytest.mark.parametrize("layers", [3, 70])
+def test_tensors_that_are_there_twice(ops, layers):
+    """Layers that share a cache: a row moves once."""
+    print(f"[case] accept twice {layers}", flush=True)
+    rng, g = random.Random(2), torch.Generator().manual_seed(2)
+    page, sizes, past = 16, [40, 30], [9, 40]
+    table, lens, count, P = _state(g, [a + b for a, b in zip(sizes, past)], page)
+    caches = [torch.randn((P, page, 2, 64), generator=g) for _ in range(2)]
+    trees = [_tree(rng, n, right=1.0) for n in sizes]
+    tokens, parents, sampled = ([v for t in trees for v in t[i]] for i in range(3))
+    dev = [c.to(DEV) for c in caches]
+    td, ld, cd = table.to(DEV), lens.to(DEV), count.to(DEV)
+    want = _expect(caches, table, lens, count, page, [0, 1], [0, 40, 70], tokens, parents, sampled)
+    path, accepted, nxt = ops.npu_kv_accept(dev * layers, td, ld, cd, _ints([0, 1]), _ints([0, 40, 70]), _ints(tokens), _ints(parents),
+                                            _ints(sampled), page)
+    assert path.tolist() == want[0] and accepted.tolist() == want[1] and nxt.tolist() == want[2] and min(want[1]) >= 3
+    for a, b in zip(dev, caches):
+        assert torch.equal(a.cpu(), b)
+    with pytest.raises(RuntimeError, match="begin at one place"):
+        ops.npu_kv_accept([dev[0], dev[0][:, :, :1]], td, ld, cd, _ints([0, 1]), _ints([0, 40, 70]), _ints(tokens), _ints(parents),
+                          _ints(sampled), page)
+
+
 def test_bad_pages(ops):
     """A page id outside the pool is not followed: its rows stay, the others move, and it is not counted."""
     print("[case] accept bad pages", flush=True)

@@ -258,3 +258,29 @@ def test_step_as_a_graph(q, kind):
         for a, b in zip(state[3:], after[3:]):
             assert torch.equal(a[held].view(torch.uint8), b[held].view(torch.uint8)), turn
         roots = want[6].tolist()
+
+
+def test_step_without_room(q):
+    """A step that finds no pages leaves everything as it was where its sequences are passed over for it."""
+    print("[case] step without room", flush=True)
+    from op_plugin_amd.tree import tree_mask, tree_positions
+    m = Decoder(q, BF16)
+    m.prompt([0], [[1] * 50])
+    c = m.cache
+    c.ref_count[c.ref_count == 0] = 1  # every other page is somebody's
+    start = [t.clone() for t in (c.block_table, c.context_lens, c.ref_count)]
+    held = m.held(0, 50)
+    parents, tokens = (_ints(v) for v in _tree(random.Random(3), 30))
+    seqs, cu = _ints([0]), _ints([0, 30])
+    slots, positions, missing = c.extend(seqs, cu, 30)
+    assert int(missing) > 0 and (slots == -1).all()
+    seqs = torch.where(missing == 0, seqs, -1)
+    mask, depth = tree_mask(parents, cu)
+    out = m.block(m.embedding[tokens.long()], 0, seqs, cu, slots, tree_positions(positions, cu, depth), c.rows(seqs), mask)
+    assert (out == 0).all()
+    path, accepted, nxt = c.accept(seqs, cu, tokens, parents, tokens)
+    assert (path == -1).all() and accepted.tolist() == [0] and nxt.tolist() == [-1]
+    for a, b in zip((c.block_table, c.context_lens, c.ref_count), start):
+        assert torch.equal(a, b)
+    for a, b in zip(m.held(0, 50), held):
+        assert torch.equal(a, b)
