@@ -5,16 +5,22 @@
 // which they are made, so the same call gives the same token however the work is split.  F = 62 - log2(vocab), at most 50: what is
 // rounded away is below 2^-(F + 1) of the largest weight each.
 //
-// Bound by HBM for many rows (each logit is read from it once), by latency for few.  No row is sorted.  A row is cut into segments of 256
-// 16-byte vectors, a wave's step, and the segments dealt to workgroups; what one knows of its part goes to the last of the row's
-// to arrive:
+// Each logit is read from HBM once, and once or twice more from the caches; no row is sorted.  A row is cut into segments of one
+// 16-byte vector a lane of a wave (four where there would be more than 1024 of them), and the segments dealt to workgroups; what one
+// knows of its part goes to the last of the row's to arrive:
 //   look   the largest logit; where a filter cuts, a histogram of the logits in bins of 1/64 of the temperature below the part's
 //          largest, counts and weights (near enough: in units of the bin's upper end).  The last one joins them and finds the
 //          bins in which the border of the kept tokens lies: counts are exact, and a border in the weights is bracketed.
 //   draw   exact sums of the bins above those, by segment, and a list of the tokens in them.  The last one sorts the
 //          list, finds the border in exact sums, the segment in which the drawn number falls, and the token there.
 // A row whose list would be too long, or whose border is not where the histogram put it, is done by one workgroup that finds each border
-// in the logits' bits, eleven at a time.  Rows that fill the card by themselves go through both steps in one launch.
+// in the logits' bits, eleven at a time.  Rows that fill the card by themselves, and short ones, go through both steps in one launch.
+//
+// What bounds it: one row, the chain of steps (two launches, a join each, thresholds searched among the logits, a sort): a row of
+// 65536 takes 15 us without filters and 38 with all three, and eight times the tokens half as much again.  Many rows, the vector units: an exact weight is
+// 21 instructions in 64 bits, which a nucleus asks of every logit (its goal is a part of the exact sum), and the histogram an
+// atomic in LDS each.  Measured on one MI355X: 96 rows of 65536 without filters 24 us (0.52 TB/s; most is one workgroup's 65536
+// weights); 256 rows of 131072 under nuclei and min_p 94 us; 48 of 128257 in 32 bits under all three 46 us; one row of 32001 30 us.
 #include "sample.h"
 
 namespace qk {
@@ -26,6 +32,7 @@ constexpr int kBins = 2048;      // of the histograms
 constexpr int kPerUnit = 64;     // bins per temperature
 constexpr float kSlope = 0.0155038f;  // 1 - e^(-1 / 64): what a weight falls in a bin
 constexpr int kList = 4096;      // tokens in the border's bins
+constexpr int kAhead = 4;        // parts' histograms that are read at a time
 constexpr int kBatch = 4;        // 16-byte vectors that a lane asks for at a time
 constexpr int kSegments = 1024;  // of a row at most
 constexpr int64_t kMostTokens = 1 << 20;  // of a row that is split: a bin's count and weight share 64 bits
@@ -983,12 +990,20 @@ __global__ __launch_bounds__(kThreads) void sample_look(SplitArgs g) {
         p = plan_row(s, top, g.bits, valid, sh, group, [&](int b, uint32_t& count, float& weight) {
             count = 0;
             weight = 0.0f;
-            for (int c = 0; c < g.groups; ++c) {
-                const int32_t at = b - sh.shift[c];
-                if (at < 0) continue;
-                const uint64_t v = get(bins + (int64_t)c * kBins + at);
-                count += (uint32_t)(v >> 40);
-                weight += (float)(v & ((1ull << 40) - 1)) * 0x1p-20f;
+            for (int c0 = 0; c0 < g.groups; c0 += kAhead) {
+                uint64_t v[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int c = c0 + k < g.groups ? c0 + k : c0;
+                    const int32_t at = c0 + k < g.groups ? b - sh.shift[c] : -1;
+                    v[k] = get(bins + (int64_t)c * kBins + (at < 0 ? 0 : at));
+                    if (at < 0) v[k] = 0;
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    count += (uint32_t)(v[k] >> 40);
+                    weight += (float)(v[k] & ((1ull << 40) - 1)) * 0x1p-20f;
+                }
             }
         });
     }
@@ -1013,30 +1028,30 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SplitArgs g) {
     const Settings s = settings_of(a, r);
     bool alone = p.mode == kAlone;
     if (!alone) {
-    const Weights w = weights_of(s, p.top, g.bits);
-    const int32_t seg0 = which * g.per_group, seg1 = seg0 + g.per_group < g.segments ? seg0 + g.per_group : g.segments;
-    uint64_t* const kept = g.kept + r * g.segments;
-    uint64_t* const list = g.list + r * kList;
-    Drawn* const sums = g.sums + r * g.groups;
-    Drawn d = draw_part(row, s, w, p, seg0, seg1, sh, group, [&](int32_t at, uint64_t sum) { put(kept + at, sum); });
-    const uint32_t own = sh.listed < (uint32_t)kList ? sh.listed : kList;
-    if (tid == 0) {
-        put(&sums[which].all, d.all);
-        put(&sums[which].above, d.above);
-        sh.base = own ? __hip_atomic_fetch_add(g.listed + r, own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
-    }
-    __syncthreads();
-    for (uint32_t i = tid; i < own; i += kThreads)
-        if (sh.base + i < (uint32_t)kList) put(list + sh.base + i, sh.list[i]);
-    if (!splitk_last(g.draw_arrivals + r, (uint32_t)g.groups, g.tag)) return;
+        const Weights w = weights_of(s, p.top, g.bits);
+        const int32_t seg0 = which * g.per_group, seg1 = seg0 + g.per_group < g.segments ? seg0 + g.per_group : g.segments;
+        uint64_t* const kept = g.kept + r * g.segments;
+        uint64_t* const list = g.list + r * kList;
+        Drawn* const sums = g.sums + r * g.groups;
+        Drawn d = draw_part(row, s, w, p, seg0, seg1, sh, group, [&](int32_t at, uint64_t sum) { put(kept + at, sum); });
+        const uint32_t own = sh.listed < (uint32_t)kList ? sh.listed : kList;
+        if (tid == 0) {
+            put(&sums[which].all, d.all);
+            put(&sums[which].above, d.above);
+            sh.base = own ? __hip_atomic_fetch_add(g.listed + r, own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < own; i += kThreads)
+            if (sh.base + i < (uint32_t)kList) put(list + sh.base + i, sh.list[i]);
+        if (!splitk_last(g.draw_arrivals + r, (uint32_t)g.groups, g.tag)) return;
 
-    uint32_t listed = get(g.listed + r);
-    listed = listed < (uint32_t)kList ? listed : kList;
-    for (uint32_t i = tid; i < listed; i += kThreads) sh.list[i] = get(list + i);
-    for (int32_t i = tid; i < g.segments; i += kThreads) sh.kept[i] = get(kept + i);
-    d.all = group.sum(tid < g.groups ? get(&sums[tid].all) : 0);
-    d.above = group.sum(tid < g.groups ? get(&sums[tid].above) : 0);
-    alone = !draw_row(a, r, row, s, w, g.bits, p, d, g.segments, listed, sh, group);
+        uint32_t listed = get(g.listed + r);
+        listed = listed < (uint32_t)kList ? listed : kList;
+        for (uint32_t i = tid; i < listed; i += kThreads) sh.list[i] = get(list + i);
+        for (int32_t i = tid; i < g.segments; i += kThreads) sh.kept[i] = get(kept + i);
+        d.all = group.sum(tid < g.groups ? get(&sums[tid].all) : 0);
+        d.above = group.sum(tid < g.groups ? get(&sums[tid].above) : 0);
+        alone = !draw_row(a, r, row, s, w, g.bits, p, d, g.segments, listed, sh, group);
     }
     if (alone) draw_alone<DT>(a, r, row.start(), s, p.top, g.bits, space.digits, group);
 }
@@ -1050,30 +1065,34 @@ int weight_bits(int64_t vocab) {
     return 62 - bits < 50 ? 62 - bits : 50;
 }
 
-// A row is split over workgroups where that makes three parts at least of each and the parts fill the card once: two launches and
-// their joins cost what a workgroup needs for some 30000 tokens.
-constexpr int64_t kWanted = 256, kLeastGroups = 3;
-
-// Rows up to so many tokens have short segments: their few vectors spread over more waves.
-constexpr int64_t kShortRow = 65536;
+// A row is split over workgroups where the parts fill the card once: two launches and their joins cost what a workgroup needs for some
+// 35000 tokens (one row of 32001 16-bit logits under all filters, split 30.9 us, in one launch 29.8; of 40000 32.2 and 34.3; of
+// 131072 32-bit ones 37 and 72), so neither shorter rows are, nor rows that would have two parts each (120 rows of 131072 without
+// filters 49.0 us, in one launch 43.2; 96 of 65536 28.2 and 24.1; with filters two parts are 3% faster).  Past some 24 parts the
+// joins take longer than the parts gain (one row of 200000 under all filters: up to 24 38.8 us, 32 40.0, one a segment of each wave 47).
+constexpr int64_t kWanted = 256, kLeastGroups = 3, kMostGroups = 24, kLeastSplit = 32769;
 
 struct Split {
-    bool small;
+    // Segments of one vector a lane: few vectors spread over more waves and workgroups (one row of 65536 without filters 15 us, with
+    // segments of four 21; of 20000 in one launch 10.7 and 12.6; rows that fill the card alike).
+    bool fine;
     int32_t segments, per_group;
     int64_t groups;
     int64_t arrivals, plans, listed, parts, bins, sums, kept, list, bytes;  // offsets in the workspace
 };
 Split split(int64_t rows, int64_t vocab, int dtype) {
     Split p = {};
-    p.small = vocab <= kShortRow;
     p.groups = 1;
     if (vocab > kMostTokens - 8) return p;
-    const int64_t per = dtype == QK_F32 ? 4 : 8, segment = 64 * (p.small ? 1 : kBatch);
+    const int64_t per = dtype == QK_F32 ? 4 : 8;
     const int64_t most = (vocab + per - 1 + per - 1) / per;  // vectors of a row that begins with the last element of one
+    p.fine = most <= 64 * kSegments;
+    const int64_t segment = 64 * (p.fine ? 1 : kBatch);
     p.segments = (int32_t)((most + segment - 1) / segment);
     const int64_t steps = (p.segments + kWaves - 1) / kWaves;  // of a workgroup that has all
     int64_t groups = kWanted / rows;
-    if (groups < kLeastGroups) return p;
+    if (groups < kLeastGroups || vocab < kLeastSplit) return p;
+    groups = groups < kMostGroups ? groups : kMostGroups;
     groups = groups < steps ? groups : steps;
     p.per_group = (int32_t)((steps + groups - 1) / groups) * kWaves;
     p.groups = (p.segments + p.per_group - 1) / p.per_group;
@@ -1128,7 +1147,7 @@ hipError_t launch_steps(const SampleArgs& a, const Split& p, void* workspace, hi
 template <int DT>
 hipError_t launch(const SampleArgs& a, void* workspace, hipStream_t stream) {
     const Split p = split(a.rows, a.vocab, a.dtype);
-    return p.small ? launch_steps<DT, 1>(a, p, workspace, stream) : launch_steps<DT, kBatch>(a, p, workspace, stream);
+    return p.fine ? launch_steps<DT, 1>(a, p, workspace, stream) : launch_steps<DT, kBatch>(a, p, workspace, stream);
 }
 
 }  // namespace
