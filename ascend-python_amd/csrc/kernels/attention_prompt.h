@@ -43,8 +43,10 @@ constexpr int kSplitTiles = 8;
 // Workgroups that the card holds, two per CU; cutting up to 768 or 1024 takes longer where tiles are nearly enough (1500
 // tokens 41.5 -> 46.9 us, chunks with a window 64 -> 69).
 constexpr int64_t kResident = 512;
-// Trees: a part's steps at least; parts that are joined by one workgroup, and in groups of how many where there are more; and at
-// most (128 parts are 32 groups of 4; 512, all that there are, 16 of 32).
+// Trees: a part's steps at least (7 drafted tokens over 997: of four 15.2 us, of eight 17.8; of two no faster anywhere); parts that
+// are joined by one workgroup, and in groups of how many where there are more (two trees of 117 over 6001, all at once 38.4 us, in
+// two steps 32.2; 24 trees up to 16 over 8191 38.2 and 36.8); and at most (128 parts are 32 groups of 4; 512, all that there are,
+// 16 of 32).
 constexpr int kTreeSteps = 4;
 constexpr int kJoinAtOnce = 8, kJoinGroup = 4, kJoined = 32;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -793,6 +795,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attention_prompt(
             if (it + 1 < tiles) step(it + 1, xb, xa);
         }
     }
+    // what was sent for past the last tile has come: it would land in LDS that is used for something else
+    if constexpr (!Q8) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
 
     l = pair_sum(l);
     if constexpr (HALF) {
