@@ -14,13 +14,15 @@
 //   draw   exact sums of the bins above those, by segment, and a list of the tokens in them.  The last one sorts the
 //          list, finds the border in exact sums, the segment in which the drawn number falls, and the token there.
 // A row whose list would be too long, or whose border is not where the histogram put it, is done by one workgroup that finds each border
-// in the logits' bits, eleven at a time.  Rows that fill the card by themselves, and short ones, go through both steps in one launch.
+// in the logits' bits, eleven at a time.  Rows that fill the card by themselves, and short ones, go through both steps in one workgroup; in
+rows whose look is little beside their draw each workgroup looks at the whole row, and one launch does (way_of).
 //
-// What bounds it: one row, the chain of steps (two launches, a join each, thresholds searched among the logits, a sort): a row of
-// 65536 takes 15 us without filters and 38 with all three, and eight times the tokens half as much again.  Many rows, the vector units: an exact weight is
-// 21 instructions in 64 bits, which a nucleus asks of every logit (its goal is a part of the exact sum), and the histogram an
-// atomic in LDS each.  Measured on one MI355X: 96 rows of 65536 without filters 24 us (0.52 TB/s; most is one workgroup's 65536
-// weights); 256 rows of 131072 under nuclei and min_p 94 us; 48 of 128257 in 32 bits under all three 46 us; one row of 32001 30 us.
+// What bounds it: one row, the chain of steps (passes over the row, thresholds searched among the logits, a sort, scans): a row of
+// 65536 takes 10 us without filters and 37 with all three, and twice the tokens 12 and 37.  Many rows, the vector units: an exact
+// weight is 21 instructions in 64 bits, which a nucleus asks of every logit (its goal is a part of the exact sum), and the histogram an
+// atomic in LDS each.  Measured on one MI355X: 96 rows of 65536 without filters 18.6 us (0.68 TB/s); 256 rows of 131072 under nuclei
+// and min_p 94 us, of which the first pass takes 11, the histogram 17, the exact weights 45; 48 of 128257 in 32 bits under all three
+// 46 us; one row of 32001 29 us.
 #include "sample.h"
 
 namespace qk {
@@ -61,10 +63,10 @@ __device__ __forceinline__ double fma_scalar(double a, double b, double c) {
     asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
     return d;
 }
-// 2^t times 2^bits as a whole number, 0 where t is below -60 or NaN (t <= 0): 2^n times a polynomial in f = t - n, |f| <= 1/2, that
-// meets 2^f in the 11 Chebyshev nodes and stays within 2^-51 of it; rounded by adding 2^(52 - bits), in whose last bits the number
-// then stands.
-__device__ __forceinline__ uint64_t weight_of_log2(double t, int bits) {
+// 2^t + unit, unit being the power of two 2^(52 - bits): the last bits of it are then 2^t times 2^bits as a whole number, 0 where t is
+// below -60 or NaN (t <= 0).  2^n times a polynomial in f = t - n, |f| <= 1/2, that meets 2^f in the 11 Chebyshev nodes and stays
+// within 2^-51 of it; n is found by an addition whose last bits it is, and goes to the exponent as a whole number.
+__device__ __forceinline__ uint64_t raw_weight(double t, double unit) {
     double c, p;
     asm("v_max_f64 %0, %1, %2" : "=v"(c) : "v"(t), "s"(-60.0));
     const double n = __builtin_rint(c), f = c - n;
@@ -78,7 +80,7 @@ __device__ __forceinline__ uint64_t weight_of_log2(double t, int bits) {
     p = fma_scalar(p, f, 0x1.ebfbdff82c598p-3);
     p = fma_scalar(p, f, 0x1.62e42fefa3a19p-1);
     p = __builtin_fma(p, f, 1.0);
-    return __builtin_bit_cast(uint64_t, __builtin_ldexp(p, (int)n) + __builtin_ldexp(1.0, 52 - bits)) & 0xfffffffffffffull;
+    return __builtin_bit_cast(uint64_t, __builtin_ldexp(p, (int)n) + unit);
 }
 
 // Weights of a row whose largest logit is `top`.
@@ -86,16 +88,19 @@ struct Weights {
     double top, factor;  // log2 e / temperature
     int bits;            // F: the largest weight is 2^F
     bool infinite;       // top is: equal weights for its like, none for the others
+    double unit;         // 2^(52 - bits)
 
     // log2 of a logit's weight in a row without an infinite one (-inf: -inf, or NaN where the temperature is infinite)
     __device__ __forceinline__ double finite_log2(float x) const { return ((double)x - top) * factor; }
-    __device__ __forceinline__ uint64_t finite(float x) const { return weight_of_log2(finite_log2(x), bits); }
+    __device__ __forceinline__ uint64_t whole(uint64_t raw) const { return raw & 0xfffffffffffffull; }
+    __device__ __forceinline__ uint64_t raw(float x) const { return raw_weight(finite_log2(x), unit); }  // with the bits of `unit` on top
+    __device__ __forceinline__ uint64_t finite(float x) const { return whole(raw(x)); }
     // ... in any row
     __device__ __forceinline__ double log2_of(float x) const {
         if (infinite) return x == __builtin_inff() ? 0.0 : -__builtin_inf();
         return finite_log2(x);
     }
-    __device__ __forceinline__ uint64_t of(uint32_t key) const { return key < kLeast ? 0 : weight_of_log2(log2_of(value_of(key)), bits); }
+    __device__ __forceinline__ uint64_t of(uint32_t key) const { return key < kLeast ? 0 : whole(raw_weight(log2_of(value_of(key)), unit)); }
 };
 
 // ---------------------------------------------------------------- sums over a workgroup
@@ -196,7 +201,7 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int64_t r) 
     return s;
 }
 __device__ __forceinline__ Weights weights_of(const Settings& s, float top, int bits) {
-    return {(double)top, s.greedy ? 0.0 : 1.44269504088896340736 / (double)s.temperature, bits, top == __builtin_inff()};
+    return {(double)top, s.greedy ? 0.0 : 1.44269504088896340736 / (double)s.temperature, bits, top == __builtin_inff(), __builtin_ldexp(1.0, 52 - bits)};
 }
 // The least log2 of a weight that min_p keeps
 __device__ __forceinline__ double least_of(const Settings& s) {
@@ -640,35 +645,43 @@ __device__ __forceinline__ Drawn draw_part(const R& row, const Settings& s, cons
     constexpr int kPer = R::kPer;
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    const bool whole_sum = p.mode == kCut && s.top_p < 1.0f && p.top_k == 0, min_p = s.min_p > 0.0f;
-    const float keep = fmaxf(p.keep, p.above);
+    const bool cut = p.mode == kCut, min_p = s.min_p > 0.0f;
+    const bool whole_sum = cut && s.top_p < 1.0f && p.top_k == 0;
+    const bool plain = !cut && !min_p;                   // every logit counts (-inf and NaN: weight 0)
+    const float keep = fmaxf(p.keep, p.above), from = cut ? p.above : keep;
+    const uint64_t unit = __builtin_bit_cast(uint64_t, w.unit);
     Drawn d = {0, 0};
-    uint64_t above = 0, kept = 0;
+    uint64_t sum = 0, above = 0, kept = 0;  // sum: with `added` units on top
+    uint32_t added = 0;
     row.each(
         seg0, seg1,
         [&](int32_t first, const float (&x)[kPer]) {
-            bool some = whole_sum, listed = false;
+            float top = x[0];
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                some |= x[e] >= p.above;
-                listed |= x[e] < p.above && x[e] >= p.listed;
-            }
-            if (__builtin_amdgcn_ballot_w64(some)) {
-                uint64_t weight[kPer];
+            for (int e = 1; e < kPer; ++e) top = fmaxf(top, x[e]);
+            const bool some = !plain && __builtin_amdgcn_ballot_w64(top >= from);
+            auto add = [&](float v, uint64_t raw) {
+                above += v >= p.above ? w.whole(raw) : 0;
+                if (min_p) kept += v >= keep ? w.whole(raw) : 0;
+            };
+            if (whole_sum || plain) {
+                uint64_t raw[kPer];
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) weight[e] = w.finite(x[e]);
-                if (whole_sum) {
+                for (int e = 0; e < kPer; ++e) raw[e] = w.raw(x[e]);
 #pragma unroll
-                    for (int e = 0; e < kPer; ++e) d.all += weight[e];
+                for (int e = 0; e < kPer; ++e) sum += raw[e];
+                added += kPer;
+                if (some) {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) add(x[e], raw[e]);
                 }
+            } else if (some) {
+                // a few hundred of a row's tokens: most elements of a vector have none
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) above += x[e] >= p.above ? weight[e] : 0;
-                if (min_p) {
-#pragma unroll
-                    for (int e = 0; e < kPer; ++e) kept += x[e] >= keep ? weight[e] : 0;
-                }
+                for (int e = 0; e < kPer; ++e)
+                    if (__builtin_amdgcn_ballot_w64(x[e] >= from)) add(x[e], w.raw(x[e]));
             }
-            if (listed) {
+            if (cut && top >= p.listed) {
 #pragma unroll
                 for (int e = 0; e < kPer; ++e)
                     if (x[e] < p.above && x[e] >= p.listed) {
@@ -678,13 +691,18 @@ __device__ __forceinline__ Drawn draw_part(const R& row, const Settings& s, cons
             }
         },
         [&](int32_t g) {
-            const uint64_t sum = last_lane(wave_upto(min_p ? kept : above));
-            if ((threadIdx.x & 63) == 0) segment_sum(g, sum);
+            if (plain) {
+                above = sum - added * unit;
+                sum = 0;
+                added = 0;
+            }
+            const uint64_t of_segment = last_lane(wave_upto(min_p ? kept : above));
+            if ((threadIdx.x & 63) == 0) segment_sum(g, of_segment);
             d.above += above;
             above = kept = 0;
         });
-    if (p.mode == kCut) {
-        d.all = whole_sum ? group.sum(d.all) : 0;
+    if (cut) {
+        d.all = whole_sum ? group.sum(sum - added * unit) : 0;
         d.above = group.sum(d.above);
     } else {
         __syncthreads();
@@ -1056,6 +1074,77 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SplitArgs g) {
     if (alone) draw_alone<DT>(a, r, row.start(), s, p.top, g.bits, space.digits, group);
 }
 
+// Rows that are looked at as a whole by each of their workgroups, which draw from a part: one launch.  CUT: there may be a top_k or a top_p.
+template <int DT, int STEPS, bool CUT>
+__global__ __launch_bounds__(kThreads, 4) void sample_parts(SplitArgs g) {
+    __shared__ Space space;
+    __shared__ Group::Space shared;
+    Group group = {shared};
+    Draw& sh = space.draw;
+    const SampleArgs& a = g.a;
+    const int64_t r = blockIdx.x / (uint32_t)g.groups;
+    const int which = (int)(blockIdx.x % (uint32_t)g.groups), tid = threadIdx.x;
+    const Row<DT, STEPS> row(a, r);
+    const Settings s = settings_of(a, r);
+    if (s.greedy && which > 0) return;
+    const bool histogram = CUT && cuts(s, a.vocab);
+    const Part part = look_at(row, s, histogram, 0, g.segments, space.look, group);
+    Plan p = {kAlone, 0, 0, part.top, 0.0f, 0.0f, 0.0f};
+    if (part.top == -__builtin_inff()) {
+        p.mode = kDone;
+    } else if (part.top == __builtin_inff()) {
+    } else if (!histogram) {
+        p = plan_of(s, part.top, g.bits);
+    } else {
+        p = plan_row(s, part.top, g.bits, part.valid, space.look, group, [&](int b, uint32_t& count, float& weight) {
+            const uint64_t v = space.look.bins[b];
+            count = (uint32_t)(v >> 40);
+            weight = (float)(v & ((1ull << 40) - 1)) * 0x1p-20f;
+        });
+    }
+    // (the same in all of the row's workgroups)
+    if (which > 0 && (p.mode == kDone || p.mode == kAlone)) return;
+    if (p.mode == kDone) return write_plain(a, r, -1);
+    if (s.greedy) return write_plain(a, r, (int32_t)part.first);
+    __syncthreads();  // of the histogram
+    bool alone = p.mode == kAlone;
+    if (!alone) {
+        const Weights w = weights_of(s, p.top, g.bits);
+        const int32_t seg0 = which * g.per_group, seg1 = seg0 + g.per_group < g.segments ? seg0 + g.per_group : g.segments;
+        uint64_t* const kept = g.kept + r * g.segments;
+        uint64_t* const list = g.list + r * g.groups * kList;
+        Part* const parts = g.parts + r * g.groups;
+        Drawn* const sums = g.sums + r * g.groups;
+        Drawn d = draw_part(row, s, w, p, seg0, seg1, sh, group, [&](int32_t at, uint64_t sum) { put(kept + at, sum); });
+        if (CUT && p.mode == kCut) {
+            const uint32_t own = sh.listed < (uint32_t)kList ? sh.listed : kList;
+            if (tid == 0) {
+                put(&sums[which].all, d.all);
+                put(&sums[which].above, d.above);
+                put(&parts[which].valid, own);
+            }
+            for (uint32_t i = tid; i < own; i += kThreads) put(list + (int64_t)which * kList + i, sh.list[i]);
+        }
+        if (!splitk_last(g.draw_arrivals + r, (uint32_t)g.groups, g.tag)) return;
+
+        uint32_t listed = 0;
+        if (CUT && p.mode == kCut) {
+            for (int c = 0; c < g.groups; ++c) {
+                const uint32_t n = get(&parts[c].valid);
+                for (uint32_t i = tid; i < n; i += kThreads)
+                    if (listed + i < (uint32_t)kList) sh.list[listed + i] = get(list + (int64_t)c * kList + i);
+                listed = listed + n < (uint32_t)kList ? listed + n : kList;
+            }
+            d.all = group.sum(tid < g.groups ? get(&sums[tid].all) : 0);
+            d.above = group.sum(tid < g.groups ? get(&sums[tid].above) : 0);
+        }
+        for (int32_t i = tid; i < g.segments; i += kThreads) sh.kept[i] = get(kept + i);
+        if (!CUT) p.mode = kWhole;  // (it is: told to the compiler)
+        alone = !draw_row(a, r, row, s, w, g.bits, p, d, g.segments, listed, sh, group);
+    }
+    if (alone) draw_alone<DT>(a, r, row.start(), s, p.top, g.bits, space.digits, group);
+}
+
 // ---------------------------------------------------------------- host
 
 // F of the weights: the sum of `vocab` of them stays below 2^63.
@@ -1065,12 +1154,26 @@ int weight_bits(int64_t vocab) {
     return 62 - bits < 50 ? 62 - bits : 50;
 }
 
-// A row is split over workgroups where the parts fill the card once: two launches and their joins cost what a workgroup needs for some
-// 35000 tokens (one row of 32001 16-bit logits under all filters, split 30.9 us, in one launch 29.8; of 40000 32.2 and 34.3; of
-// 131072 32-bit ones 37 and 72), so neither shorter rows are, nor rows that would have two parts each (120 rows of 131072 without
-// filters 49.0 us, in one launch 43.2; 96 of 65536 28.2 and 24.1; with filters two parts are 3% faster).  Past some 24 parts the
-// joins take longer than the parts gain (one row of 200000 under all filters: up to 24 38.8 us, 32 40.0, one a segment of each wave 47).
-constexpr int64_t kWanted = 256, kLeastGroups = 3, kMostGroups = 24, kLeastSplit = 32769;
+// A row is split over workgroups where the parts fill the card once, at most 24 of them (one row of 200000 under all filters: up to 24
+// parts 38.8 us, 32 40.0, one for every segment of a wave 47), in one of two ways:
+//   apart  look and draw are both dealt, two launches with a join each.  It takes three parts (120 rows of 131072 without filters in two
+//          49.0 us, in one launch without parts 43.2), and long rows.
+//   whole  one launch, every workgroup looks at the whole row and draws from its part.
+// Without top_k and top_p a look is a pass for the largest logit, little beside the exact weights: whole up to 131072 tokens (one row of
+// 65536 10.3 us, apart 14.8; of 131072 12.0 and 15.4; of 260000 16.7 and 16.9, in 32 bits 21.1 and 16.4), and where there are two parts (96
+// rows of 65536 18.7, in one part 22.1; 128 of 260000 51 and 71); shorter rows than 16384 are done faster in one part (10000: 7.9 and 8.2).
+// With them it is a histogram: whole from 28672 to 49152 tokens (48 rows of 32001 under all filters 32.9, in one part 34.7; one 28.6 and
+// 29.8; of 20000 26.4 and 24.5; of 65536 39.9, apart 37.2), and in two parts past 98304 (128 rows of 131072 70 and 79; 100 of 65536 51.8 and
+// 49.3).
+constexpr int64_t kWanted = 256, kLeastApart = 3, kMostGroups = 24;
+enum class Way { one, whole, apart };
+Way way_of(int64_t rows, int64_t vocab, bool cut) {
+    const int64_t groups = kWanted / rows;
+    if (vocab > kMostTokens - 8 || groups < 2 || vocab < (cut ? 28672 : 16384)) return Way::one;
+    if (vocab <= (cut ? 49152 : 1 << 17)) return Way::whole;
+    if (groups >= kLeastApart) return Way::apart;
+    return !cut || vocab > 98304 ? Way::whole : Way::one;
+}
 
 struct Split {
     // Segments of one vector a lane: few vectors spread over more waves and workgroups (one row of 65536 without filters 15 us, with
@@ -1080,7 +1183,7 @@ struct Split {
     int64_t groups;
     int64_t arrivals, plans, listed, parts, bins, sums, kept, list, bytes;  // offsets in the workspace
 };
-Split split(int64_t rows, int64_t vocab, int dtype) {
+Split split(int64_t rows, int64_t vocab, int dtype, Way way) {
     Split p = {};
     p.groups = 1;
     if (vocab > kMostTokens - 8) return p;
@@ -1089,9 +1192,9 @@ Split split(int64_t rows, int64_t vocab, int dtype) {
     p.fine = most <= 64 * kSegments;
     const int64_t segment = 64 * (p.fine ? 1 : kBatch);
     p.segments = (int32_t)((most + segment - 1) / segment);
+    if (way == Way::one) return p;
     const int64_t steps = (p.segments + kWaves - 1) / kWaves;  // of a workgroup that has all
     int64_t groups = kWanted / rows;
-    if (groups < kLeastGroups || vocab < kLeastSplit) return p;
     groups = groups < kMostGroups ? groups : kMostGroups;
     groups = groups < steps ? groups : steps;
     p.per_group = (int32_t)((steps + groups - 1) / groups) * kWaves;
@@ -1103,18 +1206,19 @@ Split split(int64_t rows, int64_t vocab, int dtype) {
         return at;
     };
     p.arrivals = take(rows * 16);
-    p.plans = take(rows * (int64_t)sizeof(Plan));
-    p.listed = take(rows * 4);
+    p.kept = take(rows * p.segments * 8);
     p.parts = take(rows * p.groups * (int64_t)sizeof(Part));
     p.sums = take(rows * p.groups * (int64_t)sizeof(Drawn));
-    p.kept = take(rows * p.segments * 8);
+    p.list = take(rows * (way == Way::whole ? p.groups : 1) * kList * 8);
+    if (way == Way::whole) return p;
+    p.plans = take(rows * (int64_t)sizeof(Plan));
+    p.listed = take(rows * 4);
     p.bins = take(rows * p.groups * kBins * 8);
-    p.list = take(rows * kList * 8);
     return p;
 }
 
 template <int DT, int STEPS>
-hipError_t launch_steps(const SampleArgs& a, const Split& p, void* workspace, hipStream_t stream) {
+hipError_t launch_steps(const SampleArgs& a, const Split& p, Way way, void* workspace, hipStream_t stream) {
     const int bits = weight_bits(a.vocab);
     if (p.groups == 1) {
         sample_rows<DT, STEPS><<<dim3((unsigned)a.rows), kThreads, 0, stream>>>(a, bits, p.segments);
@@ -1138,6 +1242,11 @@ hipError_t launch_steps(const SampleArgs& a, const Split& p, void* workspace, hi
     g.kept = (uint64_t*)(ws + p.kept);
     g.list = (uint64_t*)(ws + p.list);
     const dim3 grid((unsigned)(a.rows * p.groups));
+    if (way == Way::whole) {
+        if (a.top_k || a.top_p) sample_parts<DT, STEPS, true><<<grid, kThreads, 0, stream>>>(g);
+        else sample_parts<DT, STEPS, false><<<grid, kThreads, 0, stream>>>(g);
+        return hipGetLastError();
+    }
     sample_look<DT, STEPS><<<grid, kThreads, 0, stream>>>(g);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -1146,13 +1255,20 @@ hipError_t launch_steps(const SampleArgs& a, const Split& p, void* workspace, hi
 }
 template <int DT>
 hipError_t launch(const SampleArgs& a, void* workspace, hipStream_t stream) {
-    const Split p = split(a.rows, a.vocab, a.dtype);
-    return p.fine ? launch_steps<DT, 1>(a, p, workspace, stream) : launch_steps<DT, kBatch>(a, p, workspace, stream);
+    const Way way = way_of(a.rows, a.vocab, a.top_k || a.top_p);
+    const Split p = split(a.rows, a.vocab, a.dtype, way);
+    return p.fine ? launch_steps<DT, 1>(a, p, way, workspace, stream) : launch_steps<DT, kBatch>(a, p, way, workspace, stream);
 }
 
 }  // namespace
 
-size_t sample_workspace(int64_t rows, int64_t vocab, int dtype) { return rows > 0 ? (size_t)split(rows, vocab, dtype).bytes : 0; }
+size_t sample_workspace(int64_t rows, int64_t vocab, int dtype) {
+    if (rows == 0) return 0;
+    // (which filters there are is not known here)
+    const int64_t cut = split(rows, vocab, dtype, way_of(rows, vocab, true)).bytes;
+    const int64_t whole = split(rows, vocab, dtype, way_of(rows, vocab, false)).bytes;
+    return (size_t)(cut > whole ? cut : whole);
+}
 
 hipError_t launch_sample(const SampleArgs& a, void* workspace, hipStream_t stream) {
     if (a.dtype == QK_F32) return launch<QK_F32>(a, workspace, stream);
