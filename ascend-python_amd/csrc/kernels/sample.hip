@@ -15,7 +15,7 @@
 //          list, finds the border in exact sums, the segment in which the drawn number falls, and the token there.
 // A row whose list would be too long, or whose border is not where the histogram put it, is done by one workgroup that finds each border
 // in the logits' bits, eleven at a time.  Rows that fill the card by themselves, and short ones, go through both steps in one workgroup; in
-rows whose look is little beside their draw each workgroup looks at the whole row, and one launch does (way_of).
+// rows whose look is little beside their draw each workgroup looks at the whole row, and one launch does (way_of).
 //
 // What bounds it: one row, the chain of steps (passes over the row, thresholds searched among the logits, a sort, scans): a row of
 // 65536 takes 10 us without filters and 37 with all three, and twice the tokens 12 and 37.  Many rows, the vector units: an exact
